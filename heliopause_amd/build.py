@@ -23,7 +23,7 @@ NODE_INCLUDE = Path(os.environ.get("NODE_INCLUDE", "/usr/include/node"))
 SOURCES = ["q8k.hip", "kquant_matvec.hip", "kquant_wide.hip", "kquant_mfma.hip", "kquant_prefill.hip", "kquant_mid.hip",
            "repack.hip", "topk.hip",
            "geglu.hip", "gguf.hip", "sample.hip", "decode_layer.hip", "attn_prefill.hip", "decode_fused.hip",
-           "capi.hip"]
+           "paged_append.hip", "paged_attn.hip", "packed_attn.hip", "logit_rules.hip", "capi.hip"]
 
 HIPCC = os.environ.get("HIPCC", shutil.which("hipcc") or "/opt/rocm/bin/hipcc")
 ARCH = "gfx950"

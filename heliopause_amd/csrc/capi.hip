@@ -12,6 +12,7 @@
 #include "hp_fused.h"
 #include "hp_mid_policy.h"
 #include "hp_scratch.h"
+#include "hp_serving.h"
 
 #include <algorithm>
 #include <atomic>
@@ -20,6 +21,7 @@
 #include <cmath>
 #include <map>
 #include <mutex>
+#include <new>
 #include <string>
 #include <thread>
 #include <vector>
@@ -2811,6 +2813,336 @@ int32_t hp_hip_decode_fused_status(void *stream) {
   HP_HIP_TRY(hipMemcpy(&ctl->status, &zero, sizeof(zero), hipMemcpyHostToDevice));
   return fail(HP_ERR_HIP, "persistent decode step: a stage waited past its time limit (status " +
                               std::to_string(status) + "); outputs of the failed steps are invalid");
+}
+
+}  // extern "C"
+
+// ---- several sequences at once -------------------------------------------
+
+namespace {
+
+// The library's device as the current one for as long as it lives (a caller
+// may have another).
+class OnDevice {
+ public:
+  explicit OnDevice(int device) {
+    if (hipGetDevice(&before_) != hipSuccess) before_ = device;
+    if (before_ != device) (void)hipSetDevice(device);
+    changed_ = before_ != device;
+  }
+  ~OnDevice() {
+    if (changed_) (void)hipSetDevice(before_);
+  }
+  OnDevice(const OnDevice &) = delete;
+  OnDevice &operator=(const OnDevice &) = delete;
+
+ private:
+  int before_ = 0;
+  bool changed_ = false;
+};
+
+// Checks that need no device, then `run` on the library's device under its
+// lock.  No exception leaves a C entry point.
+template <class Check, class Run>
+int32_t serving_call(void *stream, Check check, Run run) {
+  try {
+    State &s = st();
+    std::lock_guard<std::recursive_mutex> lock(s.mu);
+    int32_t rc = check();
+    if (rc != HP_OK) return rc;
+    if (stream == reinterpret_cast<void *>(hipStreamPerThread))
+      return fail(HP_ERR_ARG, "hipStreamPerThread is not one stream; pass a stream or NULL");
+    rc = ensure_init(s.ready ? s.device : 0);
+    if (rc != HP_OK) return rc;
+    OnDevice on(s.device);
+    return run(s, stream ? static_cast<hipStream_t>(stream) : s.stream);
+  } catch (const std::bad_alloc &) {
+    return HP_ERR_OOM;
+  } catch (...) {
+    return HP_ERR_HIP;
+  }
+}
+
+bool aligned16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+bool activation_type(int32_t t) { return t == HP_ELEM_F32 || t == HP_ELEM_F16 || t == HP_ELEM_BF16; }
+bool positive(double v) { return std::isfinite(v) && v > 0.0; }
+
+// A stride of `rows` rows in elements of `bytes` each: 0 stands for `dense`;
+// rows do not overlap, start at 16-byte boundaries and end within an address
+// space (so that the kernels' 64-bit offsets do).
+int32_t row_stride(size_t given, size_t dense, int bytes, size_t rows, int64_t *out) {
+  const size_t v = given ? given : dense;
+  if (v < dense || sat_mul(sat_mul(v, rows ? rows : 1), bytes) >> 47)
+    return fail(HP_ERR_SHAPE, "a stride is shorter than its row, or out of range");
+  if (v * bytes % 16 != 0) return fail(HP_ERR_ARG, "strides must be multiples of 16 bytes");
+  *out = (int64_t)v;
+  return HP_OK;
+}
+
+int32_t head_dim_check(int32_t head_dim) {
+  return head_dim == 64 || head_dim == 128 || head_dim == 256 ? HP_OK
+                                                              : fail(HP_ERR_SHAPE, "head_dim must be 64, 128 or 256");
+}
+
+int32_t heads_check(int32_t head_count, int32_t head_count_kv) {
+  if (head_count < 1 || head_count > 65535 || head_count_kv < 1 || head_count % head_count_kv != 0)
+    return fail(HP_ERR_HEADS, "head_count must be a positive multiple of head_count_kv, up to 65535");
+  return HP_OK;
+}
+
+int32_t paged_cache_check(const hp_hip_paged_cache_t *c, PagedCache *out) {
+  if (!c) return fail(HP_ERR_ARG, "null pointer");
+  if (c->type != HP_ELEM_F16 && c->type != HP_ELEM_BF16 && c->type != HP_ELEM_E4M3)
+    return fail(HP_ERR_TYPE, "cache pages are f16, bf16 or e4m3");
+  int32_t rc = head_dim_check(c->head_dim);
+  if (rc != HP_OK) return rc;
+  if (c->head_count_kv < 1 || c->head_count_kv > 65535) return fail(HP_ERR_HEADS, "head_count_kv must be 1..65535");
+  if (c->page_size < 16 || c->page_size > 4096 || (c->page_size & (c->page_size - 1)) != 0)
+    return fail(HP_ERR_SHAPE, "page_size must be a power of two, 16..4096");
+  if (c->page_count < 1) return fail(HP_ERR_SHAPE, "page_count must be positive");
+  if (c->sequence_count < 0 || c->sequence_count > 65535) return fail(HP_ERR_SHAPE, "sequence_count must be 0..65535");
+  if (c->pages_per_sequence < 1 || (int64_t)c->pages_per_sequence * c->page_size > (1 << 30))
+    return fail(HP_ERR_SHAPE, "pages_per_sequence * page_size must be 1..2^30");
+  if (c->type == HP_ELEM_E4M3 && (!positive(c->key_scale) || !positive(c->value_scale)))
+    return fail(HP_ERR_ARG, "the scales of an e4m3 cache must be finite and positive");
+  int64_t stride = 0;
+  rc = row_stride(c->page_stride, (size_t)c->head_count_kv * c->page_size * c->head_dim, elem_bytes(c->type),
+                  (size_t)c->page_count, &stride);
+  if (rc != HP_OK) return rc;
+  if (!c->d_keys || !c->d_values || !c->d_pages || !c->d_lengths) return fail(HP_ERR_ARG, "null pointer");
+  if (!aligned16(c->d_keys) || !aligned16(c->d_values)) return fail(HP_ERR_ARG, "pages must start at 16-byte boundaries");
+  const bool e4m3 = c->type == HP_ELEM_E4M3;
+  *out = PagedCache{c->d_keys,
+                    c->d_values,
+                    c->d_pages,
+                    c->d_lengths,
+                    stride,
+                    c->type,
+                    c->head_dim,
+                    c->head_count_kv,
+                    c->page_count,
+                    __builtin_ctz((unsigned)c->page_size),
+                    c->sequence_count,
+                    c->pages_per_sequence,
+                    e4m3 ? c->key_scale : 1.0f,
+                    e4m3 ? c->value_scale : 1.0f};
+  return HP_OK;
+}
+
+int32_t paged_append_check(const hp_hip_paged_cache_t *cache, const hp_hip_paged_append_t *p, PagedAppendArgs *a) {
+  if (!p) return fail(HP_ERR_ARG, "null pointer");
+  int32_t rc = paged_cache_check(cache, &a->c);
+  if (rc != HP_OK) return rc;
+  if (!activation_type(p->out_type)) return fail(HP_ERR_TYPE, "outputs are f32, f16 or bf16");
+  if (p->d_q || p->head_count != 0) rc = heads_check(p->head_count, a->c.nkv);
+  if (rc != HP_OK) return rc;
+  if (p->rope_dims < 0 || p->rope_dims % 8 != 0 || p->rope_dims > a->c.head_dim)
+    return fail(HP_ERR_SHAPE, "rope_dims must be a multiple of 8 up to head_dim");
+  if (p->rope_dims > 0 && !positive(p->rope_freq_base)) return fail(HP_ERR_ARG, "rope_freq_base must be finite and positive");
+  if (!std::isfinite(p->epsilon) || p->epsilon < 0.0) return fail(HP_ERR_ARG, "epsilon must be finite and not negative");
+  if (p->token_count > (1u << 30)) return fail(HP_ERR_SHAPE, "too many tokens");
+  if (!p->d_offsets && p->token_count != (size_t)a->c.sequences)
+    return fail(HP_ERR_SHAPE, "without offsets there is one token a sequence");
+  if (a->c.sequences == 0 || p->token_count == 0) return HP_OK;
+  if ((p->head_count > 0 && (!p->d_q || !p->d_q_out)) || !p->d_k) return fail(HP_ERR_ARG, "null pointer");
+  for (const void *ptr : {(const void *)p->d_q, (const void *)p->d_k, (const void *)p->d_v, (const void *)p->d_q_out,
+                          (const void *)p->d_k_out, (const void *)p->d_v_out})
+    if (!aligned16(ptr)) return fail(HP_ERR_ARG, "rows must start at 16-byte boundaries");
+  const size_t kv_row = (size_t)a->c.nkv * a->c.head_dim, q_row = (size_t)p->head_count * a->c.head_dim;
+  if ((rc = row_stride(p->q_stride, q_row, 4, p->token_count, &a->q_stride)) != HP_OK) return rc;
+  if ((rc = row_stride(p->k_stride, kv_row, 4, p->token_count, &a->k_stride)) != HP_OK) return rc;
+  if ((rc = row_stride(p->v_stride, kv_row, 4, p->token_count, &a->v_stride)) != HP_OK) return rc;
+  a->q = p->d_q;
+  a->k = p->d_k;
+  a->v = p->d_v;
+  a->offsets = p->d_offsets;
+  a->q_norm = p->d_q_norm;
+  a->k_norm = p->d_k_norm;
+  a->freq_factors = p->d_rope_freq_factors;
+  a->q_out = p->d_q_out;
+  a->k_out = p->d_k_out;
+  a->v_out = p->d_v_out;
+  a->tokens = (int)p->token_count;
+  a->nq = p->head_count;
+  a->out_type = p->out_type;
+  a->norm_values = p->norm_values != 0;
+  a->rope_dims = p->rope_dims;
+  a->eps = (float)p->epsilon;
+  a->log2_base = p->rope_dims > 0 ? std::log2(p->rope_freq_base) : 0.0;
+  return HP_OK;
+}
+
+int32_t paged_attention_check(const hp_hip_paged_cache_t *cache, const hp_hip_paged_attention_t *p, PagedAttnArgs *a) {
+  if (!p) return fail(HP_ERR_ARG, "null pointer");
+  int32_t rc = paged_cache_check(cache, &a->c);
+  if (rc == HP_OK) rc = heads_check(p->head_count, a->c.nkv);
+  if (rc != HP_OK) return rc;
+  if (!activation_type(p->q_type) || !activation_type(p->out_type))
+    return fail(HP_ERR_TYPE, "queries and outputs are f32, f16 or bf16");
+  if (!positive(p->scale)) return fail(HP_ERR_ARG, "scale must be finite and positive");
+  if (p->sliding_window < 0) return fail(HP_ERR_ARG, "sliding_window must not be negative");
+  const size_t row = (size_t)p->head_count * a->c.head_dim;
+  if ((rc = row_stride(p->q_stride, row, elem_bytes(p->q_type), a->c.sequences, &a->q_stride)) != HP_OK) return rc;
+  if ((rc = row_stride(p->output_stride, row, elem_bytes(p->out_type), a->c.sequences, &a->out_stride)) != HP_OK) return rc;
+  if (a->c.sequences == 0) return HP_OK;
+  if (!p->d_q || !p->d_output) return fail(HP_ERR_ARG, "null pointer");
+  if (!aligned16(p->d_q) || !aligned16(p->d_output)) return fail(HP_ERR_ARG, "rows must start at 16-byte boundaries");
+  a->q = p->d_q;
+  a->out = p->d_output;
+  a->nq = p->head_count;
+  a->q_type = p->q_type;
+  a->out_type = p->out_type;
+  a->window = p->sliding_window;
+  a->scale = p->scale;
+  if (paged_attn_most_steps(*a) >> 31)
+    return fail(HP_ERR_SHAPE, "sequences * heads * table positions are more than the kernel counts");
+  return HP_OK;
+}
+
+int32_t packed_attention_check(const hp_hip_packed_attention_t *p, PackedAttnArgs *a) {
+  if (!p) return fail(HP_ERR_ARG, "null pointer");
+  if (p->type != HP_ELEM_F16 && p->type != HP_ELEM_BF16) return fail(HP_ERR_TYPE, "queries, keys and values are f16 or bf16");
+  if (!activation_type(p->out_type)) return fail(HP_ERR_TYPE, "outputs are f32, f16 or bf16");
+  int32_t rc = head_dim_check(p->head_dim);
+  if (rc == HP_OK) rc = heads_check(p->head_count, p->head_count_kv);
+  if (rc != HP_OK) return rc;
+  if (!positive(p->scale)) return fail(HP_ERR_ARG, "scale must be finite and positive");
+  if (p->sliding_window < 0) return fail(HP_ERR_ARG, "sliding_window must not be negative");
+  if (p->sequence_count < 0 || p->sequence_count > (1 << 20)) return fail(HP_ERR_SHAPE, "sequence_count must be 0..2^20");
+  if (p->token_count > (1u << 30)) return fail(HP_ERR_SHAPE, "too many tokens");
+  const size_t q_row = (size_t)p->head_count * p->head_dim, kv_row = (size_t)p->head_count_kv * p->head_dim;
+  if ((rc = row_stride(p->q_stride, q_row, 2, p->token_count, &a->q_stride)) != HP_OK) return rc;
+  if ((rc = row_stride(p->k_stride, kv_row, 2, p->token_count, &a->k_stride)) != HP_OK) return rc;
+  if ((rc = row_stride(p->v_stride, kv_row, 2, p->token_count, &a->v_stride)) != HP_OK) return rc;
+  if ((rc = row_stride(p->output_stride, q_row, elem_bytes(p->out_type), p->token_count, &a->out_stride)) != HP_OK) return rc;
+  a->sequences = p->sequence_count;
+  a->tokens = (int)p->token_count;
+  a->nq = p->head_count;
+  a->nkv = p->head_count_kv;
+  a->head_dim = p->head_dim;
+  if (a->sequences == 0 || a->tokens == 0) return HP_OK;
+  if (!packed_attn_fits(*a)) return fail(HP_ERR_SHAPE, "too many tokens and heads for one launch");
+  if (!p->d_q || !p->d_k || !p->d_v || !p->d_output || !p->d_offsets) return fail(HP_ERR_ARG, "null pointer");
+  if (!aligned16(p->d_q) || !aligned16(p->d_k) || !aligned16(p->d_v) || !aligned16(p->d_output))
+    return fail(HP_ERR_ARG, "rows must start at 16-byte boundaries");
+  a->q = p->d_q;
+  a->k = p->d_k;
+  a->v = p->d_v;
+  a->out = p->d_output;
+  a->offsets = p->d_offsets;
+  a->type = p->type;
+  a->out_type = p->out_type;
+  a->window = p->sliding_window;
+  a->scale = p->scale;
+  return HP_OK;
+}
+
+int32_t logit_rules_check(const hp_hip_logit_rules_t *p, LogitRulesArgs *a) {
+  if (!p) return fail(HP_ERR_ARG, "null pointer");
+  constexpr size_t most = 1u << 30;
+  if (p->rows > 65535) return fail(HP_ERR_SHAPE, "too many rows");
+  if (p->n < 1 || p->n > most) return fail(HP_ERR_SHAPE, "n must be 1..2^30");
+  if (p->history_stride > most || p->bias_stride > most) return fail(HP_ERR_SHAPE, "a list is too long");
+  const size_t words = (p->n + 31) / 32;
+  const size_t logits = p->logits_stride ? p->logits_stride : p->n, output = p->output_stride ? p->output_stride : p->n;
+  const size_t allowed = p->allowed_stride ? p->allowed_stride : words;
+  if (logits < p->n || output < p->n || allowed < words || (logits | output | allowed) >> 32)
+    return fail(HP_ERR_SHAPE, "a stride is shorter than its row, or out of range");
+  if (p->rows == 0) return HP_OK;
+  if (!p->d_logits || !p->d_output || !p->d_history != !p->d_history_lengths || !p->d_bias_ids != !p->d_bias_values ||
+      !p->d_bias_ids != !p->d_bias_counts)
+    return fail(HP_ERR_ARG, "null pointer");
+  if (p->d_output == p->d_logits && logits != output) return fail(HP_ERR_ARG, "in place, both strides are the same");
+  for (const void *ptr : {(const void *)p->d_logits, (const void *)p->d_output, (const void *)p->d_history,
+                          (const void *)p->d_bias_ids, (const void *)p->d_bias_values, (const void *)p->d_allowed})
+    if (reinterpret_cast<uintptr_t>(ptr) % 4 != 0) return fail(HP_ERR_ARG, "misaligned pointer");
+  *a = LogitRulesArgs{p->d_logits,
+                      p->d_output,
+                      p->d_history,
+                      p->d_history_lengths,
+                      p->d_prompt_lengths,
+                      p->d_repetition,
+                      p->d_frequency,
+                      p->d_presence,
+                      p->d_bias_ids,
+                      p->d_bias_counts,
+                      p->d_bias_values,
+                      p->d_allowed,
+                      (int64_t)logits,
+                      (int64_t)output,
+                      (int64_t)p->history_stride,
+                      (int64_t)p->bias_stride,
+                      (int64_t)allowed,
+                      (int)p->rows,
+                      (int)p->n};
+  return HP_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int32_t hp_hip_paged_append_device(const hp_hip_paged_cache_t *cache, const hp_hip_paged_append_t *append,
+                                   void *stream) {
+  PagedAppendArgs a{};
+  return serving_call(
+      stream, [&] { return paged_append_check(cache, append, &a); },
+      [&](State &s, hipStream_t strm) -> int32_t {
+        if (a.c.sequences == 0 || a.tokens == 0) return HP_OK;
+        hipEvent_t e = prof_begin(strm);
+        HP_HIP_TRY(launch_paged_append(a, s.num_cus, strm));
+        prof_end(HP_KERNEL_ATTENTION, e, strm);
+        s.launches++;
+        return HP_OK;
+      });
+}
+
+int32_t hp_hip_paged_attention_device(const hp_hip_paged_cache_t *cache, const hp_hip_paged_attention_t *attention,
+                                      void *stream) {
+  PagedAttnArgs a{};
+  return serving_call(
+      stream, [&] { return paged_attention_check(cache, attention, &a); },
+      [&](State &s, hipStream_t strm) -> int32_t {
+        if (a.c.sequences == 0) return HP_OK;
+        const int groups = paged_attn_groups(a, s.num_cus);
+        void *scratch = nullptr;
+        int32_t rc = stream_scratch(strm, kScratchPaged, paged_attn_scratch_bytes(a, groups), &scratch);
+        if (rc != HP_OK) return rc;
+        a.partials = static_cast<float *>(scratch);
+        hipEvent_t e = prof_begin(strm);
+        HP_HIP_TRY(launch_paged_attn(a, groups, strm));
+        prof_end(HP_KERNEL_ATTENTION, e, strm);
+        s.launches += 2;
+        return HP_OK;
+      });
+}
+
+int32_t hp_hip_packed_attention_device(const hp_hip_packed_attention_t *attention, void *stream) {
+  PackedAttnArgs a{};
+  return serving_call(
+      stream, [&] { return packed_attention_check(attention, &a); },
+      [&](State &s, hipStream_t strm) -> int32_t {
+        if (a.sequences == 0 || a.tokens == 0) return HP_OK;
+        hipEvent_t e = prof_begin(strm);
+        HP_HIP_TRY(launch_packed_attn(a, strm));
+        prof_end(HP_KERNEL_ATTENTION, e, strm);
+        s.launches++;
+        return HP_OK;
+      });
+}
+
+int32_t hp_hip_logit_rules_device(const hp_hip_logit_rules_t *rules, void *stream) {
+  LogitRulesArgs a{};
+  return serving_call(
+      stream, [&] { return logit_rules_check(rules, &a); },
+      [&](State &s, hipStream_t strm) -> int32_t {
+        if (a.rows == 0) return HP_OK;
+        hipEvent_t e = prof_begin(strm);
+        HP_HIP_TRY(launch_logit_rules(a, s.num_cus, strm));
+        prof_end(HP_KERNEL_SAMPLE, e, strm);
+        s.launches++;
+        return HP_OK;
+      });
 }
 
 }  // extern "C"

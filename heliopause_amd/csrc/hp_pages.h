@@ -1,0 +1,64 @@
+// hp_pages.h -- where the operators over several sequences find things: a
+// position's page, a sequence's keys, the split of a batch's steps over
+// workgroups, a packed block's sequence.  Plain integer rules without a device
+// header, so that the CPU tests walk them over bad tables and odd batches
+// before a kernel does.
+#pragma once
+
+#include <stdint.h>
+
+#if defined(__HIPCC__)
+#define HP_PAGES_FN __host__ __device__ __forceinline__
+#else
+#define HP_PAGES_FN static inline
+#endif
+
+namespace hp {
+
+// The page that a table's entry names, or -1.
+HP_PAGES_FN int page_or_none(int entry, int page_count) { return entry >= 0 && entry < page_count ? entry : -1; }
+
+// Position of the token `behind` places before the end of a sequence of
+// `length` tokens (1: the last), or -1 where the table of `width` pages has
+// no place for it.
+HP_PAGES_FN int append_position(int length, int64_t behind, int page_shift, int width) {
+  const int64_t p = (int64_t)length - behind;
+  return p >= 0 && (p >> page_shift) < width ? (int)p : -1;
+}
+
+constexpr int kPagedSub = 32;                // keys of a wave's step of the paged attention
+constexpr int kPagedWaves = 4;
+constexpr int kPagedStep = kPagedSub * kPagedWaves;
+
+// A sequence's keys first .. end - 1, and where the walk over them begins: at
+// a multiple of 16, so that 16 keys on end share a page.
+struct KeySpan {
+  int first, begin, end;
+};
+HP_PAGES_FN KeySpan key_span(int length, int64_t table_keys, int window) {
+  KeySpan s;
+  s.end = length < 0 ? 0 : length < table_keys ? length : (int)table_keys;
+  s.first = window > 0 && s.end > window ? s.end - window : 0;
+  s.begin = s.first & ~15;
+  return s;
+}
+HP_PAGES_FN uint32_t span_steps(const KeySpan &s) { return (uint32_t)((s.end - s.begin + kPagedStep - 1) / kPagedStep); }
+
+// Share i of `shares` (<= total) of the steps 0 .. total - 1 begins here, and
+// the share that step t is in.
+HP_PAGES_FN uint32_t share_begin(uint32_t total, uint32_t i, uint32_t shares) {
+  return (uint32_t)((uint64_t)total * i / shares);
+}
+HP_PAGES_FN uint32_t share_of(uint32_t total, uint32_t t, uint32_t shares) {
+  return (uint32_t)((((uint64_t)t + 1) * shares - 1) / total);
+}
+
+constexpr int kPackedRows = 128;  // query rows of a workgroup of the packed attention
+
+// Sequence s of a packed batch has the blocks from this one up to the next
+// sequence's: at least as many as its rows fill, with no sum over the
+// sequences before it.
+HP_PAGES_FN int64_t packed_first_block(int offset, int s) { return (offset > 0 ? offset : 0) / kPackedRows + (int64_t)s; }
+HP_PAGES_FN int64_t packed_blocks(int64_t tokens, int64_t sequences) { return tokens / kPackedRows + 1 + sequences; }
+
+}  // namespace hp

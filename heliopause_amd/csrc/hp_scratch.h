@@ -42,7 +42,8 @@ enum ScratchKind {
   kScratchGeglu = 4,    // gate and up sums ahead of a GeGLU launch
   kScratchParts = 5,    // block-range sums of a prefill launch that a norm launch adds
   kScratchFused = 6,    // exchange arena and control words of the persistent decode step (zeroed when allocated)
-  kScratchKinds = 7
+  kScratchPaged = 7,    // row parts of the paged attention
+  kScratchKinds = 8
 };
 
 enum ScratchStatus { kScratchOk = 0, kScratchCapturing = 1, kScratchNoMemory = 2, kScratchZeroFailed = 3 };

@@ -1,0 +1,594 @@
+// paged_attn.hip -- attention of one new token of every sequence over its
+// pages: out_h = sum_j p_j v_j / sum_j p_j with p_j = exp(scale q_h . k_j - m)
+// over the last min(length, window) positions j of the sequence.
+//
+// Every key and value is read once per KV head for all query heads of its
+// group, so 2 (group) flop come on each 16-bit byte pair: the cache's bytes
+// bound it, and the matrix cores, which a group of eight leaves at a few
+// percent, are used because they hand every key to all heads of the group at
+// once and leave the vector unit free.
+//
+// Products.  A wave takes 32 keys at a time, v_mfma_f32_16x16x32:
+//   scores S^T = K Q^T, keys as the A rows, straight from the cache rows (a
+//     lane's 8 consecutive elements of one key).  The B columns are the eight
+//     query heads twice: column c < 8 holds the upper part of head c's query,
+//     column c + 8 the rest of it, so one product gives both and their sum is
+//     the score of the query to 22 bits (f16) or 16 (bf16; a query that came
+//     as f32 has a third part there, in a second product into the same sums);
+//   values O^T += V^T P^T, the lane's own scores as the B operand: lane (q4,
+//     c) holds the scores of keys 4 q4 .. + 3 of both 16-key halves, and the
+//     product's k index runs over just those, so the probabilities never
+//     leave their registers; columns c and c + 8 hold the upper part and the
+//     rest of p.  V^T's row index runs over the 16 lanes of a row, each with
+//     D / 16 consecutive elements of a value row: 16 lanes load whole rows and
+//     turn 8 keys x D / 16 elements into fragments with byte permutes.
+// So results are those of f32 arithmetic to a few 2^-22 (f16, e4m3) or 2^-16
+// (bf16) though the operands have 16 bits; sums, maximum and normaliser are
+// f32.  p carries a factor 2^10, which cancels: it keeps p of 2^-24 and less
+// out of f16's subnormal steps.  E4M3 elements become f16 exactly, and the
+// cache's scales join the score's factor and the end.
+//
+// Masked keys (behind the length, before the window, on an absent page) get
+// score -inf and value zero, whatever their slots hold.
+//
+// Split.  All (sequence, KV head, eight query heads) rows' steps of 128 keys
+// (32 for each of the four waves) lie end to end, and each workgroup takes an
+// equal share of that line, whatever the lengths are: 48 ragged contexts and
+// two of 131072 fill the card alike, and a captured launch serves every batch.
+// A workgroup finds its place by a scan of the lengths.  A row that one
+// workgroup finishes is written at once; parts of the others go to scratch,
+// at most two a workgroup, and the merge launch joins them in their order.
+#include "hp_mfma.h"
+#include "hp_serving.h"
+#include "hp_wave.h"
+
+namespace hp {
+
+namespace {
+
+constexpr int kWaves = kPagedWaves, kThreads = 64 * kWaves;
+constexpr int kHeads = 8;  // query heads of a row
+constexpr int kSub = kPagedSub, kStep = kPagedStep;
+constexpr float kLog2e = 1.44269504088896341f;
+constexpr float kBias = 10.0f;  // p carries 2^kBias
+constexpr float kNegInf = -__builtin_inff();
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ KeySpan span_of(const PagedAttnArgs &a, int seq) {
+  return key_span(a.c.lengths[seq], (int64_t)a.c.width << a.c.page_shift, a.window);
+}
+
+// Heads of a KV head's group in blocks of kHeads: rows of a sequence.
+__host__ __device__ __forceinline__ int blocks_of(int nq, int nkv) { return (nq / nkv + kHeads - 1) / kHeads; }
+
+// A part of a row: m and l of its heads, then the unnormalised sums.
+template <int D>
+struct Part {
+  float m[kHeads], l[kHeads];
+  float o[kHeads][D];
+};
+struct RowParts {
+  int first, last;  // workgroups that hold the row's parts (the same: none)
+};
+
+template <int CT>
+__device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
+  if (CT == kElemBf16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
+}
+
+// The operand type's bits of v, and the value they stand for.
+template <int CT>
+__device__ __forceinline__ uint32_t part_bits(float v) {
+  return CT == kElemBf16 ? bf16_bits(v) : f16_bits(v);
+}
+template <int CT>
+__device__ __forceinline__ float part_value(uint32_t b) {
+  return CT == kElemBf16 ? bf16_value(b) : (float)__builtin_bit_cast(_Float16, (uint16_t)b);
+}
+
+// Bytes 2 i, 2 i + 1 of four fp8 values as two halves (exact: f16 holds every
+// e4m3 value).  The results are taken as one dword; a bit cast of a vector's
+// element reads element 0.
+template <bool HI>
+__device__ __forceinline__ uint32_t halves_of_e4m3(uint32_t w) {
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, HI));
+}
+
+// maximum / sum over the lanes c, c + 16, c + 32, c + 48
+__device__ __forceinline__ float column_max(float v) {
+  v = fmaxf(v, __shfl_xor(v, 16));
+  return fmaxf(v, __shfl_xor(v, 32));
+}
+__device__ __forceinline__ float column_sum(float v) {
+  v += __shfl_xor(v, 16);
+  return v + __shfl_xor(v, 32);
+}
+
+// A lane's elements of a key tile's row (D / 32 operand fragments) and of the
+// eight value rows (D / 16 elements each), as loaded.
+template <int D, int CT>
+struct Tile {
+  static constexpr int kE = CT == kElemE4m3 ? 1 : 2;   // bytes an element
+  static constexpr int kKeyWords = D * kE / 4 / 4;     // dwords of a quarter key row
+  static constexpr int kValueWords = D * kE / 16 / 4;  // dwords of a sixteenth of a value row
+  uint32_t k[2][kKeyWords];
+  uint32_t v[8][kValueWords];
+};
+
+template <int N>
+__device__ __forceinline__ void load_words(uint32_t (&d)[N], const uint8_t *p) {
+  if (N == 1) {
+    d[0] = *reinterpret_cast<const uint32_t *>(p);
+  } else if (N == 2) {
+    const uint2 w = *reinterpret_cast<const uint2 *>(p);
+    d[0] = w.x;
+    d[1 % N] = w.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      const uint4 w = *reinterpret_cast<const uint4 *>(p + 4 * i);
+      d[i] = w.x;
+      d[(i + 1) % N] = w.y;
+      d[(i + 2) % N] = w.z;
+      d[(i + 3) % N] = w.w;
+    }
+  }
+}
+
+template <int D, int CT, bool THIRD>
+__global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(const PagedAttnArgs a, RowParts *__restrict__ rows,
+                                                                 Part<D> *__restrict__ parts) {
+  using T = Tile<D, CT>;
+  constexpr int kE = T::kE, kFrags = D / 32, kRowBytes = D * kE, kT = D / 16;
+  __shared__ float4 sh_o[kWaves][kHeads][D / 4];
+  __shared__ float sh_m[kWaves][kHeads], sh_l[kWaves][kHeads];
+  __shared__ uint32_t sh_scan[kWaves];
+  __shared__ int sh_place[3];  // sequence, its first step on the line, the line's length
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int q4 = lane >> 4, c16 = lane & 15;
+  const int group = a.nq / a.c.nkv, blocks = blocks_of(a.nq, a.c.nkv), units = a.c.nkv * blocks;
+
+  // the line of steps: each thread sums a run of sequences, then the runs are
+  // scanned
+  const int run = (a.c.sequences + kThreads - 1) / kThreads;
+  uint32_t mine = 0;
+  for (int i = 0; i < run; i++) {
+    const int s = tid * run + i;
+    if (s < a.c.sequences) mine += span_steps(span_of(a, s));
+  }
+  uint32_t before = mine;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const uint32_t up = __shfl_up(before, o);
+    if (lane >= o) before += up;
+  }
+  if (lane == 63) sh_scan[wave] = before;
+  __syncthreads();
+  uint32_t total = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; w++) {
+    if (w < wave) before += sh_scan[w];
+    total += sh_scan[w];
+  }
+  before -= mine;
+  total *= units;
+  before *= units;
+  mine *= units;
+  const uint32_t shares = min((uint32_t)gridDim.x, total), me = blockIdx.x;
+  if (me >= shares) return;
+  uint32_t at = share_begin(total, me, shares);
+  const uint32_t stop = share_begin(total, me + 1, shares);
+  if (at >= before && at - before < mine) {  // one thread
+    int s = tid * run;
+    uint32_t start = before;
+    for (;; s++) {
+      const uint32_t n = span_steps(span_of(a, s)) * units;
+      if (at - start < n) break;
+      start += n;
+    }
+    sh_place[0] = s;
+    sh_place[1] = (int)start;
+  }
+  __syncthreads();
+  int seq = sh_place[0];
+  uint32_t seq_start = (uint32_t)sh_place[1];
+
+  const uint8_t *keys = static_cast<const uint8_t *>(a.c.keys), *values = static_cast<const uint8_t *>(a.c.values);
+  const int page_mask = (1 << a.c.page_shift) - 1;
+
+  while (at < stop) {
+    const KeySpan span = span_of(a, seq);
+    const uint32_t steps = span_steps(span);
+    if (at - seq_start >= steps * units) {  // (also past sequences without a key)
+      seq_start += steps * units;
+      seq++;
+      continue;
+    }
+    const uint32_t unit = (at - seq_start) / steps, row_start = seq_start + unit * steps;
+    const uint32_t i0 = at - row_start, n = min(stop - at, steps - i0);
+    const int kvh = unit / blocks, h0 = (unit - kvh * blocks) * kHeads;  // KV head, first head of the group
+    const int live = min(kHeads, group - h0);
+
+    // the query: row c16 % 8's elements, in parts
+    u32x4 qa[kFrags], qb[THIRD ? kFrags : 1];
+    float factor;  // of a score, to base 2
+    {
+      const int c = c16 & 7;
+      const int64_t at_q = seq * a.q_stride + (int64_t)(kvh * group + h0 + min(c, live - 1)) * D;
+      float x[kFrags][8], most = 0.0f;
+#pragma unroll
+      for (int f = 0; f < kFrags; f++) {
+        // element j of fragment f: where the lane's keys have theirs
+        const int d = CT == kElemE4m3 ? 64 * (f >> 1) + 16 * q4 + 8 * (f & 1) : 32 * f + 8 * q4;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+          const float v = load_elem(a.q, at_q + d + j, a.q_type);
+          x[f][j] = c < live ? v : 0.0f;
+          most = fmaxf(most, fabsf(x[f][j]));
+        }
+      }
+      most = column_max(most);
+      // the row times the power of two that puts its largest element into
+      // [16, 32): the parts' range is then no concern (not for zeros and
+      // infinities, which stay)
+      const int e = (int)(__builtin_bit_cast(uint32_t, most) >> 23) - 127;
+      const int shift = most > 0.0f && e < 128 ? 4 - max(e, -100) : 0;
+      const float up = __builtin_bit_cast(float, (uint32_t)(127 + shift) << 23);
+      factor = a.scale * (CT == kElemE4m3 ? a.c.key_scale : 1.0f) * kLog2e / up;
+      const bool rest = c16 >= kHeads;
+#pragma unroll
+      for (int f = 0; f < kFrags; f++) {
+        uint32_t p0[8], p2[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+          const float v = x[f][j] * up;
+          const uint32_t hi = part_bits<CT>(v);
+          const float r1 = v - part_value<CT>(hi);
+          const uint32_t mid = part_bits<CT>(r1);
+          p0[j] = rest ? mid : hi;
+          p2[j] = rest ? 0u : part_bits<CT>(r1 - part_value<CT>(mid));
+        }
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+          qa[f][w] = p0[2 * w] | p0[2 * w + 1] << 16;
+          if (THIRD) qb[THIRD ? f : 0][w] = p2[2 * w] | p2[2 * w + 1] << 16;
+        }
+      }
+    }
+
+    f32x4 acc[kT];
+#pragma unroll
+    for (int t = 0; t < kT; t++) acc[t] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+    float m_run = kNegInf, l_part = 0.0f;
+
+    // this wave's tiles: key .. key + 31 at key = begin + kStep i + kSub wave
+    const int key0 = span.begin + (int)i0 * kStep + kSub * wave;
+    const int key_stop = min(span.end, span.begin + (int)(i0 + n) * kStep);
+    const int *table = a.c.pages + (int64_t)seq * a.c.width;
+    const int64_t head_at = ((int64_t)kvh << a.c.page_shift) * D;
+    // Page of the 16 keys from `key` on (the same for the wave), -1 for none.
+    // Only entries of pages that hold a key of the sequence are read.
+    auto page_of = [&](int key) -> int {
+      if (key >= span.end) return -1;
+      return page_or_none(table[key >> a.c.page_shift], a.c.page_count);
+    };
+    // Bytes of the first of those keys' rows for this head; an absent page's
+    // are page 0's, which are there and masked.
+    auto tile_at = [&](int page, int key) -> int64_t {
+      return (max(page, 0) * a.c.page_stride + head_at + (int64_t)(key & page_mask) * D) * kE;
+    };
+    T t;
+    auto load_keys = [&](int key, int p0, int p1) {
+      const int64_t b0 = tile_at(p0, key), b1 = tile_at(p1, key + 16);
+      if (CT == kElemE4m3) {
+        // 16 bytes are the lane's elements of two fragments
+        constexpr int kN = D / 64;
+#pragma unroll
+        for (int i = 0; i < kN; i++) {
+          const int off = c16 * kRowBytes + 64 * i + 16 * q4;
+          uint32_t w[4];
+          load_words<4>(w, keys + b0 + off);
+#pragma unroll
+          for (int j = 0; j < 4; j++) t.k[0][4 * i + j] = w[j];
+          load_words<4>(w, keys + b1 + off);
+#pragma unroll
+          for (int j = 0; j < 4; j++) t.k[1][4 * i + j] = w[j];
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < kFrags; i++) {
+          const int off = c16 * kRowBytes + 64 * i + 16 * q4;
+          uint32_t w[4];
+          load_words<4>(w, keys + b0 + off);
+#pragma unroll
+          for (int j = 0; j < 4; j++) t.k[0][(4 * i + j) % T::kKeyWords] = w[j];
+          load_words<4>(w, keys + b1 + off);
+#pragma unroll
+          for (int j = 0; j < 4; j++) t.k[1][(4 * i + j) % T::kKeyWords] = w[j];
+        }
+      }
+    };
+    auto load_values = [&](int key, int p0, int p1) {
+      const int64_t b0 = tile_at(p0, key), b1 = tile_at(p1, key + 16);
+#pragma unroll
+      for (int j = 0; j < 8; j++)
+        load_words<T::kValueWords>(t.v[j], values + (j < 4 ? b0 : b1) + (4 * q4 + (j & 3)) * kRowBytes + c16 * kT * kE);
+    };
+
+    int key = key0;
+    if (key < key_stop) {
+      int p0 = page_of(key), p1 = page_of(key + 16);
+      int np0 = page_of(key + kStep), np1 = page_of(key + kStep + 16);
+      load_keys(key, p0, p1);
+      load_values(key, p0, p1);
+      for (; key < key_stop; key += kStep) {
+        const int next = key + kStep;
+        const bool more = next < key_stop;
+        f32x4 s[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+          for (int f = 0; f < kFrags; f++) {
+            u32x4 kf;
+            if (CT == kElemE4m3) {
+              const uint32_t lo = t.k[h][2 * f], hi = t.k[h][2 * f + 1];
+              kf = (u32x4){halves_of_e4m3<false>(lo), halves_of_e4m3<true>(lo), halves_of_e4m3<false>(hi),
+                           halves_of_e4m3<true>(hi)};
+            } else {
+              constexpr int kN = T::kKeyWords;
+              kf = (u32x4){t.k[h][4 * f % kN], t.k[h][(4 * f + 1) % kN], t.k[h][(4 * f + 2) % kN],
+                           t.k[h][(4 * f + 3) % kN]};
+            }
+            s[h] = mfma16<CT>(kf, qa[f], s[h]);
+            if (THIRD) s[h] = mfma16<CT>(kf, qb[THIRD ? f : 0], s[h]);
+          }
+        // the next keys stream in while these are worked on
+        if (more) load_keys(next, np0, np1);
+        const bool edge = key < span.first || key + kSub > span.end || p0 < 0 || p1 < 0;
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+          const float v = s[j >> 2][j & 3];
+          x[j] = (v + dpp_f32<kDppRor8>(v)) * factor;
+        }
+        if (edge) {  // the same for the wave
+#pragma unroll
+          for (int j = 0; j < 8; j++) {
+            const int at_key = key + 16 * (j >> 2) + 4 * q4 + (j & 3);
+            const bool off = at_key < span.first || at_key >= span.end || (j < 4 ? p0 : p1) < 0;
+            x[j] = off ? kNegInf : x[j];
+#pragma unroll
+            for (int w = 0; w < T::kValueWords; w++) t.v[j][w] = off ? 0u : t.v[j][w];
+          }
+        }
+        float most = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+        most = column_max(most);
+        if (__any(most > m_run)) {
+          const float m_new = fmaxf(m_run, most);
+          const float alpha = m_new == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_new);
+          m_run = m_new;
+          l_part *= alpha;
+#pragma unroll
+          for (int i = 0; i < kT; i++) acc[i] *= alpha;
+        }
+        // a row without a key so far: exp2(-inf - 0) = 0
+        const float m_use = m_run == kNegInf ? 0.0f : m_run - kBias;
+        u32x4 pf;
+        const bool rest = c16 >= kHeads;
+        uint32_t pb[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+          const float p = __builtin_amdgcn_exp2f(x[j] - m_use);
+          l_part += p;
+          const uint32_t hi = part_bits<CT>(p), lo = part_bits<CT>(p - part_value<CT>(hi));
+          pb[j] = rest ? lo : hi;
+        }
+#pragma unroll
+        for (int w = 0; w < 4; w++) pf[w] = pb[2 * w] | pb[2 * w + 1] << 16;
+        // V^T fragments: element i of the lane's D / 16 from eight keys
+#pragma unroll
+        for (int i = 0; i < kT; i++) {
+          u32x4 vf;
+#pragma unroll
+          for (int w = 0; w < 4; w++) {
+            const uint32_t sel = (i & 1) ? 0x07060302u : 0x05040100u;
+            if (CT == kElemE4m3) {
+              const uint32_t a0 = t.v[2 * w][i >> 2], a1 = t.v[2 * w + 1][i >> 2];
+              const uint32_t x0 = (i & 2) ? halves_of_e4m3<true>(a0) : halves_of_e4m3<false>(a0);
+              const uint32_t x1 = (i & 2) ? halves_of_e4m3<true>(a1) : halves_of_e4m3<false>(a1);
+              vf[w] = __builtin_amdgcn_perm(x1, x0, sel);
+            } else {
+              constexpr int kN = T::kValueWords;
+              vf[w] = __builtin_amdgcn_perm(t.v[2 * w + 1][(i >> 1) % kN], t.v[2 * w][(i >> 1) % kN], sel);
+            }
+          }
+          acc[i] = mfma16<CT>(vf, pf, acc[i]);
+        }
+        if (more) load_values(next, np0, np1);
+        p0 = np0;
+        p1 = np1;
+        np0 = page_of(next + kStep);
+        np1 = page_of(next + kStep + 16);
+      }
+    }
+
+    // the four waves' parts, joined in LDS.  Lane (q4, c): head c, elements
+    // kT (4 q4 + r) + i
+    const float l_run = column_sum(l_part);
+#pragma unroll
+    for (int i = 0; i < kT; i++)
+#pragma unroll
+      for (int r = 0; r < 4; r++) acc[i][r] += dpp_f32<kDppRor8>(acc[i][r]);
+    if (c16 < kHeads) {
+      if (q4 == 0) {
+        sh_m[wave][c16] = m_run;
+        sh_l[wave][c16] = l_run;
+      }
+#pragma unroll
+      for (int r = 0; r < 4; r++)
+#pragma unroll
+        for (int i = 0; i < kT; i += 4)
+          sh_o[wave][c16][(kT * (4 * q4 + r) + i) / 4] =
+              make_float4(acc[i][r], acc[i + 1][r], acc[i + 2][r], acc[i + 3][r]);
+    }
+    __syncthreads();
+    const bool whole = i0 == 0 && n == steps;
+    Part<D> *part = parts + 2 * (int64_t)me + (i0 == 0 ? 1 : 0);
+    if (i0 == 0 && tid == 0) {
+      rows[(int64_t)seq * units + unit] = RowParts{(int)me, (int)share_of(total, row_start + steps - 1, shares)};
+    }
+    for (int i = tid; i < kHeads * (D / 4); i += kThreads) {
+      const int h = i / (D / 4), d = i - h * (D / 4);
+      float m = kNegInf;
+#pragma unroll
+      for (int w = 0; w < kWaves; w++) m = fmaxf(m, sh_m[w][h]);
+      float l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int w = 0; w < kWaves; w++) {
+        const float mw = sh_m[w][h], f = mw == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(mw - m);
+        const float4 v = sh_o[w][h][d];
+        l += f * sh_l[w][h];
+        o[0] += f * v.x;
+        o[1] += f * v.y;
+        o[2] += f * v.z;
+        o[3] += f * v.w;
+      }
+      if (h >= live) continue;
+      if (whole) {
+        const float inv = l == 0.0f ? 0.0f : (CT == kElemE4m3 ? a.c.value_scale : 1.0f) / l;
+#pragma unroll
+        for (int j = 0; j < 4; j++) o[j] *= inv;
+        store4(a.out, seq * a.out_stride + (int64_t)(kvh * group + h0 + h) * D + 4 * d, a.out_type, o);
+      } else {
+        *reinterpret_cast<float4 *>(&part->o[h][4 * d]) = make_float4(o[0], o[1], o[2], o[3]);
+        if (d == 0) {
+          part->m[h] = m;
+          part->l[h] = l;
+        }
+      }
+    }
+    __syncthreads();  // the LDS is the next row's
+    at += n;
+  }
+}
+
+// One (sequence, head): the parts of its row in order, o = sum f o_c / sum f
+// l_c with f = 2^(m_c - m); D / 4 threads a part, several parts at once.
+template <int D>
+__global__ __launch_bounds__(kThreads) void paged_merge_kernel(const PagedAttnArgs a, const RowParts *__restrict__ rows,
+                                                               const Part<D> *__restrict__ parts) {
+  constexpr int kPer = D / 4, kAtOnce = kThreads / kPer;
+  __shared__ float sh_m[kAtOnce], sh_l[kAtOnce];
+  __shared__ float4 sh_o[kAtOnce][kPer];
+  const int group = a.nq / a.c.nkv, blocks = blocks_of(a.nq, a.c.nkv);
+  const int head = blockIdx.x, seq = blockIdx.y;
+  const int kvh = head / group, in_group = head - kvh * group, h = in_group % kHeads;
+  const int tid = threadIdx.x, sub = tid / kPer, d = tid - sub * kPer;
+  const int64_t out = seq * a.out_stride + (int64_t)head * D + 4 * d;
+  if (span_steps(span_of(a, seq)) == 0) {  // no key: zeros
+    const float zero[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (sub == 0) store4(a.out, out, a.out_type, zero);
+    return;
+  }
+  const RowParts r = rows[((int64_t)seq * a.c.nkv + kvh) * blocks + in_group / kHeads];
+  if (r.first == r.last) return;  // written by the workgroup that had it whole
+  float m = kNegInf, l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int c = r.first + sub; c <= r.last; c += kAtOnce) {
+    const Part<D> &p = parts[2 * (int64_t)c + (c == r.first ? 1 : 0)];
+    const float mc = p.m[h], lc = p.l[h];
+    const float4 v = *reinterpret_cast<const float4 *>(&p.o[h][4 * d]);
+    const float m_new = fmaxf(m, mc);
+    const float f = m == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(m - m_new);
+    const float g = mc == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(mc - m_new);
+    l = l * f + lc * g;
+    o[0] = o[0] * f + v.x * g;
+    o[1] = o[1] * f + v.y * g;
+    o[2] = o[2] * f + v.z * g;
+    o[3] = o[3] * f + v.w * g;
+    m = m_new;
+  }
+  if (d == 0) {
+    sh_m[sub] = m;
+    sh_l[sub] = l;
+  }
+  sh_o[sub][d] = make_float4(o[0], o[1], o[2], o[3]);
+  __syncthreads();
+  if (sub != 0) return;
+  float most = kNegInf;
+#pragma unroll
+  for (int c = 0; c < kAtOnce; c++) most = fmaxf(most, sh_m[c]);
+  l = o[0] = o[1] = o[2] = o[3] = 0.0f;
+#pragma unroll
+  for (int c = 0; c < kAtOnce; c++) {
+    const float f = sh_m[c] == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(sh_m[c] - most);
+    const float4 v = sh_o[c][d];
+    l += f * sh_l[c];
+    o[0] += f * v.x;
+    o[1] += f * v.y;
+    o[2] += f * v.z;
+    o[3] += f * v.w;
+  }
+  const float inv = l == 0.0f ? 0.0f : (a.c.type == kElemE4m3 ? a.c.value_scale : 1.0f) / l;
+#pragma unroll
+  for (int j = 0; j < 4; j++) o[j] *= inv;
+  store4(a.out, out, a.out_type, o);
+}
+
+template <int D, int CT, bool THIRD>
+hipError_t launch(const PagedAttnArgs &a, int groups, hipStream_t s) {
+  const int64_t rows = (int64_t)a.c.sequences * a.c.nkv * blocks_of(a.nq, a.c.nkv);
+  Part<D> *parts = reinterpret_cast<Part<D> *>(a.partials);
+  RowParts *row_parts = reinterpret_cast<RowParts *>(parts + 2 * (int64_t)groups);
+  (void)rows;
+  hipLaunchKernelGGL((paged_attn_kernel<D, CT, THIRD>), dim3(groups), dim3(kThreads), 0, s, a, row_parts, parts);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL(paged_merge_kernel<D>, dim3(a.nq, a.c.sequences), dim3(kThreads), 0, s, a, row_parts, parts);
+  return hipGetLastError();
+}
+
+template <int D>
+hipError_t launch_type(const PagedAttnArgs &a, int groups, hipStream_t s) {
+  if (a.c.type == kElemF16) return launch<D, kElemF16, false>(a, groups, s);
+  if (a.c.type == kElemE4m3) return launch<D, kElemE4m3, false>(a, groups, s);
+  // two bf16 parts hold an f16 or bf16 query; an f32 one has a third
+  return a.q_type == kElemF32 ? launch<D, kElemBf16, true>(a, groups, s) : launch<D, kElemBf16, false>(a, groups, s);
+}
+
+size_t part_bytes(int head_dim) { return (size_t)kHeads * (head_dim + 2) * sizeof(float); }
+
+}  // namespace
+
+uint64_t paged_attn_most_steps(const PagedAttnArgs &a) {
+  uint64_t keys = (uint64_t)a.c.width << a.c.page_shift;
+  if (a.window > 0 && keys > (uint64_t)a.window + 15) keys = (uint64_t)a.window + 15;
+  return (keys + kStep - 1) / kStep * a.c.sequences * a.c.nkv * blocks_of(a.nq, a.c.nkv);
+}
+
+int paged_attn_groups(const PagedAttnArgs &a, int num_cus) {
+  const uint64_t most = paged_attn_most_steps(a);
+  return (int)(most < 2ull * num_cus ? most : 2ull * num_cus);
+}
+
+size_t paged_attn_scratch_bytes(const PagedAttnArgs &a, int groups) {
+  return 2 * (size_t)groups * part_bytes(a.c.head_dim) +
+         (size_t)a.c.sequences * a.c.nkv * blocks_of(a.nq, a.c.nkv) * sizeof(RowParts);
+}
+
+hipError_t launch_paged_attn(const PagedAttnArgs &a, int groups, hipStream_t s) {
+  if (groups < 1 || a.c.sequences < 1 || a.c.nkv < 1 || a.nq % a.c.nkv != 0 || !a.partials ||
+      paged_attn_most_steps(a) >> 31)
+    return hipErrorInvalidValue;
+  switch (a.c.head_dim) {
+    case 64: return launch_type<64>(a, groups, s);
+    case 128: return launch_type<128>(a, groups, s);
+    case 256: return launch_type<256>(a, groups, s);
+    default: return hipErrorInvalidValue;
+  }
+}
+
+}  // namespace hp

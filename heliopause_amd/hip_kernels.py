@@ -158,6 +158,64 @@ def _declare_decode(L: ctypes.CDLL) -> None:
         getattr(L, name).restype = i32
 
 
+class HipPagedCache(ctypes.Structure):
+    """hp_hip_paged_cache_t: a pool of pages and what a batch's sequences hold in it."""
+    _fields_ = [("d_keys", ctypes.c_void_p), ("d_values", ctypes.c_void_p), ("type", ctypes.c_int32),
+                ("head_dim", ctypes.c_int32), ("head_count_kv", ctypes.c_int32), ("page_size", ctypes.c_int32),
+                ("page_count", ctypes.c_int32), ("sequence_count", ctypes.c_int32),
+                ("pages_per_sequence", ctypes.c_int32), ("key_scale", ctypes.c_float),
+                ("value_scale", ctypes.c_float), ("page_stride", _sz), ("d_pages", ctypes.c_void_p),
+                ("d_lengths", ctypes.c_void_p)]
+
+
+class HipPagedAppend(ctypes.Structure):
+    """hp_hip_paged_append_t: the new tokens of a batch."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("d_q", "d_k", "d_v")] + \
+               [(n, _sz) for n in ("q_stride", "k_stride", "v_stride")] + \
+               [(n, ctypes.c_void_p) for n in ("d_offsets", "d_q_norm", "d_k_norm", "d_rope_freq_factors", "d_q_out",
+                                               "d_k_out", "d_v_out")] + \
+               [("token_count", _sz)] + \
+               [(n, ctypes.c_int32) for n in ("head_count", "out_type", "norm_values", "rope_dims")] + \
+               [("rope_freq_base", ctypes.c_double), ("epsilon", ctypes.c_double)]
+
+
+class HipPagedAttention(ctypes.Structure):
+    """hp_hip_paged_attention_t: one query token of every sequence."""
+    _fields_ = [("d_q", ctypes.c_void_p), ("d_output", ctypes.c_void_p), ("q_stride", _sz), ("output_stride", _sz)] + \
+               [(n, ctypes.c_int32) for n in ("head_count", "q_type", "out_type", "sliding_window")] + \
+               [("scale", ctypes.c_float), ("reserved", ctypes.c_int32)]
+
+
+class HipPackedAttention(ctypes.Structure):
+    """hp_hip_packed_attention_t: prompts end to end."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("d_q", "d_k", "d_v", "d_output", "d_offsets")] + \
+               [(n, _sz) for n in ("token_count", "q_stride", "k_stride", "v_stride", "output_stride")] + \
+               [(n, ctypes.c_int32) for n in ("sequence_count", "head_count", "head_count_kv", "head_dim", "type",
+                                              "out_type", "sliding_window")] + [("scale", ctypes.c_float)]
+
+
+class HipLogitRules(ctypes.Structure):
+    """hp_hip_logit_rules_t: penalties, biases and the mask of a batch's logits."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("d_logits", "d_output", "d_history", "d_history_lengths",
+                                               "d_prompt_lengths", "d_repetition", "d_frequency", "d_presence",
+                                               "d_bias_ids", "d_bias_values", "d_bias_counts", "d_allowed")] + \
+               [(n, _sz) for n in ("rows", "n", "logits_stride", "output_stride", "history_stride", "bias_stride",
+                                   "allowed_stride")]
+
+
+def _declare_serving(L: ctypes.CDLL) -> None:
+    """Entry points of several sequences at once."""
+    vp = ctypes.c_void_p
+    cache = ctypes.POINTER(HipPagedCache)
+    L.hp_hip_paged_append_device.argtypes = [cache, ctypes.POINTER(HipPagedAppend), vp]
+    L.hp_hip_paged_attention_device.argtypes = [cache, ctypes.POINTER(HipPagedAttention), vp]
+    L.hp_hip_packed_attention_device.argtypes = [ctypes.POINTER(HipPackedAttention), vp]
+    L.hp_hip_logit_rules_device.argtypes = [ctypes.POINTER(HipLogitRules), vp]
+    for name in ("hp_hip_paged_append_device", "hp_hip_paged_attention_device", "hp_hip_packed_attention_device",
+                 "hp_hip_logit_rules_device"):
+        getattr(L, name).restype = ctypes.c_int32
+
+
 def _declare_optional(L: ctypes.CDLL) -> None:
     """Top-k, GeGLU, sampling and tuning entry points."""
     i32 = ctypes.c_int32
@@ -193,6 +251,7 @@ def _declare_optional(L: ctypes.CDLL) -> None:
                  "hp_hip_geglu", "hp_hip_geglu_device"):
         getattr(L, name).restype = i32
     _declare_decode(L)
+    _declare_serving(L)
 
 
 def lib() -> ctypes.CDLL:
@@ -705,3 +764,64 @@ def decode_layers_device(layers: Sequence[HipDecodeLayer], d_hidden: int, d_posi
     assertHipOk(lib().hp_hip_decode_layers_device(arr, len(layers), token_count, d_hidden, d_position,
                                                   d_output_norm or None, d_output or None, stream or None),
                 "decode_layers")
+
+
+# ---- several sequences at once (device pointers; asynchronous on ``stream``; no counterpart in the reference) ----------
+
+HP_ELEM_F32, HP_ELEM_F16, HP_ELEM_BF16, HP_ELEM_E4M3 = 0, 1, 2, 3
+
+
+def paged_cache(d_keys: int, d_values: int, type: int, *, page_count: int, page_size: int, head_count_kv: int,
+                head_dim: int, d_pages: int, d_lengths: int, sequence_count: int, pages_per_sequence: int,
+                key_scale: float = 1.0, value_scale: float = 1.0, page_stride: int = 0) -> HipPagedCache:
+    """hp_hip_paged_cache_t: pages [page][kv head][slot][head_dim] of ``type`` and the batch's tables."""
+    return HipPagedCache(d_keys, d_values, type, head_dim, head_count_kv, page_size, page_count, sequence_count,
+                         pages_per_sequence, key_scale, value_scale, page_stride, d_pages, d_lengths)
+
+
+def paged_append_device(cache: HipPagedCache, token_count: int, head_count: int, d_q: int, d_k: int, d_v: int,
+                        d_q_out: int, out_type: int, *, d_offsets: int = 0, d_q_norm: int = 0, d_k_norm: int = 0,
+                        norm_values: bool = False, epsilon: float = 1e-6, rope_dims: int = 0,
+                        rope_freq_base: float = 10000.0, d_rope_freq_factors: int = 0, q_stride: int = 0,
+                        k_stride: int = 0, v_stride: int = 0, d_k_out: int = 0, d_v_out: int = 0,
+                        stream: int = 0) -> None:
+    """Head norms, rotation, and the batch's new keys and values into their pages (and, with d_k_out / d_v_out, into
+    rows for packed_attention_device)."""
+    p = HipPagedAppend(d_q, d_k, d_v, q_stride, k_stride, v_stride, d_offsets, d_q_norm, d_k_norm,
+                       d_rope_freq_factors, d_q_out, d_k_out, d_v_out, token_count, head_count, out_type,
+                       1 if norm_values else 0, rope_dims, rope_freq_base, epsilon)
+    assertHipOk(lib().hp_hip_paged_append_device(ctypes.byref(cache), ctypes.byref(p), stream or None), "paged_append")
+
+
+def paged_attention_device(cache: HipPagedCache, head_count: int, d_q: int, q_type: int, d_output: int, out_type: int,
+                           *, scale: float = 1.0, sliding_window: int = 0, q_stride: int = 0, output_stride: int = 0,
+                           stream: int = 0) -> None:
+    """Attention of one token of every sequence, the last, over its pages."""
+    p = HipPagedAttention(d_q, d_output, q_stride, output_stride, head_count, q_type, out_type, sliding_window, scale,
+                          0)
+    assertHipOk(lib().hp_hip_paged_attention_device(ctypes.byref(cache), ctypes.byref(p), stream or None),
+                "paged_attention")
+
+
+def packed_attention_device(sequence_count: int, d_offsets: int, token_count: int, head_count: int,
+                            head_count_kv: int, head_dim: int, d_q: int, d_k: int, d_v: int, type: int, d_output: int,
+                            out_type: int, *, scale: float = 1.0, sliding_window: int = 0, q_stride: int = 0,
+                            k_stride: int = 0, v_stride: int = 0, output_stride: int = 0, stream: int = 0) -> None:
+    """Causal attention over whole prompts that lie end to end."""
+    p = HipPackedAttention(d_q, d_k, d_v, d_output, d_offsets, token_count, q_stride, k_stride, v_stride,
+                           output_stride, sequence_count, head_count, head_count_kv, head_dim, type, out_type,
+                           sliding_window, scale)
+    assertHipOk(lib().hp_hip_packed_attention_device(ctypes.byref(p), stream or None), "packed_attention")
+
+
+def logit_rules_device(rows: int, n: int, d_logits: int, d_output: int, *, d_history: int = 0,
+                       history_stride: int = 0, d_history_lengths: int = 0, d_prompt_lengths: int = 0,
+                       d_repetition: int = 0, d_frequency: int = 0, d_presence: int = 0, d_bias_ids: int = 0,
+                       d_bias_values: int = 0, d_bias_counts: int = 0, bias_stride: int = 0, d_allowed: int = 0,
+                       allowed_stride: int = 0, logits_stride: int = 0, output_stride: int = 0,
+                       stream: int = 0) -> None:
+    """Penalties for repeated tokens, biases and the grammar's mask on [rows][n] logits (d_output may be d_logits)."""
+    p = HipLogitRules(d_logits, d_output, d_history, d_history_lengths, d_prompt_lengths, d_repetition, d_frequency,
+                      d_presence, d_bias_ids, d_bias_values, d_bias_counts, d_allowed, rows, n, logits_stride,
+                      output_stride, history_stride, bias_stride, allowed_stride)
+    assertHipOk(lib().hp_hip_logit_rules_device(ctypes.byref(p), stream or None), "logit_rules")

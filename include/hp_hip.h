@@ -16,7 +16,7 @@
  * by concurrent calls on one device must not overlap.
  *
  * Intermediate device memory of the *_device entry points (decode
- * activations, attention partials, top-k selection state, prefill images,
+ * activations, attention partials and row parts, top-k selection state, prefill images,
  * gate/up sums) belongs to the stream a call is queued on: calls on
  * different streams never share it, and calls queued on one stream run in
  * order.  It only grows, and replaced buffers are kept until
@@ -504,6 +504,160 @@ int32_t hp_hip_decode_fused_status(void *stream);
  * products done, 6 chains done, 7 end (points a stage lacks stay 0).
  * NULL turns it off; a shorter buffer is not written. */
 int32_t hp_hip_set_fused_trace(uint64_t *d_stamps, size_t len);
+
+/* ---- Several sequences at once ------------------------------------------
+ * What a program that serves a batch of conversations runs between the
+ * projections and the sampler (no counterpart in the reference, which keeps
+ * one sequence): a key/value cache in pages, the attention of one new token
+ * of every sequence over it, causal attention over packed prompts, and the
+ * penalties, biases and masks of the logits.  Device pointers, asynchronous on
+ * `stream` (NULL = library stream; hipStreamPerThread: HP_ERR_ARG, its scratch
+ * could not be told apart by thread).  Lengths, offsets and page tables are
+ * read on the device when the kernels run, so a captured call serves every
+ * batch of its shape.  The arguments are checked on the host before anything
+ * is launched; nothing in a device array can lead a kernel out of the buffers
+ * that the arguments describe.  Outputs must not overlap inputs except where
+ * it says so.  Rows of 16-bit and fp8 elements, and f32 rows that are read or
+ * written here, start at 16-byte boundaries: base pointers and strides are
+ * multiples of 16 bytes (HP_ERR_ARG otherwise).  Strides are in elements; 0
+ * stands for rows without gaps. */
+
+/* Element types of these entry points. */
+#define HP_ELEM_F32 0
+#define HP_ELEM_F16 1
+#define HP_ELEM_BF16 2
+#define HP_ELEM_E4M3 3 /* OCP fp8, cache pages only: value = stored * scale */
+
+/* A pool of pages and what a batch's sequences hold in it.  Position i of
+ * sequence s is slot i % page_size of page d_pages[s * pages_per_sequence + i /
+ * page_size]; the head_dim elements of KV head h there start at element
+ *   page * page_stride + (h * page_size + slot) * head_dim
+ * of d_keys and of d_values.  A table entry outside 0 .. page_count - 1 names
+ * no page (for instance one that a sliding window has passed): its positions
+ * are left out of the attention, and rows appended there are dropped.  Entries
+ * behind a sequence's last page are not read.  d_lengths[s] counts the tokens
+ * of sequence s, those of this call among them; below 1 the sequence is
+ * empty, and past the table's end it counts as the table's end. */
+typedef struct hp_hip_paged_cache {
+  void *d_keys, *d_values;
+  int32_t type;          /* HP_ELEM_F16, HP_ELEM_BF16 or HP_ELEM_E4M3 */
+  int32_t head_dim;      /* 64, 128 or 256 */
+  int32_t head_count_kv;
+  int32_t page_size;     /* a power of two, 16 .. 4096 */
+  int32_t page_count;
+  int32_t sequence_count;     /* up to 65535; 0: calls do nothing */
+  int32_t pages_per_sequence; /* pages_per_sequence * page_size <= 2^30 */
+  float key_scale, value_scale; /* HP_ELEM_E4M3: finite, > 0; otherwise not used */
+  size_t page_stride;         /* elements; 0: head_count_kv * page_size * head_dim */
+  const int32_t *d_pages, *d_lengths;
+} hp_hip_paged_cache_t;
+
+/* The new tokens of a batch, as the projections leave them (f32 rows of
+ * [heads][head_dim]). */
+typedef struct hp_hip_paged_append {
+  const float *d_q, *d_k, *d_v; /* d_q NULL: no query rows (head_count 0); d_v NULL: the value shares the key projection */
+  size_t q_stride, k_stride, v_stride; /* from token to token */
+  const int32_t *d_offsets; /* [sequence_count + 1], rising: rows d_offsets[s] .. d_offsets[s + 1] - 1 are sequence s's
+                               last tokens.  NULL: row s is sequence s's last token (token_count = sequence_count) */
+  const float *d_q_norm, *d_k_norm;   /* [head_dim], or NULL: no norm */
+  const float *d_rope_freq_factors;   /* [rope_dims / 2], or NULL */
+  void *d_q_out, *d_k_out, *d_v_out;  /* [token][heads][head_dim] of out_type; d_k_out, d_v_out may be NULL */
+  size_t token_count;    /* rows, those behind the last sequence among them */
+  int32_t head_count;    /* query heads; a multiple of head_count_kv */
+  int32_t out_type;      /* HP_ELEM_F32, HP_ELEM_F16 or HP_ELEM_BF16 */
+  int32_t norm_values;   /* 1: values have the norm without a weight (rmsNormRowsNoWeight) */
+  int32_t rope_dims;     /* a multiple of 8 up to head_dim; 0: no rotation */
+  double rope_freq_base; /* finite, > 0 */
+  double epsilon;        /* of the norms; finite, >= 0 */
+} hp_hip_paged_append_t;
+
+/* Head norms, rotation of pairs (u, u + rope_dims / 2) by position *
+ * rope_freq_base^(-2u / rope_dims) / factor_u, and the keys and values into
+ * their pages: hp_hip_attention_prep_device for a batch, with the angles formed
+ * in 64 bits (the ring's prologue multiplies them up in 32, as the reference
+ * does).  Position of row t of sequence s: d_lengths[s] - (d_offsets[s + 1] -
+ * t).  Rows behind the last sequence, of an empty one, or of a position
+ * outside the table are left as they were.  Values are rounded to nearest
+ * even; E4M3 ones are held within +-448 * scale.  A page may be written through
+ * one position of the batch only (two sequences that share a page must not
+ * both append to it). */
+int32_t hp_hip_paged_append_device(const hp_hip_paged_cache_t *cache, const hp_hip_paged_append_t *append,
+                                   void *stream);
+
+/* Attention of one token of every sequence, the one at position d_lengths[s]
+ * - 1, over the sequence's last min(length, sliding_window) positions:
+ * softmax(scale * q . k) v per query head, query head h on KV head h /
+ * (head_count / head_count_kv).  Any query type goes with any cache type; the
+ * sums are f32 and the products exact to some 2^-16 (bf16 pages) or 2^-22
+ * (others) of the largest.  A sequence without a key (empty, or all its pages
+ * absent) has zeros.  What masked places hold does not matter; an infinity or
+ * NaN among the elements that count leaves no finite number in the outputs that
+ * it reaches, and the others as they are.  Two launches, over scratch of the
+ * stream's. */
+typedef struct hp_hip_paged_attention {
+  const void *d_q; /* [sequence_count][head_count][head_dim] of q_type */
+  void *d_output;  /* [sequence_count][head_count][head_dim] of out_type */
+  size_t q_stride, output_stride; /* from sequence to sequence */
+  int32_t head_count;
+  int32_t q_type, out_type;       /* HP_ELEM_F32, HP_ELEM_F16 or HP_ELEM_BF16 */
+  int32_t sliding_window;         /* 0: none */
+  float scale;                    /* finite, > 0 */
+  int32_t reserved;               /* 0 */
+} hp_hip_paged_attention_t;
+int32_t hp_hip_paged_attention_device(const hp_hip_paged_cache_t *cache, const hp_hip_paged_attention_t *attention,
+                                      void *stream);
+
+/* Causal attention over whole prompts that lie end to end: row i of a sequence
+ * over its rows max(0, i - sliding_window + 1) .. i (0: no window).  Rows
+ * d_offsets[s] .. d_offsets[s + 1] - 1 (rising, [sequence_count + 1]) are
+ * sequence s; rows behind the last are left as they were.  Queries, keys and
+ * values are of one type, which the probabilities are rounded to as well;
+ * scores, softmax statistics and sums are f32.  Token strides of their own let
+ * them lie in one projection's rows. */
+typedef struct hp_hip_packed_attention {
+  const void *d_q, *d_k, *d_v; /* [token][heads][head_dim] of type */
+  void *d_output;              /* [token][head_count][head_dim] of out_type */
+  const int32_t *d_offsets;
+  size_t token_count;          /* rows of the buffers, up to 2^30 */
+  size_t q_stride, k_stride, v_stride, output_stride; /* from token to token */
+  int32_t sequence_count;      /* up to 2^20; 0: the call does nothing */
+  int32_t head_count, head_count_kv;
+  int32_t head_dim;            /* 64, 128 or 256 */
+  int32_t type;                /* HP_ELEM_F16 or HP_ELEM_BF16 */
+  int32_t out_type;            /* HP_ELEM_F32, HP_ELEM_F16 or HP_ELEM_BF16 */
+  int32_t sliding_window;
+  float scale;                 /* finite, > 0 */
+} hp_hip_packed_attention_t;
+int32_t hp_hip_packed_attention_device(const hp_hip_packed_attention_t *attention, void *stream);
+
+/* What a request changes about its logits ahead of hp_hip_topk_device: per row
+ * and token, in f32 and in this order,
+ *   x > 0 ? x / repetition : x * repetition   the token is in the row's history
+ *   x - frequency * count                     count: its places in the history from
+ *   x - presence, if count > 0                d_prompt_lengths[row] on
+ *   x + bias                                  the last entry of the token in the row's list
+ *   -inf                                      bit token % 32 of mask word token / 32 is 0
+ * A row that the mask leaves nothing is all -inf.  Tokens outside 0 .. n - 1
+ * (padding) count nowhere.  Each array may be NULL where the rule is not used
+ * (d_history with its lengths; the three bias arrays together).  d_output may
+ * be d_logits. */
+typedef struct hp_hip_logit_rules {
+  const float *d_logits; /* [rows][n] */
+  float *d_output;       /* [rows][n] */
+  const int32_t *d_history, *d_history_lengths; /* [rows][history_stride], [rows] */
+  const int32_t *d_prompt_lengths;              /* [rows]; NULL: 0 */
+  const float *d_repetition, *d_frequency, *d_presence; /* [rows]; NULL: 1, 0, 0 */
+  const int32_t *d_bias_ids;                    /* [rows][bias_stride] */
+  const float *d_bias_values;                   /* [rows][bias_stride] */
+  const int32_t *d_bias_counts;                 /* [rows] */
+  const uint32_t *d_allowed;                    /* [rows][allowed_stride]; NULL: every token */
+  size_t rows;           /* up to 65535; 0: the call does nothing */
+  size_t n;              /* 1 .. 2^30 */
+  size_t logits_stride, output_stride;          /* from row to row, below 2^32; 0: n */
+  size_t history_stride, bias_stride;           /* up to 2^30; longer lengths count as these */
+  size_t allowed_stride;                        /* words; 0: (n + 31) / 32 */
+} hp_hip_logit_rules_t;
+int32_t hp_hip_logit_rules_device(const hp_hip_logit_rules_t *rules, void *stream);
 
 #ifdef __cplusplus
 }
