@@ -45,12 +45,15 @@ HP_PAGES_FN KeySpan key_span(int length, int64_t table_keys, int window) {
 HP_PAGES_FN uint32_t span_steps(const KeySpan &s) { return (uint32_t)((s.end - s.begin + kPagedStep - 1) / kPagedStep); }
 
 // Share i of `shares` (<= total) of the steps 0 .. total - 1 begins here, and
-// the share that step t is in.
+// the share that step t is in: the first total % shares shares have one step
+// more than the others.
 HP_PAGES_FN uint32_t share_begin(uint32_t total, uint32_t i, uint32_t shares) {
-  return (uint32_t)((uint64_t)total * i / shares);
+  const uint32_t each = total / shares, more = total - each * shares;
+  return i * each + (i < more ? i : more);
 }
 HP_PAGES_FN uint32_t share_of(uint32_t total, uint32_t t, uint32_t shares) {
-  return (uint32_t)((((uint64_t)t + 1) * shares - 1) / total);
+  const uint32_t each = total / shares, more = total - each * shares, long_part = more * (each + 1);
+  return t < long_part ? t / (each + 1) : more + (t - long_part) / each;
 }
 
 constexpr int kPackedRows = 128;  // query rows of a workgroup of the packed attention

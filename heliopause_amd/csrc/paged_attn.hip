@@ -38,6 +38,8 @@
 // A workgroup finds its place by a scan of the lengths.  A row that one
 // workgroup finishes is written at once; parts of the others go to scratch,
 // at most two a workgroup, and the merge launch joins them in their order.
+#include <type_traits>
+
 #include "hp_mfma.h"
 #include "hp_serving.h"
 #include "hp_wave.h"
@@ -145,9 +147,11 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(const PagedAttn
   using T = Tile<D, CT>;
   constexpr int kE = T::kE, kFrags = D / 32, kRowBytes = D * kE, kT = D / 16;
   __shared__ float4 sh_o[kWaves][kHeads][D / 4];
+  __shared__ u32x4 sh_q[THIRD ? 2 : 1][kFrags][64];  // the query's operand fragments, the same for every wave
   __shared__ float sh_m[kWaves][kHeads], sh_l[kWaves][kHeads];
+  __shared__ float sh_most[kWaves][16];  // largest elements of the query rows
   __shared__ uint32_t sh_scan[kWaves];
-  __shared__ int sh_place[3];  // sequence, its first step on the line, the line's length
+  __shared__ int sh_place[2];  // sequence, its first step on the line
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int q4 = lane >> 4, c16 = lane & 15;
   const int group = a.nq / a.c.nkv, blocks = blocks_of(a.nq, a.c.nkv), units = a.c.nkv * blocks;
@@ -174,28 +178,29 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(const PagedAttn
     if (w < wave) before += sh_scan[w];
     total += sh_scan[w];
   }
-  before -= mine;
-  total *= units;
-  before *= units;
+  before = (before - mine) * units;
   mine *= units;
+  total = __builtin_amdgcn_readfirstlane(total) * units;
   const uint32_t shares = min((uint32_t)gridDim.x, total), me = blockIdx.x;
   if (me >= shares) return;
   uint32_t at = share_begin(total, me, shares);
   const uint32_t stop = share_begin(total, me + 1, shares);
   if (at >= before && at - before < mine) {  // one thread
     int s = tid * run;
-    uint32_t start = before;
-    for (;; s++) {
-      const uint32_t n = span_steps(span_of(a, s)) * units;
-      if (at - start < n) break;
-      start += n;
-    }
+    uint32_t start = before, n = mine;
+    if (run > 1)
+      for (;; s++) {
+        n = span_steps(span_of(a, s)) * units;
+        if (at - start < n) break;
+        start += n;
+      }
     sh_place[0] = s;
     sh_place[1] = (int)start;
   }
   __syncthreads();
-  int seq = sh_place[0];
-  uint32_t seq_start = (uint32_t)sh_place[1];
+  // (the same for the workgroup, in scalar registers)
+  int seq = __builtin_amdgcn_readfirstlane(sh_place[0]);
+  uint32_t seq_start = __builtin_amdgcn_readfirstlane(sh_place[1]);
 
   const uint8_t *keys = static_cast<const uint8_t *>(a.c.keys), *values = static_cast<const uint8_t *>(a.c.values);
   const int page_mask = (1 << a.c.page_shift) - 1;
@@ -213,49 +218,23 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(const PagedAttn
     const int kvh = unit / blocks, h0 = (unit - kvh * blocks) * kHeads;  // KV head, first head of the group
     const int live = min(kHeads, group - h0);
 
-    // the query: row c16 % 8's elements, in parts
-    u32x4 qa[kFrags], qb[THIRD ? kFrags : 1];
-    float factor;  // of a score, to base 2
-    {
-      const int c = c16 & 7;
-      const int64_t at_q = seq * a.q_stride + (int64_t)(kvh * group + h0 + min(c, live - 1)) * D;
-      float x[kFrags][8], most = 0.0f;
+    // the query: each wave takes a share of the fragments, lane c16 % 8's head
+    // and the elements that the lane's keys have there
+    constexpr int kMine = kFrags < kWaves ? 1 : kFrags / kWaves;
+    const bool has = wave * kMine < kFrags;
+    const int c8 = c16 & 7;
+    uint4 raw[kMine][2];
+    if (has) {
+      const int64_t at_q = seq * a.q_stride + (int64_t)(kvh * group + h0 + min(c8, live - 1)) * D;
 #pragma unroll
-      for (int f = 0; f < kFrags; f++) {
-        // element j of fragment f: where the lane's keys have theirs
-        const int d = CT == kElemE4m3 ? 64 * (f >> 1) + 16 * q4 + 8 * (f & 1) : 32 * f + 8 * q4;
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-          const float v = load_elem(a.q, at_q + d + j, a.q_type);
-          x[f][j] = c < live ? v : 0.0f;
-          most = fmaxf(most, fabsf(x[f][j]));
-        }
-      }
-      most = column_max(most);
-      // the row times the power of two that puts its largest element into
-      // [16, 32): the parts' range is then no concern (not for zeros and
-      // infinities, which stay)
-      const int e = (int)(__builtin_bit_cast(uint32_t, most) >> 23) - 127;
-      const int shift = most > 0.0f && e < 128 ? 4 - max(e, -100) : 0;
-      const float up = __builtin_bit_cast(float, (uint32_t)(127 + shift) << 23);
-      factor = a.scale * (CT == kElemE4m3 ? a.c.key_scale : 1.0f) * kLog2e / up;
-      const bool rest = c16 >= kHeads;
-#pragma unroll
-      for (int f = 0; f < kFrags; f++) {
-        uint32_t p0[8], p2[8];
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-          const float v = x[f][j] * up;
-          const uint32_t hi = part_bits<CT>(v);
-          const float r1 = v - part_value<CT>(hi);
-          const uint32_t mid = part_bits<CT>(r1);
-          p0[j] = rest ? mid : hi;
-          p2[j] = rest ? 0u : part_bits<CT>(r1 - part_value<CT>(mid));
-        }
-#pragma unroll
-        for (int w = 0; w < 4; w++) {
-          qa[f][w] = p0[2 * w] | p0[2 * w + 1] << 16;
-          if (THIRD) qb[THIRD ? f : 0][w] = p2[2 * w] | p2[2 * w + 1] << 16;
+      for (int i = 0; i < kMine; i++) {
+        const int f = wave * kMine + i, d = CT == kElemE4m3 ? 64 * (f >> 1) + 16 * q4 + 8 * (f & 1) : 32 * f + 8 * q4;
+        if (a.q_type == kElemF32) {
+          const uint4 *p = reinterpret_cast<const uint4 *>(static_cast<const float *>(a.q) + at_q + d);
+          raw[i][0] = p[0];
+          raw[i][1] = p[1];
+        } else {
+          raw[i][0] = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(a.q) + at_q + d);
         }
       }
     }
@@ -270,11 +249,15 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(const PagedAttn
     const int key_stop = min(span.end, span.begin + (int)(i0 + n) * kStep);
     const int *table = a.c.pages + (int64_t)seq * a.c.width;
     const int64_t head_at = ((int64_t)kvh << a.c.page_shift) * D;
-    // Page of the 16 keys from `key` on (the same for the wave), -1 for none.
-    // Only entries of pages that hold a key of the sequence are read.
-    auto page_of = [&](int key) -> int {
-      if (key >= span.end) return -1;
-      return page_or_none(table[key >> a.c.page_shift], a.c.page_count);
+    // Table entry of the 16 keys from `key` on (the same for the wave), and the
+    // page that it names or -1.  Only entries of pages that hold a key of the
+    // sequence are read, a step ahead of their rows.  Here and below loads take
+    // no branch: one that may not have been issued would make the next wait
+    // one for all.
+    auto entry_of = [&](int key) -> int { return table[min(key, span.end - 1) >> a.c.page_shift]; };
+    auto page_of = [&](int key, int entry) -> int {
+      const int p = page_or_none(__builtin_amdgcn_readfirstlane(entry), a.c.page_count);
+      return key < span.end ? p : -1;
     };
     // Bytes of the first of those keys' rows for this head; an absent page's
     // are page 0's, which are there and masked.
@@ -319,101 +302,184 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(const PagedAttn
         load_words<T::kValueWords>(t.v[j], values + (j < 4 ? b0 : b1) + (4 * q4 + (j & 3)) * kRowBytes + c16 * kT * kE);
     };
 
+    // (a wave whose keys are all behind the end loads its first tile for nothing)
     int key = key0;
-    if (key < key_stop) {
-      int p0 = page_of(key), p1 = page_of(key + 16);
-      int np0 = page_of(key + kStep), np1 = page_of(key + kStep + 16);
-      load_keys(key, p0, p1);
-      load_values(key, p0, p1);
-      for (; key < key_stop; key += kStep) {
-        const int next = key + kStep;
-        const bool more = next < key_stop;
-        f32x4 s[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+    int e0 = entry_of(key), e1 = entry_of(key + 16);
+    int p0 = page_of(key, e0), p1 = page_of(key + 16, e1);
+    e0 = entry_of(key + kStep);
+    e1 = entry_of(key + kStep + 16);
+    load_keys(key, p0, p1);
+    load_values(key, p0, p1);
+
+    // the query in parts, while the first keys are on their way
+    float x[kMine][8];
+    {
+      float most = 0.0f;
 #pragma unroll
-        for (int h = 0; h < 2; h++)
+      for (int i = 0; i < kMine; i++) {
+        const uint32_t w[8] = {raw[i][0].x, raw[i][0].y, raw[i][0].z, raw[i][0].w,
+                               raw[i][1].x, raw[i][1].y, raw[i][1].z, raw[i][1].w};
+        if (a.q_type == kElemF32) {
 #pragma unroll
-          for (int f = 0; f < kFrags; f++) {
-            u32x4 kf;
-            if (CT == kElemE4m3) {
-              const uint32_t lo = t.k[h][2 * f], hi = t.k[h][2 * f + 1];
-              kf = (u32x4){halves_of_e4m3<false>(lo), halves_of_e4m3<true>(lo), halves_of_e4m3<false>(hi),
-                           halves_of_e4m3<true>(hi)};
-            } else {
-              constexpr int kN = T::kKeyWords;
-              kf = (u32x4){t.k[h][4 * f % kN], t.k[h][(4 * f + 1) % kN], t.k[h][(4 * f + 2) % kN],
-                           t.k[h][(4 * f + 3) % kN]};
-            }
-            s[h] = mfma16<CT>(kf, qa[f], s[h]);
-            if (THIRD) s[h] = mfma16<CT>(kf, qb[THIRD ? f : 0], s[h]);
-          }
-        // the next keys stream in while these are worked on
-        if (more) load_keys(next, np0, np1);
-        const bool edge = key < span.first || key + kSub > span.end || p0 < 0 || p1 < 0;
-        float x[8];
+          for (int j = 0; j < 8; j++) x[i][j] = __builtin_bit_cast(float, w[j]);
+        } else if (a.q_type == kElemF16) {
+#pragma unroll
+          for (int j = 0; j < 8; j++)
+            x[i][j] = (float)__builtin_bit_cast(_Float16, (uint16_t)(w[j >> 1] >> (16 * (j & 1))));
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; j++) x[i][j] = bf16_value(w[j >> 1] >> (16 * (j & 1)) & 0xffffu);
+        }
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-          const float v = s[j >> 2][j & 3];
-          x[j] = (v + dpp_f32<kDppRor8>(v)) * factor;
+          x[i][j] = c8 < live && has ? x[i][j] : 0.0f;
+          most = fmaxf(most, fabsf(x[i][j]));
         }
-        if (edge) {  // the same for the wave
+      }
+      most = column_max(most);
+      if (q4 == 0) sh_most[wave][c16] = most;
+    }
+    __syncthreads();
+    float factor;  // of a score, to base 2
+    {
+      float most = sh_most[0][c16];
 #pragma unroll
-          for (int j = 0; j < 8; j++) {
-            const int at_key = key + 16 * (j >> 2) + 4 * q4 + (j & 3);
-            const bool off = at_key < span.first || at_key >= span.end || (j < 4 ? p0 : p1) < 0;
-            x[j] = off ? kNegInf : x[j];
+      for (int w = 1; w < kWaves; w++) most = fmaxf(most, sh_most[w][c16]);
+      // the row times the power of two that puts its largest element into
+      // [16, 32): the parts' range is then no concern (not for zeros and
+      // infinities, which stay)
+      const int e = (int)(__builtin_bit_cast(uint32_t, most) >> 23) - 127;
+      const int shift = most > 0.0f && e < 128 ? 4 - max(e, -100) : 0;
+      const float up = __builtin_bit_cast(float, (uint32_t)(127 + shift) << 23);
+      factor = a.scale * (CT == kElemE4m3 ? a.c.key_scale : 1.0f) * kLog2e / up;
+      const bool rest = c16 >= kHeads;
 #pragma unroll
-            for (int w = 0; w < T::kValueWords; w++) t.v[j][w] = off ? 0u : t.v[j][w];
+      for (int i = 0; i < kMine; i++) {
+        u32x4 qa, qb;
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+          uint32_t p0[2], p2[2];
+#pragma unroll
+          for (int b = 0; b < 2; b++) {
+            const float v = x[i][2 * w + b] * up;
+            const uint32_t hi = part_bits<CT>(v);
+            const float r1 = v - part_value<CT>(hi);
+            const uint32_t mid = part_bits<CT>(r1);
+            p0[b] = rest ? mid : hi;
+            p2[b] = rest ? 0u : part_bits<CT>(r1 - part_value<CT>(mid));
           }
+          qa[w] = p0[0] | p0[1] << 16;
+          qb[w] = p2[0] | p2[1] << 16;
         }
-        float most = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-        most = column_max(most);
-        if (__any(most > m_run)) {
-          const float m_new = fmaxf(m_run, most);
-          const float alpha = m_new == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_new);
-          m_run = m_new;
-          l_part *= alpha;
+        if (has) {
+          sh_q[0][wave * kMine + i][lane] = qa;
+          if (THIRD) sh_q[THIRD ? 1 : 0][wave * kMine + i][lane] = qb;
+        }
+      }
+    }
+    __syncthreads();
+
+    // One step: the scores of this tile, the next keys on their way, weights,
+    // the products with the values, the next values on their way.
+    auto step = [&](auto last) {
+      constexpr bool kMore = !decltype(last)::value;
+      const int next = key + kStep;
+      f32x4 s[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
-          for (int i = 0; i < kT; i++) acc[i] *= alpha;
+      for (int h = 0; h < 2; h++)
+#pragma unroll
+        for (int f = 0; f < kFrags; f++) {
+          u32x4 kf;
+          if (CT == kElemE4m3) {
+            const uint32_t lo = t.k[h][2 * f], hi = t.k[h][2 * f + 1];
+            kf = (u32x4){halves_of_e4m3<false>(lo), halves_of_e4m3<true>(lo), halves_of_e4m3<false>(hi),
+                         halves_of_e4m3<true>(hi)};
+          } else {
+            constexpr int kN = T::kKeyWords;
+            kf = (u32x4){t.k[h][4 * f % kN], t.k[h][(4 * f + 1) % kN], t.k[h][(4 * f + 2) % kN],
+                         t.k[h][(4 * f + 3) % kN]};
+          }
+          s[h] = mfma16<CT>(kf, sh_q[0][f][lane], s[h]);
+          if (THIRD) s[h] = mfma16<CT>(kf, sh_q[THIRD ? 1 : 0][f][lane], s[h]);
         }
-        // a row without a key so far: exp2(-inf - 0) = 0
-        const float m_use = m_run == kNegInf ? 0.0f : m_run - kBias;
-        u32x4 pf;
-        const bool rest = c16 >= kHeads;
-        uint32_t pb[8];
+      // the next keys stream in while these are worked on
+      int np0 = 0, np1 = 0;
+      if (kMore) {
+        np0 = page_of(next, e0);
+        np1 = page_of(next + 16, e1);
+        e0 = entry_of(next + kStep);
+        e1 = entry_of(next + kStep + 16);
+        load_keys(next, np0, np1);
+      }
+      const bool edge = key < span.first || key + kSub > span.end || p0 < 0 || p1 < 0;
+      float x[8];
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const float v = s[j >> 2][j & 3];
+        x[j] = (v + dpp_f32<kDppRor8>(v)) * factor;
+      }
+      if (edge) {  // the same for the wave
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-          const float p = __builtin_amdgcn_exp2f(x[j] - m_use);
-          l_part += p;
-          const uint32_t hi = part_bits<CT>(p), lo = part_bits<CT>(p - part_value<CT>(hi));
-          pb[j] = rest ? lo : hi;
+          const int at_key = key + 16 * (j >> 2) + 4 * q4 + (j & 3);
+          const bool off = at_key < span.first || at_key >= span.end || (j < 4 ? p0 : p1) < 0;
+          x[j] = off ? kNegInf : x[j];
+#pragma unroll
+          for (int w = 0; w < T::kValueWords; w++) t.v[j][w] = off ? 0u : t.v[j][w];
         }
+      }
+      float most = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+      most = column_max(most);
+      if (__any(most > m_run)) {
+        const float m_new = fmaxf(m_run, most);
+        const float alpha = m_new == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_new);
+        m_run = m_new;
+        l_part *= alpha;
 #pragma unroll
-        for (int w = 0; w < 4; w++) pf[w] = pb[2 * w] | pb[2 * w + 1] << 16;
-        // V^T fragments: element i of the lane's D / 16 from eight keys
+        for (int i = 0; i < kT; i++) acc[i] *= alpha;
+      }
+      // a row without a key so far: exp2(-inf - 0) = 0
+      const float m_use = m_run == kNegInf ? 0.0f : m_run - kBias;
+      u32x4 pf;
+      const bool rest = c16 >= kHeads;
+      uint32_t pb[8];
 #pragma unroll
-        for (int i = 0; i < kT; i++) {
-          u32x4 vf;
+      for (int j = 0; j < 8; j++) {
+        const float p = __builtin_amdgcn_exp2f(x[j] - m_use);
+        l_part += p;
+        const uint32_t hi = part_bits<CT>(p), lo = part_bits<CT>(p - part_value<CT>(hi));
+        pb[j] = rest ? lo : hi;
+      }
 #pragma unroll
-          for (int w = 0; w < 4; w++) {
-            const uint32_t sel = (i & 1) ? 0x07060302u : 0x05040100u;
-            if (CT == kElemE4m3) {
-              const uint32_t a0 = t.v[2 * w][i >> 2], a1 = t.v[2 * w + 1][i >> 2];
-              const uint32_t x0 = (i & 2) ? halves_of_e4m3<true>(a0) : halves_of_e4m3<false>(a0);
-              const uint32_t x1 = (i & 2) ? halves_of_e4m3<true>(a1) : halves_of_e4m3<false>(a1);
-              vf[w] = __builtin_amdgcn_perm(x1, x0, sel);
-            } else {
-              constexpr int kN = T::kValueWords;
-              vf[w] = __builtin_amdgcn_perm(t.v[2 * w + 1][(i >> 1) % kN], t.v[2 * w][(i >> 1) % kN], sel);
-            }
+      for (int w = 0; w < 4; w++) pf[w] = pb[2 * w] | pb[2 * w + 1] << 16;
+      // V^T fragments: element i of the lane's D / 16 from eight keys
+#pragma unroll
+      for (int i = 0; i < kT; i++) {
+        u32x4 vf;
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+          const uint32_t sel = (i & 1) ? 0x07060302u : 0x05040100u;
+          if (CT == kElemE4m3) {
+            const uint32_t a0 = t.v[2 * w][i >> 2], a1 = t.v[2 * w + 1][i >> 2];
+            const uint32_t x0 = (i & 2) ? halves_of_e4m3<true>(a0) : halves_of_e4m3<false>(a0);
+            const uint32_t x1 = (i & 2) ? halves_of_e4m3<true>(a1) : halves_of_e4m3<false>(a1);
+            vf[w] = __builtin_amdgcn_perm(x1, x0, sel);
+          } else {
+            constexpr int kN = T::kValueWords;
+            vf[w] = __builtin_amdgcn_perm(t.v[2 * w + 1][(i >> 1) % kN], t.v[2 * w][(i >> 1) % kN], sel);
           }
-          acc[i] = mfma16<CT>(vf, pf, acc[i]);
         }
-        if (more) load_values(next, np0, np1);
+        acc[i] = mfma16<CT>(vf, pf, acc[i]);
+      }
+      if (kMore) {
+        load_values(next, np0, np1);
         p0 = np0;
         p1 = np1;
-        np0 = page_of(next + kStep);
-        np1 = page_of(next + kStep + 16);
       }
+    };
+    if (key < key_stop) {
+      for (; key + kStep < key_stop; key += kStep) step(std::false_type{});
+      step(std::true_type{});
     }
 
     // the four waves' parts, joined in LDS.  Lane (q4, c): head c, elements
@@ -497,18 +563,38 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(const PagedAttnAr
   const RowParts r = rows[((int64_t)seq * a.c.nkv + kvh) * blocks + in_group / kHeads];
   if (r.first == r.last) return;  // written by the workgroup that had it whole
   float m = kNegInf, l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int c = r.first + sub; c <= r.last; c += kAtOnce) {
-    const Part<D> &p = parts[2 * (int64_t)c + (c == r.first ? 1 : 0)];
-    const float mc = p.m[h], lc = p.l[h];
-    const float4 v = *reinterpret_cast<const float4 *>(&p.o[h][4 * d]);
-    const float m_new = fmaxf(m, mc);
+  constexpr int kDeep = 4;  // parts that a thread has on their way
+  for (int c0 = r.first + sub; c0 <= r.last; c0 += kAtOnce * kDeep) {
+    float mc[kDeep], lc[kDeep];
+    float4 v[kDeep];
+#pragma unroll
+    for (int i = 0; i < kDeep; i++) {
+      const int c = min(c0 + i * kAtOnce, r.last);
+      const Part<D> &p = parts[2 * (int64_t)c + (c == r.first ? 1 : 0)];
+      mc[i] = p.m[h];
+      lc[i] = p.l[h];
+      v[i] = *reinterpret_cast<const float4 *>(&p.o[h][4 * d]);
+    }
+    float m_new = m;
+#pragma unroll
+    for (int i = 0; i < kDeep; i++) {
+      if (c0 + i * kAtOnce > r.last) mc[i] = kNegInf;
+      m_new = fmaxf(m_new, mc[i]);
+    }
     const float f = m == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(m - m_new);
-    const float g = mc == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(mc - m_new);
-    l = l * f + lc * g;
-    o[0] = o[0] * f + v.x * g;
-    o[1] = o[1] * f + v.y * g;
-    o[2] = o[2] * f + v.z * g;
-    o[3] = o[3] * f + v.w * g;
+    l *= f;
+#pragma unroll
+    for (int j = 0; j < 4; j++) o[j] *= f;
+#pragma unroll
+    for (int i = 0; i < kDeep; i++) {
+      if (c0 + i * kAtOnce > r.last) continue;
+      const float g = mc[i] == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(mc[i] - m_new);
+      l += lc[i] * g;
+      o[0] += v[i].x * g;
+      o[1] += v[i].y * g;
+      o[2] += v[i].z * g;
+      o[3] += v[i].w * g;
+    }
     m = m_new;
   }
   if (d == 0) {
