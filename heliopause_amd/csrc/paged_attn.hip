@@ -110,6 +110,20 @@ __device__ __forceinline__ float column_sum(float v) {
   return v + __shfl_xor(v, 32);
 }
 
+// Sum of v over the lanes up to this one.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_add(uint32_t v) {
+  return v + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+  v = dpp_add<0x111, 0xf>(v);         // row_shr 1, 2, 4, 8: within the 16 lanes
+  v = dpp_add<0x112, 0xf>(v);
+  v = dpp_add<0x114, 0xf>(v);
+  v = dpp_add<0x118, 0xf>(v);
+  v = dpp_add<0x142, 0xa>(v);         // lane 15's into rows 1 and 3
+  return dpp_add<0x143, 0xc>(v);      // lane 31's into rows 2 and 3
+}
+
 // A lane's elements of a key tile's row (D / 32 operand fragments) and of the
 // eight value rows (D / 16 elements each), as loaded.
 template <int D, int CT>
@@ -150,57 +164,40 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(const PagedAttn
   __shared__ u32x4 sh_q[THIRD ? 2 : 1][kFrags][64];  // the query's operand fragments, the same for every wave
   __shared__ float sh_m[kWaves][kHeads], sh_l[kWaves][kHeads];
   __shared__ float sh_most[kWaves][16];  // largest elements of the query rows
-  __shared__ uint32_t sh_scan[kWaves];
-  __shared__ int sh_place[2];  // sequence, its first step on the line
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int q4 = lane >> 4, c16 = lane & 15;
   const int group = a.nq / a.c.nkv, blocks = blocks_of(a.nq, a.c.nkv), units = a.c.nkv * blocks;
 
-  // the line of steps: each thread sums a run of sequences, then the runs are
-  // scanned
-  const int run = (a.c.sequences + kThreads - 1) / kThreads;
+  // The line of steps, by each wave for itself (no barrier): a lane sums a run
+  // of sequences, the runs are scanned, and the lane whose run has the
+  // workgroup's first step tells its place.
+  const int run = (a.c.sequences + 63) >> 6;
   uint32_t mine = 0;
   for (int i = 0; i < run; i++) {
-    const int s = tid * run + i;
+    const int s = lane * run + i;
     if (s < a.c.sequences) mine += span_steps(span_of(a, s));
   }
-  uint32_t before = mine;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const uint32_t up = __shfl_up(before, o);
-    if (lane >= o) before += up;
-  }
-  if (lane == 63) sh_scan[wave] = before;
-  __syncthreads();
-  uint32_t total = 0;
-#pragma unroll
-  for (int w = 0; w < kWaves; w++) {
-    if (w < wave) before += sh_scan[w];
-    total += sh_scan[w];
-  }
+  uint32_t before = wave_scan(mine);
+  const uint32_t total = (uint32_t)__builtin_amdgcn_readlane((int)before, 63) * units;
   before = (before - mine) * units;
   mine *= units;
-  total = __builtin_amdgcn_readfirstlane(total) * units;
   const uint32_t shares = min((uint32_t)gridDim.x, total), me = blockIdx.x;
   if (me >= shares) return;
   uint32_t at = share_begin(total, me, shares);
   const uint32_t stop = share_begin(total, me + 1, shares);
-  if (at >= before && at - before < mine) {  // one thread
-    int s = tid * run;
-    uint32_t start = before, n = mine;
-    if (run > 1)
-      for (;; s++) {
-        n = span_steps(span_of(a, s)) * units;
-        if (at - start < n) break;
-        start += n;
-      }
-    sh_place[0] = s;
-    sh_place[1] = (int)start;
-  }
-  __syncthreads();
-  // (the same for the workgroup, in scalar registers)
-  int seq = __builtin_amdgcn_readfirstlane(sh_place[0]);
-  uint32_t seq_start = __builtin_amdgcn_readfirstlane(sh_place[1]);
+  const bool mine_is = at >= before && at - before < mine;  // one lane
+  int place = lane * run;
+  uint32_t start = before;
+  if (run > 1 && mine_is)
+    for (;; place++) {
+      const uint32_t n = span_steps(span_of(a, place)) * units;
+      if (at - start < n) break;
+      start += n;
+    }
+  // (scalar registers from here on)
+  const int holder = __builtin_ctzll(__ballot(mine_is));
+  int seq = __builtin_amdgcn_readlane(place, holder);
+  uint32_t seq_start = (uint32_t)__builtin_amdgcn_readlane((int)start, holder);
 
   const uint8_t *keys = static_cast<const uint8_t *>(a.c.keys), *values = static_cast<const uint8_t *>(a.c.values);
   const int page_mask = (1 << a.c.page_shift) - 1;
@@ -383,6 +380,9 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(const PagedAttn
     // the products with the values, the next values on their way.
     auto step = [&](auto last) {
       constexpr bool kMore = !decltype(last)::value;
+      // the query's fragments are read anew in every step: in registers they
+      // would cost heads of 256 a spill
+      asm volatile("" ::: "memory");
       const int next = key + kStep;
       f32x4 s[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
