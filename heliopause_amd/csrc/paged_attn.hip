@@ -135,27 +135,26 @@ struct Tile {
   uint32_t v[8][kValueWords];
 };
 
-template <int N>
+// (STREAM: not to stay in the caches)
+template <bool STREAM, int N>
 __device__ __forceinline__ void load_words(uint32_t (&d)[N], const uint8_t *p) {
-  if (N == 1) {
-    d[0] = *reinterpret_cast<const uint32_t *>(p);
-  } else if (N == 2) {
-    const uint2 w = *reinterpret_cast<const uint2 *>(p);
-    d[0] = w.x;
-    d[1 % N] = w.y;
-  } else {
+  constexpr int kWide = N < 4 ? N : 4;
+  typedef uint32_t words __attribute__((ext_vector_type(kWide == 1 ? 2 : kWide)));
 #pragma unroll
-    for (int i = 0; i < N; i += 4) {
-      const uint4 w = *reinterpret_cast<const uint4 *>(p + 4 * i);
-      d[i] = w.x;
-      d[(i + 1) % N] = w.y;
-      d[(i + 2) % N] = w.z;
-      d[(i + 3) % N] = w.w;
+  for (int i = 0; i < N; i += kWide) {
+    if (kWide == 1) {
+      const uint32_t *q = reinterpret_cast<const uint32_t *>(p + 4 * i);
+      d[i] = STREAM ? __builtin_nontemporal_load(q) : *q;
+    } else {
+      const words *q = reinterpret_cast<const words *>(p + 4 * i);
+      const words w = STREAM ? __builtin_nontemporal_load(q) : *q;
+#pragma unroll
+      for (int j = 0; j < kWide; j++) d[i + j] = w[j];
     }
   }
 }
 
-template <int D, int CT, bool THIRD>
+template <int D, int CT, bool THIRD, bool STREAM>
 __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(const PagedAttnArgs a, RowParts *__restrict__ rows,
                                                                  Part<D> *__restrict__ parts) {
   using T = Tile<D, CT>;
@@ -271,10 +270,10 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(const PagedAttn
         for (int i = 0; i < kN; i++) {
           const int off = c16 * kRowBytes + 64 * i + 16 * q4;
           uint32_t w[4];
-          load_words<4>(w, keys + b0 + off);
+          load_words<STREAM>(w, keys + b0 + off);
 #pragma unroll
           for (int j = 0; j < 4; j++) t.k[0][4 * i + j] = w[j];
-          load_words<4>(w, keys + b1 + off);
+          load_words<STREAM>(w, keys + b1 + off);
 #pragma unroll
           for (int j = 0; j < 4; j++) t.k[1][4 * i + j] = w[j];
         }
@@ -283,10 +282,10 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(const PagedAttn
         for (int i = 0; i < kFrags; i++) {
           const int off = c16 * kRowBytes + 64 * i + 16 * q4;
           uint32_t w[4];
-          load_words<4>(w, keys + b0 + off);
+          load_words<STREAM>(w, keys + b0 + off);
 #pragma unroll
           for (int j = 0; j < 4; j++) t.k[0][(4 * i + j) % T::kKeyWords] = w[j];
-          load_words<4>(w, keys + b1 + off);
+          load_words<STREAM>(w, keys + b1 + off);
 #pragma unroll
           for (int j = 0; j < 4; j++) t.k[1][(4 * i + j) % T::kKeyWords] = w[j];
         }
@@ -296,7 +295,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(const PagedAttn
       const int64_t b0 = tile_at(p0, key), b1 = tile_at(p1, key + 16);
 #pragma unroll
       for (int j = 0; j < 8; j++)
-        load_words<T::kValueWords>(t.v[j], values + (j < 4 ? b0 : b1) + (4 * q4 + (j & 3)) * kRowBytes + c16 * kT * kE);
+        load_words<STREAM>(t.v[j], values + (j < 4 ? b0 : b1) + (4 * q4 + (j & 3)) * kRowBytes + c16 * kT * kE);
     };
 
     // (a wave whose keys are all behind the end loads its first tile for nothing)
@@ -555,15 +554,15 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(const PagedAttnAr
   const int kvh = head / group, in_group = head - kvh * group, h = in_group % kHeads;
   const int tid = threadIdx.x, sub = tid / kPer, d = tid - sub * kPer;
   const int64_t out = seq * a.out_stride + (int64_t)head * D + 4 * d;
+  const RowParts r = rows[((int64_t)seq * a.c.nkv + kvh) * blocks + in_group / kHeads];  // (of an earlier launch without a key)
   if (span_steps(span_of(a, seq)) == 0) {  // no key: zeros
     const float zero[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     if (sub == 0) store4(a.out, out, a.out_type, zero);
     return;
   }
-  const RowParts r = rows[((int64_t)seq * a.c.nkv + kvh) * blocks + in_group / kHeads];
   if (r.first == r.last) return;  // written by the workgroup that had it whole
   float m = kNegInf, l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  constexpr int kDeep = 4;  // parts that a thread has on their way
+  constexpr int kDeep = 8;  // parts that a thread has on their way
   for (int c0 = r.first + sub; c0 <= r.last; c0 += kAtOnce * kDeep) {
     float mc[kDeep], lc[kDeep];
     float4 v[kDeep];
@@ -624,17 +623,31 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(const PagedAttnAr
   store4(a.out, out, a.out_type, o);
 }
 
-template <int D, int CT, bool THIRD>
-hipError_t launch(const PagedAttnArgs &a, int groups, hipStream_t s) {
+template <int D, int CT, bool THIRD, bool STREAM>
+hipError_t launch_kernels(const PagedAttnArgs &a, int groups, hipStream_t s) {
   const int64_t rows = (int64_t)a.c.sequences * a.c.nkv * blocks_of(a.nq, a.c.nkv);
   Part<D> *parts = reinterpret_cast<Part<D> *>(a.partials);
   RowParts *row_parts = reinterpret_cast<RowParts *>(parts + 2 * (int64_t)groups);
   (void)rows;
-  hipLaunchKernelGGL((paged_attn_kernel<D, CT, THIRD>), dim3(groups), dim3(kThreads), 0, s, a, row_parts, parts);
+  hipLaunchKernelGGL((paged_attn_kernel<D, CT, THIRD, STREAM>), dim3(groups), dim3(kThreads), 0, s, a, row_parts, parts);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL(paged_merge_kernel<D>, dim3(a.nq, a.c.sequences), dim3(kThreads), 0, s, a, row_parts, parts);
   return hipGetLastError();
+}
+
+// Keys and values are read once where a group has one block of heads; what does
+// not fit the L2s together (32 MB) then goes past them: 122 -> 110 us (5.4 ->
+// 6.0 TB/s) on 48 contexts up to 8192, 80 -> 71 on two of 131072.  A batch that
+// does fit is read from them in repeated calls: 13.7 us and 14.4 past them on
+// one context of 4096.  The lengths are on the device, so it goes by the table.
+template <int D, int CT, bool THIRD>
+hipError_t launch(const PagedAttnArgs &a, int groups, hipStream_t s) {
+  uint64_t keys = (uint64_t)a.c.width << a.c.page_shift;
+  if (a.window > 0 && keys > (uint64_t)a.window) keys = a.window;
+  const bool stream = blocks_of(a.nq, a.c.nkv) == 1 &&
+                      keys * a.c.sequences * a.c.nkv * D * 2 * (CT == kElemE4m3 ? 1 : 2) > (32u << 20);
+  return stream ? launch_kernels<D, CT, THIRD, true>(a, groups, s) : launch_kernels<D, CT, THIRD, false>(a, groups, s);
 }
 
 template <int D>
