@@ -379,9 +379,9 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(const PagedAttn
     // the products with the values, the next values on their way.
     auto step = [&](auto last) {
       constexpr bool kMore = !decltype(last)::value;
-      // the query's fragments are read anew in every step: in registers they
-      // would cost heads of 256 a spill
-      asm volatile("" ::: "memory");
+      // the query's fragments are read anew in every step where in registers they
+      // would not fit
+      if (D == 256 && CT != kElemE4m3) asm volatile("" ::: "memory");
       const int next = key + kStep;
       f32x4 s[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
