@@ -3015,6 +3015,7 @@ int32_t packed_attention_check(const hp_hip_packed_attention_t *p, PackedAttnArg
   if ((rc = row_stride(p->k_stride, kv_row, 2, p->token_count, &a->k_stride)) != HP_OK) return rc;
   if ((rc = row_stride(p->v_stride, kv_row, 2, p->token_count, &a->v_stride)) != HP_OK) return rc;
   if ((rc = row_stride(p->output_stride, q_row, elem_bytes(p->out_type), p->token_count, &a->out_stride)) != HP_OK) return rc;
+  if ((a->k_stride | a->v_stride) >> 24) return fail(HP_ERR_SHAPE, "key and value strides must be below 2^24 elements");
   a->sequences = p->sequence_count;
   a->tokens = (int)p->token_count;
   a->nq = p->head_count;

@@ -41,6 +41,7 @@ constexpr int kThreads = 256, kWaves = 4;
 constexpr int kWaveRows = 32, kRows = kPackedRows;
 static_assert(kRows == kWaveRows * kWaves, "a block of rows");
 constexpr int kXcds = 8;
+constexpr int kWaitLoads = 0x0f70;  // s_waitcnt vmcnt(0)
 constexpr float kLog2e = 1.44269504088896341f;
 constexpr float kLazy = 8.0f;
 constexpr float kInf = __builtin_inff();
@@ -92,12 +93,29 @@ __device__ __forceinline__ void halves(float v, float *x, float *y) {
   *y = __builtin_bit_cast(float, r1);
 }
 
-// Exponent all ones (an infinity or a NaN) in the low / high half of w: a word
-// with the halves' bit 0 set there.
+// Bits 15 and 31 where the low and the high half of w are infinities or NaNs
+// (exponents all ones: one more in their last place carries); others are free.
 template <bool BF>
 __device__ __forceinline__ uint32_t nonfinite(uint32_t w) {
-  const uint32_t e = BF ? 0x7f80u : 0x7c00u;
-  return ((w & e) == e ? 1u : 0u) | ((w >> 16 & e) == e ? 0x10000u : 0u);
+  return BF ? (w & 0x7f807f80u) + 0x00800080u : (w & 0x7c007c00u) + 0x04000400u;
+}
+
+// 16 bytes a lane from base + offset into LDS, at `lds` (the same for the wave)
+// and on by lane.  As assembly, so that the compiler does not take reads of
+// the tile at hand to need the next one, which it cannot tell apart; the wait
+// is the loop's own.  Nothing comes back in a register; m0 (the LDS address,
+// one wait state ahead of its use) is as it was afterwards.
+__device__ __forceinline__ void load_to_lds(const uint8_t *base, uint32_t offset, uint32_t lds) {
+  uint32_t m0;
+  asm volatile(
+      "s_mov_b32 %0, m0\n\t"
+      "s_mov_b32 m0, %3\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %1, %2\n\t"
+      "s_mov_b32 m0, %0"
+      : "=&s"(m0)
+      : "v"(offset), "s"(base), "s"(lds)
+      : "memory");
 }
 
 // Chunk (16 bytes) where a tile's row keeps chunk c, for keys and values.  Keys
@@ -167,21 +185,22 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void packed_attn_kernel
   const uint8_t *kp = static_cast<const uint8_t *>(a.k) + ((int64_t)begin * a.k_stride + kvh * D) * 2;
   const uint8_t *vp = static_cast<const uint8_t *>(a.v) + ((int64_t)begin * a.v_stride + kvh * D) * 2;
 
-  // A lane's part of a tile: load i of this wave brings rows kLoadRows (i * 4 +
-  // wave) + lane / kChunks, LDS chunk lane % kChunks.
+  // A lane's part of a tile: load i of this wave brings rows kTurn i + kLoadRows
+  // wave + lane / kChunks, LDS chunk lane % kChunks.  Rows behind the sequence
+  // are its last, and masked.
+  constexpr int kTurn = S::kLoadRows * kWaves;
   const int load_row = S::kLoadRows * wave + lane / S::kChunks, load_chunk = lane % S::kChunks;
+  const uint32_t k_row = (uint32_t)a.k_stride * 2, v_row = (uint32_t)a.v_stride * 2;
+  const uint32_t lds_at = (uint32_t)(uintptr_t)(lds_ptr)&lds[0][0][0] + 1024 * wave;
   auto load_tile = [&](int key, int buffer) {
+    const uint8_t *kb = kp + (int64_t)key * k_row, *vb = vp + (int64_t)key * v_row;
+    const int last = len - 1 - key;
 #pragma unroll
     for (int i = 0; i < S::kLoads; i++) {
-      const int rr = load_row + S::kLoadRows * kWaves * i;
-      const int64_t from = min(key + rr, len - 1);  // rows behind the sequence are its last, and masked
-      const uint8_t *ks = kp + from * a.k_stride * 2 + 16 * (load_chunk ^ key_swizzle<D>(rr));
-      const uint8_t *vs = vp + from * a.v_stride * 2 + 16 * (load_chunk ^ value_swizzle<D>(rr));
-      const int at = 1024 * (wave + kWaves * i);
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)ks,
-                                       (__attribute__((address_space(3))) void *)&lds[buffer][0][at], 16, 0, 0);
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)vs,
-                                       (__attribute__((address_space(3))) void *)&lds[buffer][1][at], 16, 0, 0);
+      const int rr = load_row + kTurn * i, from = min(rr, last);
+      const uint32_t at = lds_at + (uint32_t)(buffer * 2 * S::kTileBytes + 1024 * kWaves * i);
+      load_to_lds(kb, from * k_row + 16 * (load_chunk ^ key_swizzle<D>(rr)), at);
+      load_to_lds(vb, from * v_row + 16 * (load_chunk ^ value_swizzle<D>(rr)), at + S::kTileBytes);
     }
   };
   load_tile(tile_first, 0);
@@ -205,7 +224,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void packed_attn_kernel
   for (int key = tile_first; key < tile_stop; key += kKeys, buffer ^= 1) {
     // this wave's part of tile `key` is in LDS; after the barrier every wave's,
     // and the other buffer has no reader left
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(kWaitLoads);
     __syncthreads();
     if (key + kKeys < tile_stop) load_tile(key + kKeys, buffer ^ 1);
     // what the wave's rows see of the tile (the same for the wave)
@@ -295,7 +314,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void packed_attn_kernel
           for (int w = 0; w < 4; w++) bad |= nonfinite<BF>(f[w]);
         }
     }
-    if (!__any(bad != 0)) {
+    if (!__any((bad & 0x80008000u) != 0)) {
 #pragma unroll
       for (int jj = 0; jj < 2 * kSubs; jj++)
 #pragma unroll

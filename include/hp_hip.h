@@ -619,7 +619,7 @@ typedef struct hp_hip_packed_attention {
   void *d_output;              /* [token][head_count][head_dim] of out_type */
   const int32_t *d_offsets;
   size_t token_count;          /* rows of the buffers, up to 2^30 */
-  size_t q_stride, k_stride, v_stride, output_stride; /* from token to token */
+  size_t q_stride, k_stride, v_stride, output_stride; /* from token to token; keys' and values' below 2^24 */
   int32_t sequence_count;      /* up to 2^20; 0: the call does nothing */
   int32_t head_count, head_count_kv;
   int32_t head_dim;            /* 64, 128 or 256 */

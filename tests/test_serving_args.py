@@ -118,7 +118,7 @@ def test_more_steps_than_the_kernel_counts():
     ({"head_count": 5}, HEADS), ({"head_count_kv": 0}, HEADS), ({"scale": INF}, ARG), ({"scale": -0.5}, ARG),
     ({"sliding_window": -3}, ARG), ({"sequence_count": -1}, SHAPE), ({"sequence_count": (1 << 20) + 1}, SHAPE),
     ({"token_count": (1 << 30) + 1}, SHAPE), ({"q_stride": 255}, SHAPE), ({"k_stride": 132}, ARG),
-    ({"v_stride": 100}, SHAPE), ({"output_stride": 260}, ARG), ({"d_q": None}, ARG), ({"d_offsets": None}, ARG),
+    ({"v_stride": 100}, SHAPE), ({"k_stride": 1 << 24}, SHAPE), ({"output_stride": 260}, ARG), ({"d_q": None}, ARG), ({"d_offsets": None}, ARG),
     ({"d_k": P + 2}, ARG), ({"d_output": None}, ARG), ({"token_count": 1 << 30, "head_count": 65534}, SHAPE)])
 def test_bad_packed(change, code):
     assert H.lib().hp_hip_packed_attention_device(packed(**change), None) == code
