@@ -30,6 +30,8 @@
 // become -inf, and where a tile has masked keys its values' infinities and
 // NaNs are taken out of the product (0 * inf) and added back for the rows
 // that do see them.
+#include <type_traits>
+
 #include "hp_mfma.h"
 #include "hp_serving.h"
 
@@ -98,6 +100,21 @@ __device__ __forceinline__ void halves(float v, float *x, float *y) {
 template <bool BF>
 __device__ __forceinline__ uint32_t nonfinite(uint32_t w) {
   return BF ? (w & 0x7f807f80u) + 0x00800080u : (w & 0x7c007c00u) + 0x04000400u;
+}
+
+// The halves of w that are of a kind -- 0: numbers, as they are; 1: +inf, 2:
+// -inf, 3: NaN, as ones -- and zeros for the others.
+template <bool BF>
+__device__ __forceinline__ uint32_t only_kind(uint32_t w, int kind) {
+  const uint32_t inf = BF ? 0x7f80u : 0x7c00u, one = BF ? 0x3f80u : 0x3c00u;
+  uint32_t x = 0;
+#pragma unroll
+  for (int b = 0; b < 2; b++) {
+    const uint32_t v = w >> (16 * b) & 0xffffu;
+    const int is = (v & inf) != inf ? 0 : v == inf ? 1 : v == (inf | 0x8000u) ? 2 : 3;
+    x |= (is == kind ? (kind == 0 ? v : one) : 0u) << (16 * b);
+  }
+  return x;
 }
 
 // 16 bytes a lane from base + offset into LDS, at `lds` (the same for the wave)
@@ -192,15 +209,35 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void packed_attn_kernel
   const int load_row = S::kLoadRows * wave + lane / S::kChunks, load_chunk = lane % S::kChunks;
   const uint32_t k_row = (uint32_t)a.k_stride * 2, v_row = (uint32_t)a.v_stride * 2;
   const uint32_t lds_at = (uint32_t)(uintptr_t)(lds_ptr)&lds[0][0][0] + 1024 * wave;
+  // (the rows of one load of all waves repeat the swizzles', but for heads of
+  // 256 every second time)
+  constexpr int kKinds = kTurn % 16 == 0 ? 1 : 2;
+  static_assert(kTurn * kKinds % 16 == 0, "the swizzles' period");
+  uint32_t k_at[kKinds], v_at[kKinds];
+#pragma unroll
+  for (int i = 0; i < kKinds; i++) {
+    const int rr = load_row + kTurn * i;
+    k_at[i] = load_row * k_row + 16 * (load_chunk ^ key_swizzle<D>(rr));
+    v_at[i] = load_row * v_row + 16 * (load_chunk ^ value_swizzle<D>(rr));
+  }
   auto load_tile = [&](int key, int buffer) {
     const uint8_t *kb = kp + (int64_t)key * k_row, *vb = vp + (int64_t)key * v_row;
-    const int last = len - 1 - key;
+    const int over = key + kKeys - len;  // rows behind the sequence
+    if (over <= 0) {                     // the same for the workgroup
 #pragma unroll
-    for (int i = 0; i < S::kLoads; i++) {
-      const int rr = load_row + kTurn * i, from = min(rr, last);
-      const uint32_t at = lds_at + (uint32_t)(buffer * 2 * S::kTileBytes + 1024 * kWaves * i);
-      load_to_lds(kb, from * k_row + 16 * (load_chunk ^ key_swizzle<D>(rr)), at);
-      load_to_lds(vb, from * v_row + 16 * (load_chunk ^ value_swizzle<D>(rr)), at + S::kTileBytes);
+      for (int i = 0; i < S::kLoads; i++) {
+        const uint32_t at = lds_at + (uint32_t)(buffer * 2 * S::kTileBytes + 1024 * kWaves * i);
+        load_to_lds(kb + (uint32_t)(kTurn * i) * (uint64_t)k_row, k_at[i % kKinds], at);
+        load_to_lds(vb + (uint32_t)(kTurn * i) * (uint64_t)v_row, v_at[i % kKinds], at + S::kTileBytes);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < S::kLoads; i++) {
+        const uint32_t at = lds_at + (uint32_t)(buffer * 2 * S::kTileBytes + 1024 * kWaves * i);
+        const int from = min(load_row + kTurn * i, kKeys - 1 - over) - load_row;
+        load_to_lds(kb, k_at[i % kKinds] + from * k_row, at);
+        load_to_lds(vb, v_at[i % kKinds] + from * v_row, at + S::kTileBytes);
+      }
     }
   };
   load_tile(tile_first, 0);
@@ -220,15 +257,9 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void packed_attn_kernel
     for (int i = 0; i < 16; i++) acc[t][i] = 0.0f;
   float m = -kInf, l = 0.0f;
 
-  int buffer = 0;
-  for (int key = tile_first; key < tile_stop; key += kKeys, buffer ^= 1) {
-    // this wave's part of tile `key` is in LDS; after the barrier every wave's,
-    // and the other buffer has no reader left
-    __builtin_amdgcn_s_waitcnt(kWaitLoads);
-    __syncthreads();
-    if (key + kKeys < tile_stop) load_tile(key + kKeys, buffer ^ 1);
-    // what the wave's rows see of the tile (the same for the wave)
-    if (key > wave0 + kWaveRows - 1 || key + kKeys - 1 < wave0 - min(wave0, window - 1)) continue;
+  // One tile in LDS: scores, weights, products with the values.
+  auto work = [&](int key, int buffer, auto edge) {
+    constexpr bool kMasked = decltype(edge)::value;
     const uint8_t *kt = lds[buffer][0];
     const uint8_t *vt = lds[buffer][1];
     f32x16 s[kSubs];
@@ -244,15 +275,25 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void packed_attn_kernel
         s[u] = mfma32<BF>(kf, q[i], s[u]);
       }
     }
-    const bool masked = key + kKeys - 1 > wave0 || key < wave0 + kWaveRows - min(wave0 + kWaveRows, window);
-    if (masked) {
+    if (kMasked) {
+      // the lane's key 32 u + 8 (i / 4) + i % 4 of the tile, from its first
+      const int to = row - key - 4 * h, from = first - key - 4 * h;
 #pragma unroll
       for (int u = 0; u < kSubs; u++)
 #pragma unroll
         for (int i = 0; i < 16; i++) {
-          const int j = key + 32 * u + 8 * (i >> 2) + 4 * h + (i & 3);
-          if (j > row || j < first) s[u][i] = -kInf;
+          const int j = 32 * u + 8 * (i >> 2) + (i & 3);
+          s[u][i] = j > to ? -kInf : s[u][i];
         }
+      if (from > -kKeys) {
+#pragma unroll
+        for (int u = 0; u < kSubs; u++)
+#pragma unroll
+          for (int i = 0; i < 16; i++) {
+            const int j = 32 * u + 8 * (i >> 2) + (i & 3);
+            s[u][i] = j < from ? -kInf : s[u][i];
+          }
+      }
     }
     float most = s[0][0];
 #pragma unroll
@@ -303,60 +344,79 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void packed_attn_kernel
       }
       return f;
     };
-    uint32_t bad = 0;
-    if (masked) {
+    bool odd = false;
 #pragma unroll
-      for (int jj = 0; jj < 2 * kSubs; jj++)
+    for (int jj = 0; jj < 2 * kSubs; jj++) {
+      u32x4 f[D / 32];
+#pragma unroll
+      for (int t = 0; t < D / 32; t++) f[t] = value_frag(jj, t);
+      if (kMasked) {  // (a weight of 0 times an infinity would be a NaN)
+        uint32_t bad = 0;
+#pragma unroll
+        for (int t = 0; t < D / 32; t++)
+#pragma unroll
+          for (int w = 0; w < 4; w++) bad |= nonfinite<BF>(f[t][w]);
+        if (__any((bad & 0x80008000u) != 0)) {
+          odd = true;
+#pragma unroll
+          for (int t = 0; t < D / 32; t++)
+#pragma unroll
+            for (int w = 0; w < 4; w++) f[t][w] = only_kind<BF>(f[t][w], 0);
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < D / 32; t++) acc[t] = mfma32<BF>(f[t], p[jj], acc[t]);
+    }
+    if (kMasked && odd) {
+      // what infinities and NaNs come to in the rows that see them: the weights
+      // of +inf, of -inf and of NaN, each as a product of its own
+#pragma unroll 1
+      for (int kind = 1; kind < 4; kind++) {
+        const float add = kind == 1 ? kInf : kind == 2 ? -kInf : __builtin_nanf("");
 #pragma unroll
         for (int t = 0; t < D / 32; t++) {
-          const u32x4 f = value_frag(jj, t);
+          f32x16 weight;
 #pragma unroll
-          for (int w = 0; w < 4; w++) bad |= nonfinite<BF>(f[w]);
-        }
-    }
-    if (!__any((bad & 0x80008000u) != 0)) {
+          for (int i = 0; i < 16; i++) weight[i] = 0.0f;
 #pragma unroll
-      for (int jj = 0; jj < 2 * kSubs; jj++)
+          for (int jj = 0; jj < 2 * kSubs; jj++) {
+            u32x4 f = value_frag(jj, t);
 #pragma unroll
-        for (int t = 0; t < D / 32; t++) acc[t] = mfma32<BF>(value_frag(jj, t), p[jj], acc[t]);
-    } else {
-      // the finite values, then what the others come to in the rows that see
-      // them: the weights of +inf, -inf and NaN, each as a product of its own
-      const uint32_t one = BF ? 0x3f80u : 0x3c00u, inf = BF ? 0x7f80u : 0x7c00u;
-      for (int jj = 0; jj < 2 * kSubs; jj++)
-#pragma unroll
-        for (int t = 0; t < D / 32; t++) {
-          const u32x4 f = value_frag(jj, t);
-          u32x4 part[4];
-#pragma unroll
-          for (int w = 0; w < 4; w++) {
-            uint32_t x[4] = {0, 0, 0, 0};
-#pragma unroll
-            for (int b = 0; b < 2; b++) {
-              const uint32_t v = f[w] >> (16 * b) & 0xffffu;
-              const int kind = (v & inf) != inf ? 0 : v == inf ? 1 : v == (inf | 0x8000u) ? 2 : 3;
-#pragma unroll
-              for (int k = 0; k < 4; k++) x[k] |= (kind == k ? (k == 0 ? v : one) : 0u) << (16 * b);
-            }
-#pragma unroll
-            for (int k = 0; k < 4; k++) part[k][w] = x[k];
+            for (int w = 0; w < 4; w++) f[w] = only_kind<BF>(f[w], kind);
+            weight = mfma32<BF>(f, p[jj], weight);
           }
-          u32x4 pj = p[0];
 #pragma unroll
-          for (int k = 1; k < 2 * kSubs; k++) pj = jj == k ? p[k] : pj;
-          acc[t] = mfma32<BF>(part[0], pj, acc[t]);
-#pragma unroll
-          for (int k = 1; k < 4; k++) {
-            f32x16 weight;
-#pragma unroll
-            for (int i = 0; i < 16; i++) weight[i] = 0.0f;
-            weight = mfma32<BF>(part[k], pj, weight);
-            const float add = k == 1 ? kInf : k == 2 ? -kInf : __builtin_nanf("");
-#pragma unroll
-            for (int i = 0; i < 16; i++) acc[t][i] += weight[i] > 0.0f ? add : 0.0f;
-          }
+          for (int i = 0; i < 16; i++) acc[t][i] += weight[i] > 0.0f ? add : 0.0f;
         }
+      }
     }
+  };
+  // This wave's part of tile `key` is in LDS after the wait; after the barrier
+  // every wave's is, and the other buffer has no reader left: the tile after
+  // goes there.
+  auto next_tile = [&](int key, int buffer) {
+    __builtin_amdgcn_s_waitcnt(kWaitLoads);
+    __syncthreads();
+    if (key + kKeys < tile_stop) load_tile(key + kKeys, buffer ^ 1);
+  };
+  // Tiles of which every row of the workgroup sees every key, in a loop of their
+  // own; the others mask.
+  const int whole_first = (row0 + kRows - min(row0 + kRows, window) + kKeys - 1) / kKeys * kKeys;
+  const int whole_stop = (row0 + 1) / kKeys * kKeys;
+  int buffer = 0;
+  for (int key = tile_first; key < tile_stop;) {
+    if (key >= whole_first && key < whole_stop) {
+      for (; key < whole_stop; key += kKeys, buffer ^= 1) {
+        next_tile(key, buffer);
+        work(key, buffer, std::false_type{});
+      }
+      continue;
+    }
+    next_tile(key, buffer);
+    // (what the wave's rows see of it, the same for the wave)
+    if (key <= wave0 + kWaveRows - 1 && key + kKeys - 1 >= wave0 - min(wave0, window - 1)) work(key, buffer, std::true_type{});
+    key += kKeys;
+    buffer ^= 1;
   }
 
   float x, y;
