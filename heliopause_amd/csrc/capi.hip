@@ -3125,7 +3125,7 @@ int32_t hp_hip_packed_attention_device(const hp_hip_packed_attention_t *attentio
       [&](State &s, hipStream_t strm) -> int32_t {
         if (a.sequences == 0 || a.tokens == 0) return HP_OK;
         hipEvent_t e = prof_begin(strm);
-        HP_HIP_TRY(launch_packed_attn(a, strm));
+        HP_HIP_TRY(launch_packed_attn(a, s.num_cus, strm));
         prof_end(HP_KERNEL_ATTENTION, e, strm);
         s.launches++;
         return HP_OK;

@@ -56,12 +56,10 @@ HP_PAGES_FN uint32_t share_of(uint32_t total, uint32_t t, uint32_t shares) {
   return t < long_part ? t / (each + 1) : more + (t - long_part) / each;
 }
 
-constexpr int kPackedRows = 128;  // query rows of a workgroup of the packed attention
-
-// Sequence s of a packed batch has the blocks from this one up to the next
-// sequence's: at least as many as its rows fill, with no sum over the
-// sequences before it.
-HP_PAGES_FN int64_t packed_first_block(int offset, int s) { return (offset > 0 ? offset : 0) / kPackedRows + (int64_t)s; }
-HP_PAGES_FN int64_t packed_blocks(int64_t tokens, int64_t sequences) { return tokens / kPackedRows + 1 + sequences; }
+// A packed batch in blocks of `rows` query rows: sequence s has the blocks from
+// this one up to the next sequence's, at least as many as its rows fill, with
+// no sum over the sequences before it.
+HP_PAGES_FN int64_t packed_first_block(int offset, int s, int rows) { return (offset > 0 ? offset : 0) / rows + (int64_t)s; }
+HP_PAGES_FN int64_t packed_blocks(int64_t tokens, int64_t sequences, int rows) { return tokens / rows + 1 + sequences; }
 
 }  // namespace hp

@@ -67,7 +67,7 @@ struct PackedAttnArgs {
 };
 // Whether the launch's grid is within what a launch takes.
 bool packed_attn_fits(const PackedAttnArgs &a);
-hipError_t launch_packed_attn(const PackedAttnArgs &a, hipStream_t s);
+hipError_t launch_packed_attn(const PackedAttnArgs &a, int num_cus, hipStream_t s);
 
 struct LogitRulesArgs {
   const float *logits;

@@ -7,9 +7,12 @@
 // close behind: every pair costs one exponential, a quarter-rate instruction.
 //
 // A workgroup is 128 query rows of one head, 32 for each of its four waves,
-// and walks the keys in tiles of kKeys through LDS, double buffered: tile t +
-// 1 goes from memory straight into LDS while tile t is worked on.  Two
-// workgroups share a CU, and one's products run under the other's softmax.
+// and walks the keys in tiles of kKeys through LDS, double buffered: the next
+// tiles go from memory straight into LDS while one is worked on.  Up to heads
+// of 128 two workgroups share a CU; the scores of the next tile are formed
+// ahead of this one's weights, so that a wave's products run under its
+// exponentials as well (heads of 256, one wave a SIMD: 192 -> 166 us on six
+// prompts of 9000 rows).
 // Per 32 keys a wave forms, on v_mfma_f32_32x32x16,
 //   S^T = K Q^T: the keys are the A rows, read as they lie; the query is the
 //     B operand, in registers throughout.  Lane (n, h) then has query row n's
@@ -40,8 +43,7 @@ namespace hp {
 namespace {
 
 constexpr int kThreads = 256, kWaves = 4;
-constexpr int kWaveRows = 32, kRows = kPackedRows;
-static_assert(kRows == kWaveRows * kWaves, "a block of rows");
+constexpr int kWaveRows = 32;
 constexpr int kXcds = 8;
 constexpr int kWaitLoads = 0x0f70;  // s_waitcnt vmcnt(0)
 constexpr float kLog2e = 1.44269504088896341f;
@@ -146,22 +148,26 @@ __device__ __forceinline__ int value_swizzle(int row) {
   return D == 64 ? (row & 2) << 1 : (row & 3) << 2;
 }
 
-template <int D>
+// Heads of D, the keys of a block split over G groups of waves.
+template <int D, int G>
 struct Shape {
-  static constexpr int kKeys = D == 256 ? 32 : 64;     // of a tile
+  static constexpr int kGroupWaves = kWaves / G, kRows = kWaveRows * kGroupWaves;  // query rows of a workgroup
+  static constexpr int kKeys = D == 256 ? 32 : 64;         // of a tile
   static constexpr int kRowBytes = 2 * D, kChunks = D / 8;
-  static constexpr int kTileBytes = kKeys * kRowBytes;  // of K or V
-  static constexpr int kLoads = kTileBytes / 1024 / kWaves;  // 16-byte loads a lane, of K or V
-  static constexpr int kLoadRows = 1024 / kRowBytes;    // rows of one load of a wave
+  static constexpr int kTileBytes = kKeys * kRowBytes;            // of K or V
+  static constexpr int kLoads = kTileBytes / 1024 / kGroupWaves;  // 16-byte loads a lane, of K or V
+  static constexpr int kLoadRows = 1024 / kRowBytes;              // rows of one load of a wave
 };
 
-template <int D, bool BF>
-__global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void packed_attn_kernel(const PackedAttnArgs a, int slots) {
-  using S = Shape<D>;
-  constexpr int kKeys = S::kKeys, kSubs = kKeys / 32, kRowBytes = S::kRowBytes;
-  __shared__ __align__(1024) uint8_t lds[2][2][S::kTileBytes];  // [buffer][K, V]
+template <int D, bool BF, int G>
+__global__ __launch_bounds__(kThreads, D * G >= 256 ? 1 : 2) void packed_attn_kernel(const PackedAttnArgs a, int slots) {
+  using S = Shape<D, G>;
+  constexpr int kKeys = S::kKeys, kSubs = kKeys / 32, kRowBytes = S::kRowBytes, kRows = S::kRows;
+  __shared__ __align__(1024) uint8_t lds_all[G][2][2][S::kTileBytes];  // [group][buffer][K, V]
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n32 = lane & 31, h = lane >> 5;
+  const int part = wave / S::kGroupWaves, member = wave % S::kGroupWaves;  // group of waves, place in it
+  auto &lds = lds_all[part];
 
   // Work: (slot, KV head) units from the last slot down -- a sequence's last
   // rows have the most keys -- dealt round the XCDs, the heads of a unit one
@@ -177,22 +183,22 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void packed_attn_kernel
     int lo = 0, n = a.sequences;  // the largest whose first block is not behind `slot`
     while (n > 64) {
       const int step = (n + 63) >> 6, at = lo + min(lane * step, n - 1);
-      const bool le = lane * step < n && packed_first_block(a.offsets[at], at) <= slot;
+      const bool le = lane * step < n && packed_first_block(a.offsets[at], at, kRows) <= slot;
       const int c = max(__popcll(__ballot(le)), 1) - 1;
       lo += c * step;
       n = min(step, n - c * step);
     }
     const int at = lo + min(lane, n - 1);
-    const bool le = lane < n && packed_first_block(a.offsets[at], at) <= slot;
+    const bool le = lane < n && packed_first_block(a.offsets[at], at, kRows) <= slot;
     seq = lo + max(__popcll(__ballot(le)), 1) - 1;
   }
   const int begin = a.offsets[seq], end = min(a.offsets[seq + 1], a.tokens);
   if (begin < 0 || begin >= end) return;
-  const int64_t row_at = (slot - packed_first_block(begin, seq)) * kRows;
+  const int64_t row_at = (slot - packed_first_block(begin, seq, kRows)) * kRows;
   const int len = end - begin;
   if (row_at < 0 || row_at >= len) return;
   const int row0 = (int)row_at;                         // the workgroup's first row
-  const int wave0 = row0 + kWaveRows * wave;            // the wave's
+  const int wave0 = row0 + kWaveRows * member;           // the wave's
   const int row = wave0 + n32;                          // the lane's
   const int window = a.window > 0 ? a.window : 0x7fffffff;
   const int first = max(row - min(row, window - 1), 0);  // first key of the lane's row
@@ -203,15 +209,14 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void packed_attn_kernel
   const uint8_t *vp = static_cast<const uint8_t *>(a.v) + ((int64_t)begin * a.v_stride + kvh * D) * 2;
 
   // A lane's part of a tile: load i of this wave brings rows kTurn i + kLoadRows
-  // wave + lane / kChunks, LDS chunk lane % kChunks.  Rows behind the sequence
+  // member + lane / kChunks, LDS chunk lane % kChunks.  Rows behind the sequence
   // are its last, and masked.
-  constexpr int kTurn = S::kLoadRows * kWaves;
-  const int load_row = S::kLoadRows * wave + lane / S::kChunks, load_chunk = lane % S::kChunks;
+  constexpr int kTurn = S::kLoadRows * S::kGroupWaves;
+  const int load_row = S::kLoadRows * member + lane / S::kChunks, load_chunk = lane % S::kChunks;
   const uint32_t k_row = (uint32_t)a.k_stride * 2, v_row = (uint32_t)a.v_stride * 2;
-  const uint32_t lds_at = (uint32_t)(uintptr_t)(lds_ptr)&lds[0][0][0] + 1024 * wave;
-  // (the rows of one load of all waves repeat the swizzles', but for heads of
-  // 256 every second time)
-  constexpr int kKinds = kTurn % 16 == 0 ? 1 : 2;
+  const uint32_t lds_at = (uint32_t)(uintptr_t)(lds_ptr)&lds[0][0][0] + 1024 * member;
+  // (the rows of one load of the group repeat the swizzles' after kKinds)
+  constexpr int kKinds = kTurn >= 16 ? 1 : 16 / kTurn;
   static_assert(kTurn * kKinds % 16 == 0, "the swizzles' period");
   uint32_t k_at[kKinds], v_at[kKinds];
 #pragma unroll
@@ -220,27 +225,25 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void packed_attn_kernel
     k_at[i] = load_row * k_row + 16 * (load_chunk ^ key_swizzle<D>(rr));
     v_at[i] = load_row * v_row + 16 * (load_chunk ^ value_swizzle<D>(rr));
   }
-  auto load_tile = [&](int key, int buffer) {
-    const uint8_t *kb = kp + (int64_t)key * k_row, *vb = vp + (int64_t)key * v_row;
+  auto load_rows = [&](const uint8_t *rows, uint32_t row_bytes, const uint32_t (&at)[kKinds], int key, uint32_t lds) {
+    const uint8_t *base = rows + (int64_t)key * row_bytes;
     const int over = key + kKeys - len;  // rows behind the sequence
     if (over <= 0) {                     // the same for the workgroup
 #pragma unroll
-      for (int i = 0; i < S::kLoads; i++) {
-        const uint32_t at = lds_at + (uint32_t)(buffer * 2 * S::kTileBytes + 1024 * kWaves * i);
-        load_to_lds(kb + (uint32_t)(kTurn * i) * (uint64_t)k_row, k_at[i % kKinds], at);
-        load_to_lds(vb + (uint32_t)(kTurn * i) * (uint64_t)v_row, v_at[i % kKinds], at + S::kTileBytes);
-      }
+      for (int i = 0; i < S::kLoads; i++)
+        load_to_lds(base + (uint32_t)(kTurn * i) * (uint64_t)row_bytes, at[i % kKinds], lds + 1024 * S::kGroupWaves * i);
     } else {
 #pragma unroll
       for (int i = 0; i < S::kLoads; i++) {
-        const uint32_t at = lds_at + (uint32_t)(buffer * 2 * S::kTileBytes + 1024 * kWaves * i);
         const int from = min(load_row + kTurn * i, kKeys - 1 - over) - load_row;
-        load_to_lds(kb, k_at[i % kKinds] + from * k_row, at);
-        load_to_lds(vb, v_at[i % kKinds] + from * v_row, at + S::kTileBytes);
+        load_to_lds(base, at[i % kKinds] + from * row_bytes, lds + 1024 * S::kGroupWaves * i);
       }
     }
   };
-  load_tile(tile_first, 0);
+  auto load_keys = [&](int key, int buffer) { load_rows(kp, k_row, k_at, key, lds_at + buffer * 2 * S::kTileBytes); };
+  auto load_values = [&](int key, int buffer) {
+    load_rows(vp, v_row, v_at, key, lds_at + (buffer * 2 + 1) * S::kTileBytes);
+  };
 
   u32x4 q[D / 16];
   {
@@ -249,6 +252,15 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void packed_attn_kernel
     for (int i = 0; i < D / 16; i++)
       q[i] = *reinterpret_cast<const u32x4 *>(static_cast<const uint8_t *>(a.q) + (at + 16 * i) * 2);
   }
+  // Group `part` has the tiles part, part + G, ... : its tile i is key_of(i).
+  const int tiles = (tile_stop - tile_first + kKeys - 1) / kKeys;
+  const int turns = (tiles + G - 1) / G, mine = (tiles - part + G - 1) / G;
+  auto key_of = [&](int i) { return tile_first + (i * G + part) * kKeys; };
+  if (mine > 0) {
+    load_keys(key_of(0), 0);
+    load_values(key_of(0), 0);
+  }
+  if (mine > 1) load_keys(key_of(1), 1);
   const float factor = a.scale * kLog2e;
   f32x16 acc[D / 32];
 #pragma unroll
@@ -257,12 +269,9 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void packed_attn_kernel
     for (int i = 0; i < 16; i++) acc[t][i] = 0.0f;
   float m = -kInf, l = 0.0f;
 
-  // One tile in LDS: scores, weights, products with the values.
-  auto work = [&](int key, int buffer, auto edge) {
-    constexpr bool kMasked = decltype(edge)::value;
+  // The steps of a tile.  scores: S^T of the keys in LDS.
+  auto scores = [&](f32x16 (&s)[kSubs], int buffer) {
     const uint8_t *kt = lds[buffer][0];
-    const uint8_t *vt = lds[buffer][1];
-    f32x16 s[kSubs];
 #pragma unroll
     for (int u = 0; u < kSubs; u++) {
 #pragma unroll
@@ -275,6 +284,10 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void packed_attn_kernel
         s[u] = mfma32<BF>(kf, q[i], s[u]);
       }
     }
+  };
+  // settle: masks them and moves the running maximum where they pass it.
+  auto settle = [&](f32x16 (&s)[kSubs], int key, auto edge) {
+    constexpr bool kMasked = decltype(edge)::value;
     if (kMasked) {
       // the lane's key 32 u + 8 (i / 4) + i % 4 of the tile, from its first
       const int to = row - key - 4 * h, from = first - key - 4 * h;
@@ -285,7 +298,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void packed_attn_kernel
           const int j = 32 * u + 8 * (i >> 2) + (i & 3);
           s[u][i] = j > to ? -kInf : s[u][i];
         }
-      if (from > -kKeys) {
+      if (__any(from > 0)) {
 #pragma unroll
         for (int u = 0; u < kSubs; u++)
 #pragma unroll
@@ -300,11 +313,9 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void packed_attn_kernel
     for (int u = 0; u < kSubs; u++)
 #pragma unroll
       for (int i = 0; i < 16; i++) most = fmaxf(most, s[u][i]);
-    {
-      float x, y;
-      halves(most, &x, &y);
-      most = fmaxf(x, y) * factor;
-    }
+    float x, y;
+    halves(most, &x, &y);
+    most = fmaxf(x, y) * factor;
     if (__any(most > m + kLazy)) {
       const float m_new = most > m + kLazy ? most : m;
       const float alpha = m_new == m ? 1.0f : __builtin_amdgcn_exp2f(m - m_new);
@@ -313,8 +324,10 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void packed_attn_kernel
 #pragma unroll
       for (int t = 0; t < D / 32; t++) acc[t] *= alpha;
     }
+  };
+  // weigh: the probabilities, as the B operand of the second product.
+  auto weigh = [&](const f32x16 (&s)[kSubs], u32x4 (&p)[2 * kSubs]) {
     const float m_use = m == -kInf ? 0.0f : m;  // no key so far: exp2(-inf)
-    u32x4 p[2 * kSubs];
 #pragma unroll
     for (int u = 0; u < kSubs; u++)
 #pragma unroll
@@ -325,6 +338,11 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void packed_attn_kernel
         l = add2<BF>(pair, l);
         p[2 * u + (w >> 2)][w & 3] = pair;
       }
+  };
+  // gather: O^T += V^T P^T with the values in LDS (check: keys may be masked).
+  auto gather = [&](const u32x4 (&p)[2 * kSubs], int buffer, bool check, auto edge) {
+    constexpr bool kMasked = decltype(edge)::value;
+    const uint8_t *vt = lds[buffer][1];
     // V^T fragments: product jj's k index 8 h + i is key 16 jj + 4 h + i (i < 4)
     // and 16 jj + 8 + 4 h + i - 4; a lane of 16 reads 8 bytes of key row
     // (lane % 16) / 4, elements 4 (lane % 4) .. of its 16
@@ -350,7 +368,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void packed_attn_kernel
       u32x4 f[D / 32];
 #pragma unroll
       for (int t = 0; t < D / 32; t++) f[t] = value_frag(jj, t);
-      if (kMasked) {  // (a weight of 0 times an infinity would be a NaN)
+      if (kMasked && check) {  // (a weight of 0 times an infinity would be a NaN)
         uint32_t bad = 0;
 #pragma unroll
         for (int t = 0; t < D / 32; t++)
@@ -391,78 +409,171 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void packed_attn_kernel
       }
     }
   };
-  // This wave's part of tile `key` is in LDS after the wait; after the barrier
-  // every wave's is, and the other buffer has no reader left: the tile after
-  // goes there.
-  auto next_tile = [&](int key, int buffer) {
+
+  // The walk over the tiles: while tile i's weights and values are worked on,
+  // the scores of tile i + 1 are formed, so that the matrix cores have work
+  // during the exponentials, and keys i + 2 and values i + 1 are on their way
+  // into the places of keys i and values i - 1, which no wave reads any more
+  // after the barrier.
+  auto sees = [&](int i) {  // whether any of the wave's rows has a key in tile i (the same for the wave)
+    return i < mine && key_of(i) <= wave0 + kWaveRows - 1 &&
+           key_of(i) + kKeys - 1 >= wave0 - min(wave0, window - 1);
+  };
+  auto next_loads = [&](int i) {
     __builtin_amdgcn_s_waitcnt(kWaitLoads);
     __syncthreads();
-    if (key + kKeys < tile_stop) load_tile(key + kKeys, buffer ^ 1);
+    if (i + 2 < mine) load_keys(key_of(i + 2), i & 1);
+    if (i + 1 < mine) load_values(key_of(i + 1), (i + 1) & 1);
   };
-  // Tiles of which every row of the workgroup sees every key, in a loop of their
-  // own; the others mask.
-  const int whole_first = (row0 + kRows - min(row0 + kRows, window) + kKeys - 1) / kKeys * kKeys;
-  const int whole_stop = (row0 + 1) / kKeys * kKeys;
-  int buffer = 0;
-  for (int key = tile_first; key < tile_stop;) {
-    if (key >= whole_first && key < whole_stop) {
-      for (; key < whole_stop; key += kKeys, buffer ^= 1) {
-        next_tile(key, buffer);
-        work(key, buffer, std::false_type{});
-      }
-      continue;
+  // Turns whose tiles every row of the workgroup sees whole.
+  const int whole_first =
+      (max(row0 + kRows - min(row0 + kRows, window) - tile_first + kKeys - 1, 0) / kKeys + G - 1) / G;
+  const int whole_stop = (row0 + 1 - tile_first) / kKeys / G;
+  f32x16 sa[kSubs], sb[kSubs];
+  __builtin_amdgcn_s_waitcnt(kWaitLoads);
+  __syncthreads();
+  if (sees(0)) {
+    scores(sa, 0);
+    settle(sa, key_of(0), std::true_type{});
+  }
+  for (int i = 0; i < turns;) {
+    // two at a time, so that each set of scores has its registers
+    for (; i % 2 == 0 && i >= whole_first && i + 2 < whole_stop; i += 2) {
+      u32x4 p[2 * kSubs];
+      next_loads(i);
+      scores(sb, 1);
+      weigh(sa, p);
+      gather(p, 0, false, std::false_type{});
+      settle(sb, 0, std::false_type{});
+      next_loads(i + 1);
+      scores(sa, 0);
+      weigh(sb, p);
+      gather(p, 1, false, std::false_type{});
+      settle(sa, 0, std::false_type{});
     }
-    next_tile(key, buffer);
-    // (what the wave's rows see of it, the same for the wave)
-    if (key <= wave0 + kWaveRows - 1 && key + kKeys - 1 >= wave0 - min(wave0, window - 1)) work(key, buffer, std::true_type{});
-    key += kKeys;
-    buffer ^= 1;
+    next_loads(i);
+    const bool more = sees(i + 1);
+    if (more) scores(sb, (i + 1) & 1);
+    if (sees(i)) {
+      u32x4 p[2 * kSubs];
+      weigh(sa, p);
+      gather(p, i & 1, i < whole_first || i >= whole_stop, std::true_type{});
+    }
+    if (more) {
+      settle(sb, key_of(i + 1), std::true_type{});
+#pragma unroll
+      for (int u = 0; u < kSubs; u++) sa[u] = sb[u];
+    }
+    i++;
   }
 
-  float x, y;
-  halves(l, &x, &y);
-  l = x + y;
+  {
+    float x, y;
+    halves(l, &x, &y);
+    l = x + y;
+  }
+  if (G > 1) {
+    // the groups' parts of a row, through the tiles' place in LDS: the first
+    // group's wave takes the others' in their order
+    constexpr int kPart = 64 * (D / 2 + 2);  // floats of a wave: acc, m, l by lane
+    float *place = reinterpret_cast<float *>(lds_all);
+    static_assert((G - 1) * S::kGroupWaves * kPart * 4 <= (int)sizeof(lds_all), "the parts fit the tiles' place");
+    __syncthreads();
+    if (part > 0) {
+      float *to = place + ((part - 1) * S::kGroupWaves + member) * kPart + lane;
+#pragma unroll
+      for (int t = 0; t < D / 32; t++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) to[64 * (16 * t + i)] = acc[t][i];
+      to[64 * (D / 2)] = m;
+      to[64 * (D / 2 + 1)] = l;
+    }
+    __syncthreads();
+    if (part > 0) return;
+#pragma unroll 1
+    for (int g = 1; g < G; g++) {
+      const float *from = place + ((g - 1) * S::kGroupWaves + member) * kPart + lane;
+      const float mg = from[64 * (D / 2)], lg = from[64 * (D / 2 + 1)];
+      const float m_new = fmaxf(m, mg);
+      const float f = m == -kInf ? 0.0f : __builtin_amdgcn_exp2f(m - m_new);
+      const float e = mg == -kInf ? 0.0f : __builtin_amdgcn_exp2f(mg - m_new);
+      m = m_new;
+      l = l * f + lg * e;
+#pragma unroll
+      for (int t = 0; t < D / 32; t++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) acc[t][i] = acc[t][i] * f + from[64 * (16 * t + i)] * e;
+    }
+  }
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   if (row >= len) return;
   const int64_t o = (int64_t)(begin + row) * a.out_stride + head * D;
+  auto store = [&](auto type) {
 #pragma unroll
-  for (int t = 0; t < D / 32; t++)
+    for (int t = 0; t < D / 32; t++)
 #pragma unroll
-    for (int b = 0; b < 4; b++) {
-      const float v[4] = {acc[t][4 * b] * inv, acc[t][4 * b + 1] * inv, acc[t][4 * b + 2] * inv, acc[t][4 * b + 3] * inv};
-      store4(a.out, o + 32 * t + 8 * b + 4 * h, a.out_type, v);
-    }
-}
-
-int64_t slots_of(const PackedAttnArgs &a) { return packed_blocks(a.tokens, a.sequences); }
-int64_t grid_of(const PackedAttnArgs &a) {
-  return (slots_of(a) * a.nkv + kXcds - 1) / kXcds * kXcds * (a.nq / a.nkv);
-}
-
-template <int D>
-hipError_t launch(const PackedAttnArgs &a, hipStream_t s) {
-  const int64_t slots = slots_of(a), grid = grid_of(a);
-  if (a.type == kElemBf16)
-    hipLaunchKernelGGL((packed_attn_kernel<D, true>), dim3((unsigned)grid), dim3(kThreads), 0, s, a, (int)slots);
+      for (int b = 0; b < 4; b++) {
+        const float v[4] = {acc[t][4 * b] * inv, acc[t][4 * b + 1] * inv, acc[t][4 * b + 2] * inv,
+                            acc[t][4 * b + 3] * inv};
+        store4(a.out, o + 32 * t + 8 * b + 4 * h, decltype(type)::value, v);
+      }
+  };
+  if (a.out_type == kElemF32)
+    store(std::integral_constant<int, kElemF32>{});
+  else if (a.out_type == kElemF16)
+    store(std::integral_constant<int, kElemF16>{});
   else
-    hipLaunchKernelGGL((packed_attn_kernel<D, false>), dim3((unsigned)grid), dim3(kThreads), 0, s, a, (int)slots);
+    store(std::integral_constant<int, kElemBf16>{});
+}
+
+// Groups of waves that the keys of a block are split over.  A block of 128 rows
+// with its waves side by side reads each key once for the most rows, which is
+// best where the blocks fill the card.  Where they do not, the block with the
+// most keys is what a launch takes, and blocks of 64 rows with two groups walk
+// half of them each.  Measured with one group and two, one prompt: heads of 64,
+// 280 blocks 34.6 and 23.5 us, 658 92 and 96; heads of 128 (a CU then has one
+// workgroup), 160 blocks 46.1 and 35.3, 224 blocks 20.8 and 23.6; heads of 256,
+// 256 blocks 152 and 115, 710 166 and 199.  Up to one tile of rows there is
+// nothing to split (40 rows: heads of 128 6.3 and 7.5, of 256 8.8 and 9.8, but
+// of 64 5.7 and 5.3).
+int groups_of(const PackedAttnArgs &a, int num_cus) {
+  const int64_t blocks = ((int64_t)a.tokens / (kWaveRows * kWaves) + 1) * a.nq;
+  if (a.head_dim > 64 && a.tokens <= 64) return 1;
+  return 4 * blocks < (a.head_dim == 128 ? 3 : 8) * (int64_t)num_cus ? 2 : 1;
+}
+
+int64_t slots_of(const PackedAttnArgs &a, int groups) {
+  return packed_blocks(a.tokens, a.sequences, kWaveRows * kWaves / groups);
+}
+int64_t grid_of(const PackedAttnArgs &a, int groups) {
+  return (slots_of(a, groups) * a.nkv + kXcds - 1) / kXcds * kXcds * (a.nq / a.nkv);
+}
+
+template <int D, int G>
+hipError_t launch(const PackedAttnArgs &a, hipStream_t s) {
+  const unsigned grid = (unsigned)grid_of(a, G);
+  const int slots = (int)slots_of(a, G);
+  if (a.type == kElemBf16)
+    hipLaunchKernelGGL((packed_attn_kernel<D, true, G>), dim3(grid), dim3(kThreads), 0, s, a, slots);
+  else
+    hipLaunchKernelGGL((packed_attn_kernel<D, false, G>), dim3(grid), dim3(kThreads), 0, s, a, slots);
   return hipGetLastError();
 }
 
 }  // namespace
 
-// (a launch has fewer than 2^32 threads in a dimension)
-bool packed_attn_fits(const PackedAttnArgs &a) { return grid_of(a) <= 0xffffffffll / kThreads; }
+// (a launch has fewer than 2^32 threads in a dimension; the shortest blocks
+// are for batches far below it)
+bool packed_attn_fits(const PackedAttnArgs &a) { return grid_of(a, 1) <= 0xffffffffll / kThreads / 8; }
 
-hipError_t launch_packed_attn(const PackedAttnArgs &a, hipStream_t s) {
+hipError_t launch_packed_attn(const PackedAttnArgs &a, int num_cus, hipStream_t s) {
   if (a.tokens < 1 || a.sequences < 1 || a.nkv < 1 || a.nq % a.nkv != 0 || !packed_attn_fits(a))
     return hipErrorInvalidValue;
-  switch (a.head_dim) {
-    case 64: return launch<64>(a, s);
-    case 128: return launch<128>(a, s);
-    case 256: return launch<256>(a, s);
-    default: return hipErrorInvalidValue;
-  }
+  const int groups = groups_of(a, num_cus);
+  if (a.head_dim == 64) return groups == 1 ? launch<64, 1>(a, s) : launch<64, 2>(a, s);
+  if (a.head_dim == 128) return groups == 1 ? launch<128, 1>(a, s) : launch<128, 2>(a, s);
+  if (a.head_dim == 256) return groups == 1 ? launch<256, 1>(a, s) : launch<256, 2>(a, s);
+  return hipErrorInvalidValue;
 }
 
 }  // namespace hp

@@ -91,13 +91,15 @@ def paged_attention(q, keys, values, lengths, pages, page_size, page_count, wind
     return out, mass, size, count
 
 
-def packed_attention(q, k, v, offsets, window, scale):
-    """Rows of every sequence: {row: (out [Hq][D], sum p |v|, score size [Hq], keys)}."""
+def packed_attention(q, k, v, offsets, window, scale, only=None):
+    """Rows of every sequence (or those in `only`): {row: (out [Hq][D], sum p |v|, score size [Hq], keys)}."""
     group = q.shape[1] // k.shape[1]
     got = {}
     q, k, v = (np.asarray(x, np.float64) for x in (q, k, v))
     for begin, end in zip(offsets[:-1], offsets[1:]):
         for t in range(begin, end):
+            if only is not None and t not in only:
+                continue
             first = max(begin, t - window + 1) if window else begin
             rows = [attend(q[t, h], k[first:t + 1, h // group], v[first:t + 1, h // group], scale)
                     for h in range(q.shape[1])]

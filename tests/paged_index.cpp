@@ -71,20 +71,20 @@ int main() {
   CHECK(share_begin(big, 511, 512) < big && share_of(big, big - 1, 512) == 511);
 
   // packed blocks: in order, and enough for every sequence
-  for (int round = 0; round < 2000; round++) {
-    const int n = 1 + rng() % 20;
+  for (int round = 0; round < 3000; round++) {
+    const int n = 1 + rng() % 20, rows = 32 << (round % 3);
     std::vector<int> offset(n + 1);
     offset[0] = rng() % 200;
     for (int s = 0; s < n; s++) offset[s + 1] = offset[s] + (rng() % 4 ? rng() % 400 : 0);
-    const int64_t blocks = packed_blocks(offset[n], n);
+    const int64_t blocks = packed_blocks(offset[n], n, rows);
     for (int s = 0; s < n; s++) {
-      const int64_t b = packed_first_block(offset[s], s);
-      const int64_t e = s + 1 < n ? packed_first_block(offset[s + 1], s + 1) : blocks;
+      const int64_t b = packed_first_block(offset[s], s, rows);
+      const int64_t e = s + 1 < n ? packed_first_block(offset[s + 1], s + 1, rows) : blocks;
       CHECK(b < e && e <= blocks);
-      CHECK((e - b) * kPackedRows >= offset[s + 1] - offset[s]);
+      CHECK((e - b) * rows >= offset[s + 1] - offset[s]);
     }
   }
-  CHECK(packed_first_block(-7, 3) == 3);
+  CHECK(packed_first_block(-7, 3, 128) == 3);
   puts("ok");
   return 0;
 }
