@@ -2940,7 +2940,7 @@ int32_t paged_append_check(const hp_hip_paged_cache_t *cache, const hp_hip_paged
     return fail(HP_ERR_SHAPE, "rope_dims must be a multiple of 8 up to head_dim");
   if (p->rope_dims > 0 && !positive(p->rope_freq_base)) return fail(HP_ERR_ARG, "rope_freq_base must be finite and positive");
   if (!std::isfinite(p->epsilon) || p->epsilon < 0.0) return fail(HP_ERR_ARG, "epsilon must be finite and not negative");
-  if (p->token_count > (1u << 30)) return fail(HP_ERR_SHAPE, "too many tokens");
+  if (p->token_count > (1u << 23)) return fail(HP_ERR_SHAPE, "too many tokens");
   if (!p->d_offsets && p->token_count != (size_t)a->c.sequences)
     return fail(HP_ERR_SHAPE, "without offsets there is one token a sequence");
   if (a->c.sequences == 0 || p->token_count == 0) return HP_OK;
@@ -3139,7 +3139,7 @@ int32_t hp_hip_logit_rules_device(const hp_hip_logit_rules_t *rules, void *strea
       [&](State &s, hipStream_t strm) -> int32_t {
         if (a.rows == 0) return HP_OK;
         hipEvent_t e = prof_begin(strm);
-        HP_HIP_TRY(launch_logit_rules(a, s.num_cus, strm));
+        HP_HIP_TRY(launch_logit_rules(a, strm));
         prof_end(HP_KERNEL_SAMPLE, e, strm);
         s.launches++;
         return HP_OK;

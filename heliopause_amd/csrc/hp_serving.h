@@ -80,7 +80,7 @@ struct LogitRulesArgs {
   int64_t logits_stride, out_stride, history_stride, bias_stride, allowed_stride;
   int rows, n;
 };
-hipError_t launch_logit_rules(const LogitRulesArgs &a, int num_cus, hipStream_t s);
+hipError_t launch_logit_rules(const LogitRulesArgs &a, hipStream_t s);
 
 // Largest s in 0 .. n such that offsets[1 .. s] <= t, by a whole wave: the
 // sequence of packed row t (n: a row behind the last).  64 entries are probed

@@ -14,8 +14,12 @@
 // history falls into the slice, one word a token, with integer atomics, whose
 // order changes nothing; so there is one launch, no scratch and no table of
 // the vocabulary's size in memory.  Every slice reads the history again (from
-// the L2), so slices are as long as leaves the card full.  The logits are
-// loaded first and wait in registers while the history is counted.
+// the L2).  The logits are loaded first and wait in registers while the history
+// is counted.  Slices of 2048 tokens by 256 threads: 6.1 us for one row of
+// 262144 and 37.5 us (4.2 TB/s) for 128 of 151669, against 7.7 and 39.8 in
+// slices of 16384, and 6.0 and 47.9 in slices of 1024.  Stores past the caches
+// make the launch alone faster (30 us) and with the top-k behind it, which reads
+// them, slower (196 -> 200 us), so they stay ordinary.
 #include "hp_serving.h"
 
 namespace hp {
@@ -28,11 +32,10 @@ constexpr uint32_t kInPrompt = 0x80000000u;  // of a word: the token is in the p
 typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));
 typedef int int4u __attribute__((ext_vector_type(4), aligned(4)));
 
-constexpr int kPer = 4;  // groups of four tokens a thread
+// A slice: a workgroup's threads with kPer groups of four tokens each.
+constexpr int kThreads = 256, kPer = 2, kSlice = kThreads * 4 * kPer;
 
-template <int THREADS>
-__global__ __launch_bounds__(THREADS) void logit_rules_kernel(const LogitRulesArgs a) {
-  constexpr int kSlice = THREADS * 4 * kPer;
+__global__ __launch_bounds__(kThreads) void logit_rules_kernel(const LogitRulesArgs a) {
   __shared__ uint32_t words[kSlice];
   const int tid = threadIdx.x, row = blockIdx.y, base = blockIdx.x * kSlice;
   const float *in = a.logits + row * a.logits_stride + base;
@@ -43,7 +46,7 @@ __global__ __launch_bounds__(THREADS) void logit_rules_kernel(const LogitRulesAr
   uint32_t allowed[kPer];
 #pragma unroll
   for (int g = 0; g < kPer; g++) {
-    const int i = 4 * (g * THREADS + tid);
+    const int i = 4 * (g * kThreads + tid);
     if (i + 4 <= left) {
       const float4u v = *reinterpret_cast<const float4u *>(in + i);
 #pragma unroll
@@ -63,7 +66,7 @@ __global__ __launch_bounds__(THREADS) void logit_rules_kernel(const LogitRulesAr
   if (told > 0 || biases > 0) {
 #pragma unroll
     for (int g = 0; g < kPer; g++)
-      *reinterpret_cast<uint4 *>(&words[4 * (g * THREADS + tid)]) = make_uint4(0, 0, 0, 0);
+      *reinterpret_cast<uint4 *>(&words[4 * (g * kThreads + tid)]) = make_uint4(0, 0, 0, 0);
     __syncthreads();
   }
   if (told > 0) {
@@ -77,13 +80,25 @@ __global__ __launch_bounds__(THREADS) void logit_rules_kernel(const LogitRulesAr
       else
         atomicAdd(&words[at], 1u);
     };
-    for (int i = 4 * tid; i < told; i += 4 * THREADS) {
-      if (i + 4 <= told) {
-        const int4u t = *reinterpret_cast<const int4u *>(history + i);
+    if (told < 4) {
+      if (tid < told) count(history[tid], tid);
+    } else {
+      // four at a time, the loads of kDeep fours on their way together; a four
+      // that would pass the end is the last four, of which the thread counts
+      // its own
+      constexpr int kDeep = 4;
+      for (int i0 = 4 * tid; i0 < told; i0 += 4 * kThreads * kDeep) {
+        int4u t[kDeep];
 #pragma unroll
-        for (int j = 0; j < 4; j++) count(t[j], i + j);
-      } else {
-        for (int j = i; j < told; j++) count(history[j], j);
+        for (int k = 0; k < kDeep; k++)
+          t[k] = *reinterpret_cast<const int4u *>(history + min(i0 + 4 * kThreads * k, told - 4));
+#pragma unroll
+        for (int k = 0; k < kDeep; k++) {
+          const int i = i0 + 4 * kThreads * k, from = min(i, told - 4);
+#pragma unroll
+          for (int j = 0; j < 4; j++)
+            if (from + j >= i) count(t[k][j], from + j);
+        }
       }
     }
     __syncthreads();
@@ -91,7 +106,7 @@ __global__ __launch_bounds__(THREADS) void logit_rules_kernel(const LogitRulesAr
     const float f = a.frequency ? a.frequency[row] : 0.0f, p = a.presence ? a.presence[row] : 0.0f;
 #pragma unroll
     for (int g = 0; g < kPer; g++) {
-      uint4 *at = reinterpret_cast<uint4 *>(&words[4 * (g * THREADS + tid)]);
+      uint4 *at = reinterpret_cast<uint4 *>(&words[4 * (g * kThreads + tid)]);
       const uint4 w4 = *at;
       const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
       *at = make_uint4(0, 0, 0, 0);  // the biases'
@@ -110,14 +125,14 @@ __global__ __launch_bounds__(THREADS) void logit_rules_kernel(const LogitRulesAr
     const int *ids = a.bias_ids + row * a.bias_stride;
     const float *values = a.bias_values + row * a.bias_stride;
     __syncthreads();  // every word is 0 again
-    for (int i = tid; i < biases; i += THREADS) {
+    for (int i = tid; i < biases; i += kThreads) {
       const uint32_t at = (uint32_t)ids[i] - (uint32_t)base;
       if (at < (uint32_t)left) atomicMax(&words[at], (uint32_t)i + 1);
     }
     __syncthreads();
 #pragma unroll
     for (int g = 0; g < kPer; g++) {
-      const uint4 w4 = *reinterpret_cast<const uint4 *>(&words[4 * (g * THREADS + tid)]);
+      const uint4 w4 = *reinterpret_cast<const uint4 *>(&words[4 * (g * kThreads + tid)]);
       const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
 #pragma unroll
       for (int j = 0; j < 4; j++)
@@ -126,7 +141,7 @@ __global__ __launch_bounds__(THREADS) void logit_rules_kernel(const LogitRulesAr
   }
 #pragma unroll
   for (int g = 0; g < kPer; g++) {
-    const int i = 4 * (g * THREADS + tid);
+    const int i = 4 * (g * kThreads + tid);
     float4u v;
 #pragma unroll
     for (int j = 0; j < 4; j++) v[j] = (allowed[g] >> j & 1) ? x[g][j] : -__builtin_inff();
@@ -140,22 +155,12 @@ __global__ __launch_bounds__(THREADS) void logit_rules_kernel(const LogitRulesAr
   }
 }
 
-template <int THREADS>
-hipError_t launch(const LogitRulesArgs &a, hipStream_t s) {
-  constexpr int kSlice = THREADS * 4 * kPer;
-  hipLaunchKernelGGL(logit_rules_kernel<THREADS>, dim3((a.n + kSlice - 1) / kSlice, a.rows), dim3(THREADS), 0, s, a);
-  return hipGetLastError();
-}
-
 }  // namespace
 
-hipError_t launch_logit_rules(const LogitRulesArgs &a, int num_cus, hipStream_t s) {
+hipError_t launch_logit_rules(const LogitRulesArgs &a, hipStream_t s) {
   if (a.rows < 1 || a.rows > 65535 || a.n < 1) return hipErrorInvalidValue;
-  // slices of 16384 tokens where they leave a workgroup a CU, else of 4096 or 1024
-  auto groups = [&](int slice) { return (int64_t)a.rows * ((a.n + slice - 1) / slice); };
-  if (groups(16384) >= num_cus) return launch<1024>(a, s);
-  if (groups(4096) >= num_cus) return launch<256>(a, s);
-  return launch<64>(a, s);
+  hipLaunchKernelGGL(logit_rules_kernel, dim3((a.n + kSlice - 1) / kSlice, a.rows), dim3(kThreads), 0, s, a);
+  return hipGetLastError();
 }
 
 }  // namespace hp

@@ -15,14 +15,15 @@
 // used as f32, as the rest of the arithmetic (a row's sum of squares is a tree
 // of f32 sums over the lanes that hold it).
 //
-// A workgroup takes `batch` tokens.  Its threads first form the batch's
-// angles, one (token, u) each, into LDS -- every head row of a token has the
-// same -- and then take the rows, D / 8 lanes a row: lane l holds elements
-// 4l .. 4l+3 of both halves of the rotated part (or eight consecutive ones of
-// the rest), so that a pair sits in one lane and loads and stores are 16 and 8
-// bytes wide.  Few tokens spread their rows over several workgroups, each with
-// angles of its own; many take four tokens a workgroup, so that the 64-bit
-// work stays small beside the rows.
+// A workgroup takes a token, or where tokens are few a part of its rows.  Its
+// threads first form the token's angles, one u each, into LDS -- every head row
+// has the same -- and then take the rows, D / 8 lanes a row: lane l holds
+// elements 4l .. 4l+3 of both halves of the rotated part (or eight consecutive
+// ones of the rest), so that a pair sits in one lane and loads and stores are
+// 16 and 8 bytes wide.  The first rows' loads go out before the position is
+// known.  16000 tokens of 32 + 16 head rows of 128 (655 MB in and out): 121 us,
+// 5.4 TB/s, which its bytes bound; with four tokens a workgroup 131 us, with
+// loads past the caches 138.
 #include "hp_serving.h"
 #include "hp_wave.h"
 
@@ -30,7 +31,7 @@ namespace hp {
 
 namespace {
 
-constexpr int kThreads = 256, kWaves = kThreads / 64;
+constexpr int kThreads = 256;
 constexpr float kE4m3Most = 448.0f;
 constexpr double kInvTwoPi = 0.15915494309189533577;
 
@@ -66,97 +67,91 @@ __device__ __forceinline__ void store_cache4(void *p, int64_t i, const float (&v
 }
 
 template <int D, int CT>
-__global__ __launch_bounds__(kThreads) void paged_append_kernel(const PagedAppendArgs a, int batch) {
+__global__ __launch_bounds__(kThreads) void paged_append_kernel(const PagedAppendArgs a) {
   constexpr int kLanes = D / 8;  // of a row
   constexpr int kRows = kThreads / kLanes;
-  __shared__ float2 turn[kWaves][D / 2];  // cos, sin
-  __shared__ int64_t page_at[kWaves];     // element of the token's page and slot for head 0, or -1
-  __shared__ int where[kWaves];           // position, or -1: the token's rows stay as they were
-  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
-  const int t0 = blockIdx.x * batch, page_size = 1 << a.c.page_shift;
+  __shared__ float2 angle[D / 2];  // cos, sin
+  const int tid = threadIdx.x, t = blockIdx.x, page_size = 1 << a.c.page_shift;
 
-  if (wave < batch && t0 + wave < a.tokens) {  // a wave per token of the batch (batch <= kWaves)
-    const int t = t0 + wave;
-    int seq = t, pos = -1;
-    if (a.offsets) {
-      seq = packed_sequence_of(a.offsets, a.c.sequences, t);
-      if (seq < a.c.sequences) {
-        const int begin = a.offsets[seq], end = a.offsets[seq + 1];
-        if (t >= begin && t < end) pos = append_position(a.c.lengths[seq], (int64_t)end - t, a.c.page_shift, a.c.width);
-      }
-    } else {
-      pos = append_position(a.c.lengths[seq], 1, a.c.page_shift, a.c.width);
-    }
-    int page = -1;
-    if (pos >= 0) page = page_or_none(a.c.pages[(int64_t)seq * a.c.width + (pos >> a.c.page_shift)], a.c.page_count);
-    if (lane == 0) {
-      where[wave] = pos;
-      page_at[wave] = page >= 0 ? page * a.c.page_stride + (int64_t)(pos & (page_size - 1)) * D : -1;
-    }
-  }
-  __syncthreads();
-  const int half = a.rope_dims >> 1;
-  const int live = min(batch, a.tokens - t0);
-  for (int i = tid; i < live * half; i += kThreads) {
-    const int b = i / half, u = i - b * half;
-    if (where[b] < 0) continue;
-    double turns = (double)where[b] * (exp2(a.log2_base * (-2.0 * u / a.rope_dims)) * kInvTwoPi);
-    if (a.freq_factors) turns /= (double)a.freq_factors[u];
-    double s, c;
-    sincospi(2.0 * (turns - rint(turns)), &s, &c);
-    turn[b][u] = make_float2((float)c, (float)s);
-  }
-  __syncthreads();
-
-  const int rows = a.nq + 2 * a.c.nkv;
+  // A thread's work: rows row0, row0 + step, ..., its elements at0 .. and at1 ..
+  // of a row.  The next row's loads (the last row's again at the end) are on
+  // their way while one is worked on.
+  const int rows = a.nq + 2 * a.c.nkv, half = a.rope_dims >> 1;
   const int l = tid % kLanes, u0 = 4 * l;  // the lane's four pairs
   const bool paired = u0 < half;           // (half is a multiple of 4)
   const int at0 = paired ? u0 : a.rope_dims + 2 * (u0 - half), at1 = paired ? u0 + half : at0 + 4;
+  const int row0 = blockIdx.y * kRows + tid / kLanes, step = gridDim.y * kRows;
+  float4 next0, next1;
+  auto load = [&](int row) {
+    const int r = min(row, rows - 1), hk = r - a.nq, hv = hk - a.c.nkv;  // query, key, value head
+    const float *src = hk < 0           ? a.q + t * a.q_stride + (int64_t)r * D
+                       : hv < 0 || !a.v ? a.k + t * a.k_stride + (int64_t)(hv < 0 ? hk : hv) * D
+                                        : a.v + t * a.v_stride + (int64_t)hv * D;
+    next0 = *reinterpret_cast<const float4 *>(src + at0);
+    next1 = *reinterpret_cast<const float4 *>(src + at1);
+  };
+  load(row0);
+
+  // the token's sequence, position and page (each wave for itself)
+  int seq = t, pos = -1;
+  if (a.offsets) {
+    seq = packed_sequence_of(a.offsets, a.c.sequences, t);
+    if (seq < a.c.sequences) {
+      const int begin = a.offsets[seq], end = a.offsets[seq + 1];
+      if (t >= begin && t < end) pos = append_position(a.c.lengths[seq], (int64_t)end - t, a.c.page_shift, a.c.width);
+    }
+  } else {
+    pos = append_position(a.c.lengths[seq], 1, a.c.page_shift, a.c.width);
+  }
+  if (pos < 0) return;  // (the same for the workgroup) the token's rows stay as they were
+  const int page = page_or_none(a.c.pages[(int64_t)seq * a.c.width + (pos >> a.c.page_shift)], a.c.page_count);
+  const int64_t slot_at = page * a.c.page_stride + (int64_t)(pos & (page_size - 1)) * D;  // for head 0
+  for (int u = tid; u < half; u += kThreads) {
+    double turns = (double)pos * (exp2(a.log2_base * (-2.0 * u / a.rope_dims)) * kInvTwoPi);
+    if (a.freq_factors) turns /= (double)a.freq_factors[u];
+    double s, c;
+    sincospi(2.0 * (turns - rint(turns)), &s, &c);
+    angle[u] = make_float2((float)c, (float)s);
+  }
+  __syncthreads();
+
   const float inv_k = 1.0f / a.c.key_scale, inv_v = 1.0f / a.c.value_scale;
-  for (int b = 0; b < live; b++) {
-    if (where[b] < 0) continue;
-    const int64_t t = t0 + b;
-    for (int r = blockIdx.y * kRows + tid / kLanes; r < rows; r += gridDim.y * kRows) {
-      const int kind = r < a.nq ? 0 : r < a.nq + a.c.nkv ? 1 : 2;  // query, key, value
-      const int h = kind == 0 ? r : kind == 1 ? r - a.nq : r - a.nq - a.c.nkv;
-      const float *src = kind == 0           ? a.q + t * a.q_stride
-                         : kind == 1 || !a.v ? a.k + t * a.k_stride
-                                             : a.v + t * a.v_stride;
-      src += (int64_t)h * D;
-      const float4 f0 = *reinterpret_cast<const float4 *>(src + at0), f1 = *reinterpret_cast<const float4 *>(src + at1);
-      float x[4] = {f0.x, f0.y, f0.z, f0.w}, y[4] = {f1.x, f1.y, f1.z, f1.w};
-      const float *w = kind == 0 ? a.q_norm : kind == 1 ? a.k_norm : nullptr;
-      if (w || (kind == 2 && a.norm_values)) {  // the same for the lanes of a row
-        float s = 0.0f;
+  for (int r = row0; r < rows; r += step) {  // (the same for the lanes of a row)
+    float x[4] = {next0.x, next0.y, next0.z, next0.w}, y[4] = {next1.x, next1.y, next1.z, next1.w};
+    load(r + step);
+    const int kind = r < a.nq ? 0 : r < a.nq + a.c.nkv ? 1 : 2;  // query, key, value
+    const int h = kind == 0 ? r : kind == 1 ? r - a.nq : r - a.nq - a.c.nkv;
+    const float *w = kind == 0 ? a.q_norm : kind == 1 ? a.k_norm : nullptr;
+    if (w || (kind == 2 && a.norm_values)) {  // the same for the lanes of a row
+      float s = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 4; j++) s += x[j] * x[j] + y[j] * y[j];
-        const float scale = 1.0f / sqrtf(row_sum<kLanes>(s) / (float)D + a.eps);
+      for (int j = 0; j < 4; j++) s += x[j] * x[j] + y[j] * y[j];
+      const float scale = 1.0f / sqrtf(row_sum<kLanes>(s) / (float)D + a.eps);
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-          x[j] = x[j] * scale * (w ? w[at0 + j] : 1.0f);
-          y[j] = y[j] * scale * (w ? w[at1 + j] : 1.0f);
-        }
+      for (int j = 0; j < 4; j++) {
+        x[j] = x[j] * scale * (w ? w[at0 + j] : 1.0f);
+        y[j] = y[j] * scale * (w ? w[at1 + j] : 1.0f);
       }
-      if (kind != 2 && paired) {
+    }
+    if (kind != 2 && paired) {
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-          const float2 cs = turn[b][u0 + j];
-          const float p = x[j], q = y[j];
-          x[j] = p * cs.x - q * cs.y;
-          y[j] = p * cs.y + q * cs.x;
-        }
+      for (int j = 0; j < 4; j++) {
+        const float2 cs = angle[u0 + j];
+        const float p = x[j], q = y[j];
+        x[j] = p * cs.x - q * cs.y;
+        y[j] = p * cs.y + q * cs.x;
       }
-      void *out = kind == 0 ? a.q_out : kind == 1 ? a.k_out : a.v_out;
-      if (out) {
-        const int64_t o = (t * (kind == 0 ? a.nq : a.c.nkv) + h) * D;
-        store4(out, o + at0, a.out_type, x);
-        store4(out, o + at1, a.out_type, y);
-      }
-      if (kind != 0 && page_at[b] >= 0) {
-        const int64_t o = page_at[b] + (int64_t)h * page_size * D;
-        store_cache4<CT>(kind == 1 ? a.c.keys : a.c.values, o + at0, x, kind == 1 ? inv_k : inv_v);
-        store_cache4<CT>(kind == 1 ? a.c.keys : a.c.values, o + at1, y, kind == 1 ? inv_k : inv_v);
-      }
+    }
+    void *out = kind == 0 ? a.q_out : kind == 1 ? a.k_out : a.v_out;
+    if (out) {
+      const int64_t o = ((int64_t)t * (kind == 0 ? a.nq : a.c.nkv) + h) * D;
+      store4(out, o + at0, a.out_type, x);
+      store4(out, o + at1, a.out_type, y);
+    }
+    if (kind != 0 && page >= 0) {
+      const int64_t o = slot_at + (int64_t)h * page_size * D;
+      store_cache4<CT>(kind == 1 ? a.c.keys : a.c.values, o + at0, x, kind == 1 ? inv_k : inv_v);
+      store_cache4<CT>(kind == 1 ? a.c.keys : a.c.values, o + at1, y, kind == 1 ? inv_k : inv_v);
     }
   }
 }
@@ -164,18 +159,15 @@ __global__ __launch_bounds__(kThreads) void paged_append_kernel(const PagedAppen
 template <int D>
 hipError_t launch_width(const PagedAppendArgs &a, int num_cus, hipStream_t s) {
   const int passes = (a.nq + 2 * a.c.nkv + kThreads * 8 / D - 1) / (kThreads * 8 / D);
-  // four tokens a workgroup once that leaves four workgroups a CU
-  const int batch = a.tokens >= 16 * num_cus ? kWaves : 1;
-  const int groups = (a.tokens + batch - 1) / batch;
-  int split = (4 * num_cus + groups - 1) / groups;
-  split = split < 1 ? 1 : split > passes ? passes : split;
-  const dim3 grid(groups, split);
+  int split = (4 * num_cus + a.tokens - 1) / a.tokens;  // four workgroups a CU
+  split = split > passes ? passes : split;
+  const dim3 grid(a.tokens, split);
   if (a.c.type == kElemF16)
-    hipLaunchKernelGGL((paged_append_kernel<D, kElemF16>), grid, dim3(kThreads), 0, s, a, batch);
+    hipLaunchKernelGGL((paged_append_kernel<D, kElemF16>), grid, dim3(kThreads), 0, s, a);
   else if (a.c.type == kElemBf16)
-    hipLaunchKernelGGL((paged_append_kernel<D, kElemBf16>), grid, dim3(kThreads), 0, s, a, batch);
+    hipLaunchKernelGGL((paged_append_kernel<D, kElemBf16>), grid, dim3(kThreads), 0, s, a);
   else
-    hipLaunchKernelGGL((paged_append_kernel<D, kElemE4m3>), grid, dim3(kThreads), 0, s, a, batch);
+    hipLaunchKernelGGL((paged_append_kernel<D, kElemE4m3>), grid, dim3(kThreads), 0, s, a);
   return hipGetLastError();
 }
 

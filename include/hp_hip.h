@@ -562,7 +562,7 @@ typedef struct hp_hip_paged_append {
   const float *d_q_norm, *d_k_norm;   /* [head_dim], or NULL: no norm */
   const float *d_rope_freq_factors;   /* [rope_dims / 2], or NULL */
   void *d_q_out, *d_k_out, *d_v_out;  /* [token][heads][head_dim] of out_type; d_k_out, d_v_out may be NULL */
-  size_t token_count;    /* rows, those behind the last sequence among them */
+  size_t token_count;    /* rows, up to 2^23, those behind the last sequence among them */
   int32_t head_count;    /* query heads; a multiple of head_count_kv */
   int32_t out_type;      /* HP_ELEM_F32, HP_ELEM_F16 or HP_ELEM_BF16 */
   int32_t norm_values;   /* 1: values have the norm without a weight (rmsNormRowsNoWeight) */

@@ -221,7 +221,7 @@ def test_append_one_token_each(hip, S):
 
 
 def test_append_many_tokens_and_sequences(hip, S):
-    """Four tokens a workgroup, a search over more than 64 sequences in two rounds, and empty ones among them."""
+    """A search over more than 64 sequences in two rounds, and empty ones among them."""
     rng = np.random.default_rng(3)
     new = rng.integers(0, 90, 150)
     new[10:20] = 0
@@ -585,7 +585,7 @@ def test_rules_widths(hip, S, n):
 
 @pytest.mark.parametrize("rows,n", [(1, 262144), (20, 100003), (300, 20011), (70, 65536)])
 def test_rules_slices(hip, S, rows, n):
-    """Each of the slice lengths, at row widths that start rows anywhere."""
+    """Many slices, at row widths that start rows anywhere."""
     run_rules(S, rows, n, history=100, biases=7, mask=0.9, seed=rows)
 
 

@@ -91,7 +91,7 @@ def test_bad_caches(change, code):
     ({"head_count": -2}, HEADS), ({"d_q": None}, ARG), ({"d_q_out": None}, ARG), ({"d_k": None}, ARG),
     ({"rope_dims": 12}, SHAPE), ({"rope_dims": 72}, SHAPE), ({"rope_dims": -8}, SHAPE), ({"rope_freq_base": 0.0}, ARG),
     ({"rope_freq_base": NAN}, ARG), ({"epsilon": -1.0}, ARG), ({"epsilon": INF}, ARG), ({"token_count": 2}, SHAPE),
-    ({"token_count": (1 << 30) + 1, "d_offsets": P}, SHAPE), ({"q_stride": 255}, SHAPE), ({"q_stride": 258}, ARG),
+    ({"token_count": (1 << 23) + 1, "d_offsets": P}, SHAPE), ({"q_stride": 255}, SHAPE), ({"q_stride": 258}, ARG),
     ({"k_stride": 127}, SHAPE), ({"v_stride": 130}, ARG), ({"v_stride": 1 << 48}, SHAPE), ({"d_q": P + 4}, ARG),
     ({"d_v": P + 8}, ARG), ({"d_k_out": P + 4}, ARG)])
 def test_bad_appends(change, code):
