@@ -26,9 +26,7 @@ HP_PAGES_FN int append_position(int length, int64_t behind, int page_shift, int 
   return p >= 0 && (p >> page_shift) < width ? (int)p : -1;
 }
 
-constexpr int kPagedSub = 32;                // keys of a wave's step of the paged attention
-constexpr int kPagedWaves = 4;
-constexpr int kPagedStep = kPagedSub * kPagedWaves;
+constexpr int kPagedWaves = 4;  // waves of a workgroup of the paged attention, side by side along the keys
 
 // A sequence's keys first .. end - 1, and where the walk over them begins: at
 // a multiple of 16, so that 16 keys on end share a page.
@@ -42,7 +40,8 @@ HP_PAGES_FN KeySpan key_span(int length, int64_t table_keys, int window) {
   s.begin = s.first & ~15;
   return s;
 }
-HP_PAGES_FN uint32_t span_steps(const KeySpan &s) { return (uint32_t)((s.end - s.begin + kPagedStep - 1) / kPagedStep); }
+// Steps of `step` keys (a power of two) that the walk takes.
+HP_PAGES_FN uint32_t span_steps(const KeySpan &s, int step) { return (uint32_t)(s.end - s.begin + step - 1) / (uint32_t)step; }
 
 // Share i of `shares` (<= total) of the steps 0 .. total - 1 begins here, and
 // the share that step t is in: the first total % shares shares have one step

@@ -50,13 +50,21 @@ namespace {
 
 constexpr int kWaves = kPagedWaves, kThreads = 64 * kWaves;
 constexpr int kHeads = 8;  // query heads of a row
-constexpr int kSub = kPagedSub, kStep = kPagedStep;
+
+// 16-key tiles of a wave's step: heads of 256 take one where two would not fit
+// the registers beside the sums (8 / 2 heads of 256 over 28 contexts up to 4096:
+// f16 30.2 -> 27.9 us, bf16 pages with f32 queries 39.2 -> 29.0).
+__host__ __device__ constexpr int tiles_of(int head_dim, int type) { return head_dim == 256 && type != kElemE4m3 ? 1 : 2; }
+// Keys of a step of every wave.
+__host__ __device__ constexpr int step_of(int head_dim, int type) { return 16 * tiles_of(head_dim, type) * kWaves; }
 constexpr float kLog2e = 1.44269504088896341f;
 constexpr float kBias = 10.0f;  // p carries 2^kBias
 constexpr float kNegInf = -__builtin_inff();
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef short short4v __attribute__((ext_vector_type(4)));
+typedef _Float16 half4v __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ KeySpan span_of(const PagedAttnArgs &a, int seq) {
   return key_span(a.c.lengths[seq], (int64_t)a.c.width << a.c.page_shift, a.window);
@@ -80,6 +88,17 @@ __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
   if (CT == kElemBf16)
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
+}
+
+// The same with the k index over 32 keys (four dwords) or 16 (two).
+template <int CT, int N>
+__device__ __forceinline__ f32x4 mfma_keys(const uint32_t (&a)[N], const uint32_t (&b)[N], f32x4 c) {
+  if (N == 4)
+    return mfma16<CT>((u32x4){a[0], a[1], a[2 % N], a[3 % N]}, (u32x4){b[0], b[1], b[2 % N], b[3 % N]}, c);
+  const uint2 x = make_uint2(a[0], a[1]), y = make_uint2(b[0], b[1]);
+  if (CT == kElemBf16)
+    return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(short4v, x), __builtin_bit_cast(short4v, y), c, 0, 0, 0);
+  return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(half4v, x), __builtin_bit_cast(half4v, y), c, 0, 0, 0);
 }
 
 // The operand type's bits of v, and the value they stand for.
@@ -124,15 +143,16 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
   return dpp_add<0x143, 0xc>(v);      // lane 31's into rows 2 and 3
 }
 
-// A lane's elements of a key tile's row (D / 32 operand fragments) and of the
-// eight value rows (D / 16 elements each), as loaded.
+// A lane's elements of a key row of each tile (D / 32 operand fragments) and of
+// the four value rows of each (D / 16 elements each), as loaded.
 template <int D, int CT>
 struct Tile {
   static constexpr int kE = CT == kElemE4m3 ? 1 : 2;   // bytes an element
+  static constexpr int kTiles = tiles_of(D, CT), kKeys = 4 * kTiles;  // of a lane's values
   static constexpr int kKeyWords = D * kE / 4 / 4;     // dwords of a quarter key row
   static constexpr int kValueWords = D * kE / 16 / 4;  // dwords of a sixteenth of a value row
-  uint32_t k[2][kKeyWords];
-  uint32_t v[8][kValueWords];
+  uint32_t k[kTiles][kKeyWords];
+  uint32_t v[kKeys][kValueWords];
 };
 
 // (STREAM: not to stay in the caches)
@@ -158,6 +178,7 @@ template <int D, int CT, bool THIRD, bool STREAM>
 __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(const PagedAttnArgs a, RowParts *__restrict__ rows,
                                                                  Part<D> *__restrict__ parts) {
   using T = Tile<D, CT>;
+  constexpr int kTiles = T::kTiles, kKeys = T::kKeys, kSub = 16 * kTiles, kStep = kSub * kWaves;
   constexpr int kE = T::kE, kFrags = D / 32, kRowBytes = D * kE, kT = D / 16;
   __shared__ float4 sh_o[kWaves][kHeads][D / 4];
   __shared__ u32x4 sh_q[THIRD ? 2 : 1][kFrags][64];  // the query's operand fragments, the same for every wave
@@ -174,7 +195,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(const PagedAttn
   uint32_t mine = 0;
   for (int i = 0; i < run; i++) {
     const int s = lane * run + i;
-    if (s < a.c.sequences) mine += span_steps(span_of(a, s));
+    if (s < a.c.sequences) mine += span_steps(span_of(a, s), kStep);
   }
   uint32_t before = wave_scan(mine);
   const uint32_t total = (uint32_t)__builtin_amdgcn_readlane((int)before, 63) * units;
@@ -189,7 +210,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(const PagedAttn
   uint32_t start = before;
   if (run > 1 && mine_is)
     for (;; place++) {
-      const uint32_t n = span_steps(span_of(a, place)) * units;
+      const uint32_t n = span_steps(span_of(a, place), kStep) * units;
       if (at - start < n) break;
       start += n;
     }
@@ -203,7 +224,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(const PagedAttn
 
   while (at < stop) {
     const KeySpan span = span_of(a, seq);
-    const uint32_t steps = span_steps(span);
+    const uint32_t steps = span_steps(span, kStep);
     if (at - seq_start >= steps * units) {  // (also past sequences without a key)
       seq_start += steps * units;
       seq++;
@@ -240,7 +261,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(const PagedAttn
     for (int t = 0; t < kT; t++) acc[t] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
     float m_run = kNegInf, l_part = 0.0f;
 
-    // this wave's tiles: key .. key + 31 at key = begin + kStep i + kSub wave
+    // this wave's tiles: key .. key + kSub - 1 at key = begin + kStep i + kSub wave
     const int key0 = span.begin + (int)i0 * kStep + kSub * wave;
     const int key_stop = min(span.end, span.begin + (int)(i0 + n) * kStep);
     const int *table = a.c.pages + (int64_t)seq * a.c.width;
@@ -261,51 +282,43 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(const PagedAttn
       return (max(page, 0) * a.c.page_stride + head_at + (int64_t)(key & page_mask) * D) * kE;
     };
     T t;
-    auto load_keys = [&](int key, int p0, int p1) {
-      const int64_t b0 = tile_at(p0, key), b1 = tile_at(p1, key + 16);
-      if (CT == kElemE4m3) {
-        // 16 bytes are the lane's elements of two fragments
-        constexpr int kN = D / 64;
+    // (fp8: 16 bytes are the lane's elements of two fragments)
+    auto load_keys = [&](int key, const int (&pages)[kTiles]) {
 #pragma unroll
-        for (int i = 0; i < kN; i++) {
-          const int off = c16 * kRowBytes + 64 * i + 16 * q4;
+      for (int h = 0; h < kTiles; h++) {
+        const uint8_t *rows = keys + tile_at(pages[h], key + 16 * h);
+#pragma unroll
+        for (int i = 0; i < T::kKeyWords / 4; i++) {
           uint32_t w[4];
-          load_words<STREAM>(w, keys + b0 + off);
+          load_words<STREAM>(w, rows + c16 * kRowBytes + 64 * i + 16 * q4);
 #pragma unroll
-          for (int j = 0; j < 4; j++) t.k[0][4 * i + j] = w[j];
-          load_words<STREAM>(w, keys + b1 + off);
-#pragma unroll
-          for (int j = 0; j < 4; j++) t.k[1][4 * i + j] = w[j];
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < kFrags; i++) {
-          const int off = c16 * kRowBytes + 64 * i + 16 * q4;
-          uint32_t w[4];
-          load_words<STREAM>(w, keys + b0 + off);
-#pragma unroll
-          for (int j = 0; j < 4; j++) t.k[0][(4 * i + j) % T::kKeyWords] = w[j];
-          load_words<STREAM>(w, keys + b1 + off);
-#pragma unroll
-          for (int j = 0; j < 4; j++) t.k[1][(4 * i + j) % T::kKeyWords] = w[j];
+          for (int j = 0; j < 4; j++) t.k[h][4 * i + j] = w[j];
         }
       }
     };
-    auto load_values = [&](int key, int p0, int p1) {
-      const int64_t b0 = tile_at(p0, key), b1 = tile_at(p1, key + 16);
+    auto load_values = [&](int key, const int (&pages)[kTiles]) {
 #pragma unroll
-      for (int j = 0; j < 8; j++)
-        load_words<STREAM>(t.v[j], values + (j < 4 ? b0 : b1) + (4 * q4 + (j & 3)) * kRowBytes + c16 * kT * kE);
+      for (int j = 0; j < kKeys; j++)
+        load_words<STREAM>(t.v[j], values + tile_at(pages[j >> 2], key + 16 * (j >> 2)) +
+                                       (4 * q4 + (j & 3)) * kRowBytes + c16 * kT * kE);
+    };
+    int entries[kTiles], page[kTiles];
+    auto load_entries = [&](int key) {
+#pragma unroll
+      for (int h = 0; h < kTiles; h++) entries[h] = entry_of(key + 16 * h);
+    };
+    auto pages_of = [&](int key, int (&pages)[kTiles]) {
+#pragma unroll
+      for (int h = 0; h < kTiles; h++) pages[h] = page_of(key + 16 * h, entries[h]);
     };
 
     // (a wave whose keys are all behind the end loads its first tile for nothing)
     int key = key0;
-    int e0 = entry_of(key), e1 = entry_of(key + 16);
-    int p0 = page_of(key, e0), p1 = page_of(key + 16, e1);
-    e0 = entry_of(key + kStep);
-    e1 = entry_of(key + kStep + 16);
-    load_keys(key, p0, p1);
-    load_values(key, p0, p1);
+    load_entries(key);
+    pages_of(key, page);
+    load_entries(key + kStep);
+    load_keys(key, page);
+    load_values(key, page);
 
     // the query in parts, while the first keys are on their way
     float x[kMine][8];
@@ -381,11 +394,12 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(const PagedAttn
       constexpr bool kMore = !decltype(last)::value;
       // the query's fragments are read anew in every step where in registers they
       // would not fit
-      if (D == 256 && CT != kElemE4m3) asm volatile("" ::: "memory");
+      if (D == 256 && THIRD) asm volatile("" ::: "memory");
       const int next = key + kStep;
-      f32x4 s[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+      f32x4 s[kTiles];
 #pragma unroll
-      for (int h = 0; h < 2; h++)
+      for (int h = 0; h < kTiles; h++) {
+        s[h] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int f = 0; f < kFrags; f++) {
           u32x4 kf;
@@ -401,33 +415,36 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(const PagedAttn
           s[h] = mfma16<CT>(kf, sh_q[0][f][lane], s[h]);
           if (THIRD) s[h] = mfma16<CT>(kf, sh_q[THIRD ? 1 : 0][f][lane], s[h]);
         }
-      // the next keys stream in while these are worked on
-      int np0 = 0, np1 = 0;
-      if (kMore) {
-        np0 = page_of(next, e0);
-        np1 = page_of(next + 16, e1);
-        e0 = entry_of(next + kStep);
-        e1 = entry_of(next + kStep + 16);
-        load_keys(next, np0, np1);
       }
-      const bool edge = key < span.first || key + kSub > span.end || p0 < 0 || p1 < 0;
-      float x[8];
+      // the next keys stream in while these are worked on
+      int next_page[kTiles];
+      if (kMore) {
+        pages_of(next, next_page);
+        load_entries(next + kStep);
+        load_keys(next, next_page);
+      }
+      bool edge = key < span.first || key + kSub > span.end;
 #pragma unroll
-      for (int j = 0; j < 8; j++) {
+      for (int h = 0; h < kTiles; h++) edge = edge || page[h] < 0;
+      float x[kKeys];
+#pragma unroll
+      for (int j = 0; j < kKeys; j++) {
         const float v = s[j >> 2][j & 3];
         x[j] = (v + dpp_f32<kDppRor8>(v)) * factor;
       }
       if (edge) {  // the same for the wave
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
+        for (int j = 0; j < kKeys; j++) {
           const int at_key = key + 16 * (j >> 2) + 4 * q4 + (j & 3);
-          const bool off = at_key < span.first || at_key >= span.end || (j < 4 ? p0 : p1) < 0;
+          const bool off = at_key < span.first || at_key >= span.end || page[j >> 2] < 0;
           x[j] = off ? kNegInf : x[j];
 #pragma unroll
           for (int w = 0; w < T::kValueWords; w++) t.v[j][w] = off ? 0u : t.v[j][w];
         }
       }
-      float most = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+      float most = x[0];
+#pragma unroll
+      for (int j = 1; j < kKeys; j++) most = fmaxf(most, x[j]);
       most = column_max(most);
       if (__any(most > m_run)) {
         const float m_new = fmaxf(m_run, most);
@@ -439,24 +456,24 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(const PagedAttn
       }
       // a row without a key so far: exp2(-inf - 0) = 0
       const float m_use = m_run == kNegInf ? 0.0f : m_run - kBias;
-      u32x4 pf;
+      uint32_t pf[kKeys / 2];
       const bool rest = c16 >= kHeads;
-      uint32_t pb[8];
+      uint32_t pb[kKeys];
 #pragma unroll
-      for (int j = 0; j < 8; j++) {
+      for (int j = 0; j < kKeys; j++) {
         const float p = __builtin_amdgcn_exp2f(x[j] - m_use);
         l_part += p;
         const uint32_t hi = part_bits<CT>(p), lo = part_bits<CT>(p - part_value<CT>(hi));
         pb[j] = rest ? lo : hi;
       }
 #pragma unroll
-      for (int w = 0; w < 4; w++) pf[w] = pb[2 * w] | pb[2 * w + 1] << 16;
-      // V^T fragments: element i of the lane's D / 16 from eight keys
+      for (int w = 0; w < kKeys / 2; w++) pf[w] = pb[2 * w] | pb[2 * w + 1] << 16;
+      // V^T fragments: element i of the lane's D / 16 from each of its keys
 #pragma unroll
       for (int i = 0; i < kT; i++) {
-        u32x4 vf;
+        uint32_t vf[kKeys / 2];
 #pragma unroll
-        for (int w = 0; w < 4; w++) {
+        for (int w = 0; w < kKeys / 2; w++) {
           const uint32_t sel = (i & 1) ? 0x07060302u : 0x05040100u;
           if (CT == kElemE4m3) {
             const uint32_t a0 = t.v[2 * w][i >> 2], a1 = t.v[2 * w + 1][i >> 2];
@@ -468,12 +485,12 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(const PagedAttn
             vf[w] = __builtin_amdgcn_perm(t.v[2 * w + 1][(i >> 1) % kN], t.v[2 * w][(i >> 1) % kN], sel);
           }
         }
-        acc[i] = mfma16<CT>(vf, pf, acc[i]);
+        acc[i] = mfma_keys<CT>(vf, pf, acc[i]);
       }
       if (kMore) {
-        load_values(next, np0, np1);
-        p0 = np0;
-        p1 = np1;
+        load_values(next, next_page);
+#pragma unroll
+        for (int h = 0; h < kTiles; h++) page[h] = next_page[h];
       }
     };
     if (key < key_stop) {
@@ -555,7 +572,7 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(const PagedAttnAr
   const int tid = threadIdx.x, sub = tid / kPer, d = tid - sub * kPer;
   const int64_t out = seq * a.out_stride + (int64_t)head * D + 4 * d;
   const RowParts r = rows[((int64_t)seq * a.c.nkv + kvh) * blocks + in_group / kHeads];  // (of an earlier launch without a key)
-  if (span_steps(span_of(a, seq)) == 0) {  // no key: zeros
+  if (span_of(a, seq).end == 0) {  // no key: zeros
     const float zero[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     if (sub == 0) store4(a.out, out, a.out_type, zero);
     return;
@@ -665,7 +682,8 @@ size_t part_bytes(int head_dim) { return (size_t)kHeads * (head_dim + 2) * sizeo
 uint64_t paged_attn_most_steps(const PagedAttnArgs &a) {
   uint64_t keys = (uint64_t)a.c.width << a.c.page_shift;
   if (a.window > 0 && keys > (uint64_t)a.window + 15) keys = (uint64_t)a.window + 15;
-  return (keys + kStep - 1) / kStep * a.c.sequences * a.c.nkv * blocks_of(a.nq, a.c.nkv);
+  const int step = step_of(a.c.head_dim, a.c.type);
+  return (keys + step - 1) / step * a.c.sequences * a.c.nkv * blocks_of(a.nq, a.c.nkv);
 }
 
 int paged_attn_groups(const PagedAttnArgs &a, int num_cus) {

@@ -34,9 +34,11 @@ int main() {
       const int end = length < 0 ? 0 : length > 512 ? 512 : length;
       CHECK(s.end == end && s.first == (window > 0 && end > window ? end - window : 0));
       CHECK(s.begin <= s.first && s.first - s.begin < 16 && s.begin % 16 == 0);
-      CHECK((span_steps(s) == 0) == (end == 0));
-      CHECK((uint64_t)s.begin + span_steps(s) * (uint64_t)kPagedStep >= (uint64_t)end);
-      if (window > 0) CHECK(span_steps(s) <= ((uint64_t)window + 15 + kPagedStep - 1) / kPagedStep);
+      for (int step : {64, 128}) {
+        CHECK((span_steps(s, step) == 0) == (end == 0));
+        CHECK((uint64_t)s.begin + span_steps(s, step) * (uint64_t)step >= (uint64_t)end);
+        if (window > 0) CHECK(span_steps(s, step) <= ((uint64_t)window + 15 + step - 1) / step);
+      }
     }
 
   // shares: together every step once, none empty, and each step's share is found
