@@ -178,7 +178,7 @@ __global__ __launch_bounds__(kThreads, D * G >= 256 ? 1 : 2) void packed_attn_ke
   if (unit >= slots * a.nkv) return;
   const int slot = slots - 1 - unit / a.nkv, kvh = unit % a.nkv, head = kvh * group + r % group;
 
-  int seq;
+  int seq, begin, end;
   {
     int lo = 0, n = a.sequences;  // the largest whose first block is not behind `slot`
     while (n > 64) {
@@ -188,11 +188,13 @@ __global__ __launch_bounds__(kThreads, D * G >= 256 ? 1 : 2) void packed_attn_ke
       lo += c * step;
       n = min(step, n - c * step);
     }
-    const int at = lo + min(lane, n - 1);
-    const bool le = lane < n && packed_first_block(a.offsets[at], at, kRows) <= slot;
-    seq = lo + max(__popcll(__ballot(le)), 1) - 1;
+    const int at = lo + min(lane, n - 1), o0 = a.offsets[at], o1 = a.offsets[at + 1];
+    const bool le = lane < n && packed_first_block(o0, at, kRows) <= slot;
+    const int c = max(__popcll(__ballot(le)), 1) - 1;
+    seq = lo + c;
+    begin = __builtin_amdgcn_readlane(o0, c);
+    end = min(__builtin_amdgcn_readlane(o1, c), a.tokens);
   }
-  const int begin = a.offsets[seq], end = min(a.offsets[seq + 1], a.tokens);
   if (begin < 0 || begin >= end) return;
   const int64_t row_at = (slot - packed_first_block(begin, seq, kRows)) * kRows;
   const int len = end - begin;
@@ -285,10 +287,15 @@ __global__ __launch_bounds__(kThreads, D * G >= 256 ? 1 : 2) void packed_attn_ke
       }
     }
   };
+  // Whether a row of the wave has a masked key in the tile at `key` (the same for
+  // the wave).
+  auto edge_at = [&](int key) {
+    return key + kKeys - 1 > wave0 || key < wave0 + kWaveRows - min(wave0 + kWaveRows, window);
+  };
   // settle: masks them and moves the running maximum where they pass it.
   auto settle = [&](f32x16 (&s)[kSubs], int key, auto edge) {
     constexpr bool kMasked = decltype(edge)::value;
-    if (kMasked) {
+    if (kMasked && edge_at(key)) {
       // the lane's key 32 u + 8 (i / 4) + i % 4 of the tile, from its first
       const int to = row - key - 4 * h, from = first - key - 4 * h;
 #pragma unroll
@@ -457,7 +464,7 @@ __global__ __launch_bounds__(kThreads, D * G >= 256 ? 1 : 2) void packed_attn_ke
     if (sees(i)) {
       u32x4 p[2 * kSubs];
       weigh(sa, p);
-      gather(p, i & 1, i < whole_first || i >= whole_stop, std::true_type{});
+      gather(p, i & 1, edge_at(key_of(i)), std::true_type{});
     }
     if (more) {
       settle(sb, key_of(i + 1), std::true_type{});
