@@ -514,7 +514,8 @@ int32_t hp_hip_set_fused_trace(uint64_t *d_stamps, size_t len);
  * `stream` (NULL = library stream; hipStreamPerThread: HP_ERR_ARG, its scratch
  * could not be told apart by thread).  Lengths, offsets and page tables are
  * read on the device when the kernels run, so a captured call serves every
- * batch of its shape.  The arguments are checked on the host before anything
+ * batch of its shape; like the other inputs they stay as they are while a call
+ * runs.  The arguments are checked on the host before anything
  * is launched; nothing in a device array can lead a kernel out of the buffers
  * that the arguments describe.  Outputs must not overlap inputs except where
  * it says so.  Rows of 16-bit and fp8 elements, and f32 rows that are read or

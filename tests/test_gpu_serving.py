@@ -305,6 +305,35 @@ def test_paged_types(hip, S, D, type, q_type, out):
     run_paged(S, Pool(rng, LENGTHS, 2, D, 16, type), 8, q_type, out, rng=rng)
 
 
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("type,q_type", [("f16", "f32"), ("bf16", "f32"), ("bf16", "bf16"), ("e4m3", "f16")])
+def test_paged_wide_tables(hip, S, D, type, q_type):
+    """Tables with room for more than the caches hold: the loads go past them."""
+    rng = np.random.default_rng(D)
+    run_paged(S, Pool(rng, [1, 0, 129, 700, 64], 2, D, 16, type, extra=(33 << 20) // (2 * 2 * D * 5 * 16)), 8, q_type, rng=rng)
+
+
+def test_paged_offsets_past_32_bits(hip, S):
+    """Pages two gigabytes apart."""
+    t = _torch()
+    rng = np.random.default_rng(14)
+    pool = Pool(rng, [40, 17], 1, 64, 16, "f16", spare=0, extra=0)
+    stride = 1 << 30  # elements
+    far = t.empty(pool.count * stride, dtype=t.float16, device="cuda")
+    keys, values_ = far.view(pool.count, stride)[:, :1024], far.view(pool.count, stride)[:, 1 << 29:(1 << 29) + 1024]
+    keys.copy_(pool.keys.reshape(pool.count, -1))
+    values_.copy_(pool.values.reshape(pool.count, -1))
+    pool.keys, pool.values, pool.stride = keys.view(pool.count, 1, 16, 64), values_.view(pool.count, 1, 16, 64), stride
+    run_paged(S, pool, 2, rng=rng)
+    # and a row appended there
+    row = dev(np.ones((2, 1, 64), np.float32))
+    H.paged_append_device(pool.cache(), 2, 0, 0, row.data_ptr(), 0, 0, 0)
+    sync()
+    for s, n in enumerate((40, 17)):
+        assert bool((pool.keys[pool.pages[s, (n - 1) // 16], 0, (n - 1) % 16] == 1).all())
+        assert bool((pool.values[pool.pages[s, (n - 1) // 16], 0, (n - 1) % 16] == 1).all())
+
+
 @pytest.mark.parametrize("Hq,kv", [(1, 1), (2, 1), (3, 1), (7, 1), (8, 1), (9, 1), (16, 1), (21, 1), (5, 5), (14, 2), (40, 8)])
 def test_paged_groups(hip, S, Hq, kv):
     rng = np.random.default_rng(Hq)
@@ -519,6 +548,23 @@ def test_packed_later_rows_do_not_reach_back(hip, S, type, D):
     run_packed(S, [200], 2, 1, D, type, window=40, spoil=spoil_window)
 
 
+def test_packed_strides_past_32_bits(hip, S):
+    """Rows sixteen megabytes apart: the last ones lie past four gigabytes."""
+    t = _torch()
+    T, stride = 300, (1 << 23)
+    far = t.empty(T * stride, dtype=t.float16, device="cuda").view(T, stride)
+    near = t.randn(T, 3, 64, device="cuda").half()
+    far[:, :192] = near.view(T, -1)
+    offsets = dev(np.array([0, 300], np.int32))
+    outs = [t.zeros(T, 1, 64, dtype=t.float16, device="cuda") for _ in range(2)]
+    for x, o, step in ((far, outs[0], stride), (near, outs[1], 192)):
+        p = x.data_ptr()
+        H.packed_attention_device(1, offsets.data_ptr(), T, 1, 1, 64, p, p + 128, p + 256, 1, o.data_ptr(), 1, scale=0.125,
+                                  q_stride=step, k_stride=step, v_stride=step)
+    sync()
+    assert t.equal(*outs) and bool(outs[0].any())
+
+
 def test_packed_bad_offsets_stay_inside(hip):
     """Offsets that fall, or point outside the batch, name no row outside it (the result of their sequences is open)."""
     t = _torch()
@@ -595,6 +641,21 @@ def test_rules_slices(hip, S, rows, n):
                                 {"in_place": True, "mask": 0.5, "history": 5000}])
 def test_rules_alone_and_together(hip, S, kw):
     run_rules(S, 4, 1303, **kw)
+
+
+def test_rules_rows_past_32_bits(hip):
+    t = _torch()
+    stride, n = 1 << 30, 5000
+    x = t.empty(3 * stride, device="cuda").view(3, stride)
+    x[:, :n] = 2.0
+    history, one = dev(np.array([[7], [8], [9]], np.int32)), dev(np.ones(3, np.int32))
+    r = dev(np.full(3, 4.0, np.float32))
+    H.logit_rules_device(3, n, x.data_ptr(), x.data_ptr(), d_history=history.data_ptr(), history_stride=1,
+                         d_history_lengths=one.data_ptr(), d_repetition=r.data_ptr(), logits_stride=stride, output_stride=stride)
+    sync()
+    ref = t.full((3, n), 2.0, device="cuda")
+    ref[[0, 1, 2], [7, 8, 9]] = 0.5
+    assert t.equal(x[:, :n], ref)
 
 
 def test_rules_odd_values(hip, S):
