@@ -48,7 +48,7 @@ struct PagedAttnArgs {
   float scale;
   float *partials;  // paged_attn_scratch_bytes
 };
-// Workgroups of a launch, which the scratch goes by (the lengths are on the
+// Shares of a launch's keys, which the scratch goes by (the lengths are on the
 // device, so neither depends on them).
 int paged_attn_groups(const PagedAttnArgs &a, int num_cus);
 size_t paged_attn_scratch_bytes(const PagedAttnArgs &a, int groups);

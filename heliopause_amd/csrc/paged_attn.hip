@@ -31,16 +31,19 @@
 // Masked keys (behind the length, before the window, on an absent page) get
 // score -inf and value zero, whatever their slots hold.
 //
-// Split.  All (sequence, KV head, eight query heads) rows' steps of 128 keys
-// (32 for each of the four waves) lie end to end, and each workgroup takes an
-// equal share of that line, whatever the lengths are: 48 ragged contexts and
-// two of 131072 fill the card alike, and a captured launch serves every batch.
-// A workgroup finds its place by a scan of the lengths.  A row that one
-// workgroup finishes is written at once; parts of the others go to scratch,
-// at most two a workgroup, and the merge launch joins them in their order
-// (joined by the workgroup that comes last instead, with stores and loads that
-// cross the XCDs, one context of 4096 took 18.8 us for 13.9 then, and larger
-// batches the same).
+// Split.  All (sequence, KV head) rows' steps of 128 keys (32 for each of the
+// four waves; heads of 256 half as many) lie end to end, and each workgroup
+// takes an equal share of that line with eight of a group's heads, whatever the
+// lengths are: 48 ragged contexts and two of 131072 fill the card alike, and a
+// captured launch serves every batch.  A workgroup finds its place by a scan of
+// the lengths.  A row that one workgroup finishes is written at once; parts of
+// the others go to scratch, at most two a workgroup, and the merge launch joins
+// them in their order.  A group's further heads are workgroups beside one
+// another on one XCD, whose L2 has the keys for the second (24 / 2 heads of 256
+// over 20 contexts up to 6000: 26.2 us, with the blocks along the line 35.0).
+// Not kept: parts joined by the workgroup that comes last, with stores and loads
+// that cross the XCDs (one context of 4096 18.8 us for 13.9 then, larger batches
+// the same).
 //
 // 48 contexts up to 8192, 32 / 8 heads of 128, bf16: 660 MB in 108 us, 6.1 TB/s,
 // of which the merge launch is 5; two of 131072, f16: 419 MB in 69.5 us; 130
@@ -66,6 +69,7 @@ constexpr int kHeads = 8;  // query heads of a row
 __host__ __device__ constexpr int tiles_of(int head_dim, int type) { return head_dim == 256 && type != kElemE4m3 ? 1 : 2; }
 // Keys of a step of every wave.
 __host__ __device__ constexpr int step_of(int head_dim, int type) { return 16 * tiles_of(head_dim, type) * kWaves; }
+constexpr int kXcds = 8;  // workgroup i runs on XCD i % 8
 constexpr float kLog2e = 1.44269504088896341f;
 constexpr float kBias = 10.0f;  // p carries 2^kBias
 constexpr float kNegInf = -__builtin_inff();
@@ -185,7 +189,7 @@ __device__ __forceinline__ void load_words(uint32_t (&d)[N], const uint8_t *p) {
 
 template <int D, int CT, bool THIRD, bool STREAM>
 __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(const PagedAttnArgs a, RowParts *__restrict__ rows,
-                                                                 Part<D> *__restrict__ parts) {
+                                                                 Part<D> *__restrict__ parts, int groups) {
   using T = Tile<D, CT>;
   constexpr int kTiles = T::kTiles, kKeys = T::kKeys, kSub = 16 * kTiles, kStep = kSub * kWaves;
   constexpr int kE = T::kE, kFrags = D / 32, kRowBytes = D * kE, kT = D / 16;
@@ -195,7 +199,11 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(const PagedAttn
   __shared__ float sh_most[kWaves][16];  // largest elements of the query rows
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int q4 = lane >> 4, c16 = lane & 15;
-  const int group = a.nq / a.c.nkv, blocks = blocks_of(a.nq, a.c.nkv), units = a.c.nkv * blocks;
+  const int group = a.nq / a.c.nkv, blocks = blocks_of(a.nq, a.c.nkv), units = a.c.nkv;
+  // (share of the line, block of heads): a share's blocks, which read the same
+  // keys, side by side on one XCD
+  const int block = (int)blockIdx.x / kXcds % blocks;
+  const uint32_t me = (int)blockIdx.x / (kXcds * blocks) * kXcds + (int)blockIdx.x % kXcds;
 
   // The line of steps, by each wave for itself (no barrier): a lane sums a run
   // of sequences, the runs are scanned, and the lane whose run has the
@@ -210,7 +218,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(const PagedAttn
   const uint32_t total = (uint32_t)__builtin_amdgcn_readlane((int)before, 63) * units;
   before = (before - mine) * units;
   mine *= units;
-  const uint32_t shares = min((uint32_t)gridDim.x, total), me = blockIdx.x;
+  const uint32_t shares = min((uint32_t)groups, total);
   if (me >= shares) return;
   uint32_t at = share_begin(total, me, shares);
   const uint32_t stop = share_begin(total, me + 1, shares);
@@ -241,7 +249,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(const PagedAttn
     }
     const uint32_t unit = (at - seq_start) / steps, row_start = seq_start + unit * steps;
     const uint32_t i0 = at - row_start, n = min(stop - at, steps - i0);
-    const int kvh = unit / blocks, h0 = (unit - kvh * blocks) * kHeads;  // KV head, first head of the group
+    const int kvh = (int)unit, h0 = block * kHeads;  // KV head, first head of the group
     const int live = min(kHeads, group - h0);
 
     // the query: each wave takes a share of the fragments, lane c16 % 8's head
@@ -528,9 +536,9 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(const PagedAttn
     }
     __syncthreads();
     const bool whole = i0 == 0 && n == steps;
-    Part<D> *part = parts + 2 * (int64_t)me + (i0 == 0 ? 1 : 0);
+    Part<D> *part = parts + 2 * ((int64_t)me * blocks + block) + (i0 == 0 ? 1 : 0);
     if (i0 == 0 && tid == 0) {
-      rows[(int64_t)seq * units + unit] = RowParts{(int)me, (int)share_of(total, row_start + steps - 1, shares)};
+      rows[((int64_t)seq * units + unit) * blocks + block] = RowParts{(int)me, (int)share_of(total, row_start + steps - 1, shares)};
     }
     for (int i = tid; i < kHeads * (D / 4); i += kThreads) {
       const int h = i / (D / 4), d = i - h * (D / 4);
@@ -599,7 +607,7 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(const PagedAttnAr
 #pragma unroll
     for (int i = 0; i < kDeep; i++) {
       const int c = min(c0 + i * kAtOnce, r.last);
-      const Part<D> &p = parts[2 * (int64_t)c + (c == r.first ? 1 : 0)];
+      const Part<D> &p = parts[2 * ((int64_t)c * blocks + in_group / kHeads) + (c == r.first ? 1 : 0)];
       mc[i] = p.m[h];
       lc[i] = p.l[h];
       v[i] = *reinterpret_cast<const float4 *>(&p.o[h][4 * d]);
@@ -655,11 +663,11 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(const PagedAttnAr
 
 template <int D, int CT, bool THIRD, bool STREAM>
 hipError_t launch_kernels(const PagedAttnArgs &a, int groups, hipStream_t s) {
-  const int64_t rows = (int64_t)a.c.sequences * a.c.nkv * blocks_of(a.nq, a.c.nkv);
   Part<D> *parts = reinterpret_cast<Part<D> *>(a.partials);
-  RowParts *row_parts = reinterpret_cast<RowParts *>(parts + 2 * (int64_t)groups);
-  (void)rows;
-  hipLaunchKernelGGL((paged_attn_kernel<D, CT, THIRD, STREAM>), dim3(groups), dim3(kThreads), 0, s, a, row_parts, parts);
+  const int blocks = blocks_of(a.nq, a.c.nkv), grid = (groups + kXcds - 1) / kXcds * kXcds * blocks;
+  RowParts *row_parts = reinterpret_cast<RowParts *>(parts + 2 * (int64_t)groups * blocks);
+  hipLaunchKernelGGL((paged_attn_kernel<D, CT, THIRD, STREAM>), dim3(grid), dim3(kThreads), 0, s, a, row_parts, parts,
+                     groups);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL(paged_merge_kernel<D>, dim3(a.nq, a.c.sequences), dim3(kThreads), 0, s, a, row_parts, parts, groups);
@@ -696,17 +704,19 @@ uint64_t paged_attn_most_steps(const PagedAttnArgs &a) {
   uint64_t keys = (uint64_t)a.c.width << a.c.page_shift;
   if (a.window > 0 && keys > (uint64_t)a.window + 15) keys = (uint64_t)a.window + 15;
   const int step = step_of(a.c.head_dim, a.c.type);
-  return (keys + step - 1) / step * a.c.sequences * a.c.nkv * blocks_of(a.nq, a.c.nkv);
+  return (keys + step - 1) / step * a.c.sequences * a.c.nkv;
 }
 
 int paged_attn_groups(const PagedAttnArgs &a, int num_cus) {
   const uint64_t most = paged_attn_most_steps(a);
-  return (int)(most < 2ull * num_cus ? most : 2ull * num_cus);
+  const int room = 2 * num_cus / blocks_of(a.nq, a.c.nkv);  // two workgroups a CU
+  return most < (uint64_t)room ? (int)most : room < 1 ? 1 : room;
 }
 
 size_t paged_attn_scratch_bytes(const PagedAttnArgs &a, int groups) {
-  return 2 * (size_t)groups * part_bytes(a.c.head_dim) +
-         (size_t)a.c.sequences * a.c.nkv * blocks_of(a.nq, a.c.nkv) * sizeof(RowParts);
+  const size_t blocks = blocks_of(a.nq, a.c.nkv);
+  return blocks * (2 * (size_t)groups * part_bytes(a.c.head_dim) +
+                   (size_t)a.c.sequences * a.c.nkv * sizeof(RowParts));
 }
 
 hipError_t launch_paged_attn(const PagedAttnArgs &a, int groups, hipStream_t s) {
