@@ -16,7 +16,9 @@
 // of 128 two workgroups share a CU; the scores of the next tile are formed
 // ahead of this one's weights, so that a wave's products run under its
 // exponentials as well (heads of 256, one wave a SIMD: 192 -> 166 us on six
-// prompts of 9000 rows).
+// prompts of 9000 rows).  Tiles for heads of 256 are 32 keys, whose one
+// accumulator would chain sixteen products: even and odd ones go to one each
+// (the same prompts 164 -> 152 us; tiles of 64 keys instead 179).
 // Per 32 keys a wave forms, on v_mfma_f32_32x32x16,
 //   S^T = K Q^T: the keys are the A rows, read as they lie; the query is the
 //     B operand, in registers throughout.  Lane (n, h) then has query row n's
@@ -278,6 +280,9 @@ __global__ __launch_bounds__(kThreads, D * G >= 256 ? 1 : 2) void packed_attn_ke
   // The steps of a tile.  scores: S^T of the keys in LDS.
   auto scores = [&](f32x16 (&s)[kSubs], int buffer) {
     const uint8_t *kt = lds[buffer][0];
+    f32x16 odd;  // a second chain of products where there is one subtile
+#pragma unroll
+    for (int i = 0; i < 16; i++) odd[i] = 0.0f;
 #pragma unroll
     for (int u = 0; u < kSubs; u++) {
 #pragma unroll
@@ -287,9 +292,13 @@ __global__ __launch_bounds__(kThreads, D * G >= 256 ? 1 : 2) void packed_attn_ke
       for (int i = 0; i < D / 16; i++) {
         const u32x4 kf =
             *reinterpret_cast<const u32x4 *>(kt + kr * kRowBytes + 16 * ((2 * i + h) ^ key_swizzle<D>(kr)));
-        s[u] = mfma32<BF>(kf, q[i], s[u]);
+        if (kSubs == 1 && (i & 1))
+          odd = mfma32<BF>(kf, q[i], odd);
+        else
+          s[u] = mfma32<BF>(kf, q[i], s[u]);
       }
     }
+    if (kSubs == 1) s[0] += odd;
   };
   // Whether a row of the wave has a masked key in the tile at `key` (the same for
   // the wave).
@@ -544,13 +553,13 @@ __global__ __launch_bounds__(kThreads, D * G >= 256 ? 1 : 2) void packed_attn_ke
 // half of them each.  Measured with one group and two, one prompt: heads of 64,
 // 280 blocks 34.6 and 23.5 us, 658 92 and 96; heads of 128 (a CU then has one
 // workgroup), 160 blocks 46.1 and 35.3, 224 blocks 20.8 and 23.6; heads of 256,
-// 256 blocks 152 and 115, 710 166 and 199.  Up to one tile of rows there is
-// nothing to split (40 rows: heads of 128 6.3 and 7.5, of 256 8.8 and 9.8, but
-// of 64 5.7 and 5.3).
+// 256 blocks 132 and 102, 304 158 and 152, 358 186 and 195.  Up to one tile of
+// rows there is nothing to split (40 rows: heads of 128 6.3 and 7.5, of 256 8.2
+// and 9.2, but of 64 5.7 and 5.3).
 int groups_of(const PackedAttnArgs &a, int num_cus) {
   const int64_t blocks = ((int64_t)a.tokens / (kWaveRows * kWaves) + 1) * a.nq;
   if (a.head_dim > 64 && a.tokens <= 64) return 1;
-  return 4 * blocks < (a.head_dim == 128 ? 3 : 8) * (int64_t)num_cus ? 2 : 1;
+  return 4 * blocks < (a.head_dim == 128 ? 3 : a.head_dim == 256 ? 5 : 8) * (int64_t)num_cus ? 2 : 1;
 }
 
 int64_t slots_of(const PackedAttnArgs &a, int groups) {
