@@ -2866,6 +2866,11 @@ int32_t serving_call(void *stream, Check check, Run run) {
 bool aligned16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 bool activation_type(int32_t t) { return t == HP_ELEM_F32 || t == HP_ELEM_F16 || t == HP_ELEM_BF16; }
 bool positive(double v) { return std::isfinite(v) && v > 0.0; }
+// Scales that the kernels may take the reciprocal of, or multiply with others
+// of their kind and log2(e): nothing of it leaves f32's range, so that a score
+// of 0 stays 0.
+bool cache_scale(float v) { return v >= 0x1p-100f && v <= 0x1p100f; }
+bool score_scale(float v) { return v > 0.0f && v <= 0x1p120f; }
 
 // A stride of `rows` rows in elements of `bytes` each: 0 stands for `dense`;
 // rows do not overlap, start at 16-byte boundaries and end within an address
@@ -2903,8 +2908,8 @@ int32_t paged_cache_check(const hp_hip_paged_cache_t *c, PagedCache *out) {
   if (c->sequence_count < 0 || c->sequence_count > 65535) return fail(HP_ERR_SHAPE, "sequence_count must be 0..65535");
   if (c->pages_per_sequence < 1 || (int64_t)c->pages_per_sequence * c->page_size > (1 << 30))
     return fail(HP_ERR_SHAPE, "pages_per_sequence * page_size must be 1..2^30");
-  if (c->type == HP_ELEM_E4M3 && (!positive(c->key_scale) || !positive(c->value_scale)))
-    return fail(HP_ERR_ARG, "the scales of an e4m3 cache must be finite and positive");
+  if (c->type == HP_ELEM_E4M3 && (!cache_scale(c->key_scale) || !cache_scale(c->value_scale)))
+    return fail(HP_ERR_ARG, "the scales of an e4m3 cache must be 2^-100 .. 2^100");
   int64_t stride = 0;
   rc = row_stride(c->page_stride, (size_t)c->head_count_kv * c->page_size * c->head_dim, elem_bytes(c->type),
                   (size_t)c->page_count, &stride);
@@ -2979,7 +2984,8 @@ int32_t paged_attention_check(const hp_hip_paged_cache_t *cache, const hp_hip_pa
   if (rc != HP_OK) return rc;
   if (!activation_type(p->q_type) || !activation_type(p->out_type))
     return fail(HP_ERR_TYPE, "queries and outputs are f32, f16 or bf16");
-  if (!positive(p->scale)) return fail(HP_ERR_ARG, "scale must be finite and positive");
+  if (!score_scale(p->scale) || p->scale * a->c.key_scale > 0x1p120f)
+    return fail(HP_ERR_ARG, "scale (times the key scale) must be positive, up to 2^120");
   if (p->sliding_window < 0) return fail(HP_ERR_ARG, "sliding_window must not be negative");
   const size_t row = (size_t)p->head_count * a->c.head_dim;
   if ((rc = row_stride(p->q_stride, row, elem_bytes(p->q_type), a->c.sequences, &a->q_stride)) != HP_OK) return rc;
@@ -3006,7 +3012,7 @@ int32_t packed_attention_check(const hp_hip_packed_attention_t *p, PackedAttnArg
   int32_t rc = head_dim_check(p->head_dim);
   if (rc == HP_OK) rc = heads_check(p->head_count, p->head_count_kv);
   if (rc != HP_OK) return rc;
-  if (!positive(p->scale)) return fail(HP_ERR_ARG, "scale must be finite and positive");
+  if (!score_scale(p->scale)) return fail(HP_ERR_ARG, "scale must be positive, up to 2^120");
   if (p->sliding_window < 0) return fail(HP_ERR_ARG, "sliding_window must not be negative");
   if (p->sequence_count < 0 || p->sequence_count > (1 << 20)) return fail(HP_ERR_SHAPE, "sequence_count must be 0..2^20");
   if (p->token_count > (1u << 30)) return fail(HP_ERR_SHAPE, "too many tokens");

@@ -548,7 +548,7 @@ typedef struct hp_hip_paged_cache {
   int32_t page_count;
   int32_t sequence_count;     /* up to 65535; 0: calls do nothing */
   int32_t pages_per_sequence; /* pages_per_sequence * page_size <= 2^30 */
-  float key_scale, value_scale; /* HP_ELEM_E4M3: finite, > 0; otherwise not used */
+  float key_scale, value_scale; /* HP_ELEM_E4M3: 2^-100 .. 2^100; otherwise not used */
   size_t page_stride;         /* elements; 0: head_count_kv * page_size * head_dim */
   const int32_t *d_pages, *d_lengths;
 } hp_hip_paged_cache_t;
@@ -602,7 +602,7 @@ typedef struct hp_hip_paged_attention {
   int32_t head_count;
   int32_t q_type, out_type;       /* HP_ELEM_F32, HP_ELEM_F16 or HP_ELEM_BF16 */
   int32_t sliding_window;         /* 0: none */
-  float scale;                    /* finite, > 0 */
+  float scale;                    /* > 0; times the key scale up to 2^120 */
   int32_t reserved;               /* 0 */
 } hp_hip_paged_attention_t;
 int32_t hp_hip_paged_attention_device(const hp_hip_paged_cache_t *cache, const hp_hip_paged_attention_t *attention,
@@ -613,8 +613,9 @@ int32_t hp_hip_paged_attention_device(const hp_hip_paged_cache_t *cache, const h
  * d_offsets[s] .. d_offsets[s + 1] - 1 (rising, [sequence_count + 1]) are
  * sequence s; rows behind the last are left as they were.  Queries, keys and
  * values are of one type, which the probabilities are rounded to as well;
- * scores, softmax statistics and sums are f32.  Token strides of their own let
- * them lie in one projection's rows. */
+ * scores, softmax statistics and sums are f32.  What masked places hold does
+ * not matter.  Token strides of their own let them lie in one projection's
+ * rows. */
 typedef struct hp_hip_packed_attention {
   const void *d_q, *d_k, *d_v; /* [token][heads][head_dim] of type */
   void *d_output;              /* [token][head_count][head_dim] of out_type */
@@ -627,7 +628,7 @@ typedef struct hp_hip_packed_attention {
   int32_t type;                /* HP_ELEM_F16 or HP_ELEM_BF16 */
   int32_t out_type;            /* HP_ELEM_F32, HP_ELEM_F16 or HP_ELEM_BF16 */
   int32_t sliding_window;
-  float scale;                 /* finite, > 0 */
+  float scale;                 /* > 0, up to 2^120 */
 } hp_hip_packed_attention_t;
 int32_t hp_hip_packed_attention_device(const hp_hip_packed_attention_t *attention, void *stream);
 

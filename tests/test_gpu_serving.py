@@ -667,3 +667,18 @@ def test_rules_odd_values(hip, S):
         arg["repetition"][2], arg["frequency"][2], arg["presence"][2] = 1.0, 0.0, 0.0
 
     run_rules(S, 3, 500, history=3000, mask=0.7, edit=edit)
+
+
+@pytest.mark.parametrize("scale", [2.0 ** 120, 2.0 ** -149])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_largest_and_smallest_scales(hip, S, D, scale):
+    """Queries of zeros: every key weighs the same at the largest scale; at the smallest they do whatever the query."""
+    rng = np.random.default_rng(7)
+    times = 0.0 if scale > 1 else 1.0
+    for type, scales in (("f16", (1.0, 1.0)), ("e4m3", (2.0 ** -20, 0.5))):
+        run_paged(S, Pool(rng, [1, 40, 0, 333], 2, D, 16, type, scales=scales), 4, rng=rng, q_times=times, window=100,
+                  scale=scale)
+
+    def zeros(q, k, v):
+        q *= times
+    run_packed(S, [1, 100, 65], 2, 1, D, "bf16", scale=scale, spoil=zeros, seed=D, window=40)

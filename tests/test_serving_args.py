@@ -155,3 +155,17 @@ def test_wrappers_raise():
         H.logit_rules_device(1, 10, 0, P)
     with pytest.raises(ValueError, match="paged_append hip shape mismatch"):
         H.paged_append_device(cache(), 7, 4, P, P, P, P, 1)
+
+
+@pytest.mark.parametrize("scale", [3e38, 2.0 ** 121, INF])
+def test_scales_whose_factors_are_no_numbers(scale):
+    """scale * log2(e) and 1 / key_scale would be infinite, and a score or an element of 0 a NaN."""
+    assert H.lib().hp_hip_paged_attention_device(cache(), attention(scale=scale), None) == ARG
+    assert H.lib().hp_hip_packed_attention_device(packed(scale=scale), None) == ARG
+    for name in ("key_scale", "value_scale"):
+        for value in (scale, 1 / scale, 1e-39):
+            c = cache(type=H.HP_ELEM_E4M3, **{name: value})
+            assert H.lib().hp_hip_paged_append_device(c, append(), None) == ARG
+            assert H.lib().hp_hip_paged_attention_device(c, attention(), None) == ARG
+    c = cache(type=H.HP_ELEM_E4M3, key_scale=2.0 ** 100)
+    assert H.lib().hp_hip_paged_attention_device(c, attention(scale=2.0 ** 21), None) == ARG
