@@ -7,12 +7,19 @@
 // close behind: every pair costs one exponential, a quarter-rate instruction.
 // 16384 rows of 16 heads of 128, bf16: 1.1 TFLOP in 1004 us, 1096 TFLOP/s, at
 // which the card has lowered its clock to 1.6 GHz (a large library matrix
-// product reaches 1212); 15 prompts of 12345 rows, 32 heads: 111 GFLOP in 171 us,
-// 650 TFLOP/s, a quarter of their tiles being the diagonal's.
+// product reaches 1212); 15 prompts of 12345 rows, 32 heads: 111 GFLOP in 150 us,
+// 740 TFLOP/s, a quarter of their tiles being the diagonal's.
 //
-// A workgroup is 128 query rows of one head, 32 for each of its four waves,
-// and walks the keys in tiles of kKeys through LDS, double buffered: the next
-// tiles go from memory straight into LDS while one is worked on.  Up to heads
+// A workgroup is 32 query rows for each of its four waves -- 32 rows of four
+// heads that share their keys, 64 of two or 128 of one, by what the heads of a
+// group divide into -- and walks the keys in tiles of kKeys through LDS, double
+// buffered: the next tiles go from memory straight into LDS while one is worked
+// on.  The more heads, the fewer tiles of the diagonal, of a window's edge and
+// behind a prompt's end its waves wait through (15 prompts, four heads against
+// one: 171 -> 154 us; windows of 500 on 8000 rows 58 -> 55).  Query rows come in
+// and 16-bit and f32 rows leave through LDS, whole rows a load or store and not
+// 16 bytes of each (the same prompts to 150; 8 prompts of 2000 rows 22.3 -> 19.6,
+// 40 rows of heads of 128 6.0 -> 6.3).  Up to heads
 // of 128 two workgroups share a CU; the scores of the next tile are formed
 // ahead of this one's weights, so that a wave's products run under its
 // exponentials as well (heads of 256, one wave a SIMD: 192 -> 166 us on six
@@ -143,6 +150,20 @@ __device__ __forceinline__ void load_to_lds(const uint8_t *base, uint32_t offset
       : "memory");
 }
 
+// The same from a lane's own address.
+__device__ __forceinline__ void load_to_lds(const uint8_t *at, uint32_t lds) {
+  uint32_t m0;
+  asm volatile(
+      "s_mov_b32 %0, m0\n\t"
+      "s_mov_b32 m0, %2\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %1, off\n\t"
+      "s_mov_b32 m0, %0"
+      : "=&s"(m0)
+      : "v"(at), "s"(lds)
+      : "memory");
+}
+
 // Chunk (16 bytes) where a tile's row keeps chunk c, for keys and values.  Keys
 // are read 16 rows at a time at one chunk, values 4 rows at 4 chunks.
 template <int D>
@@ -157,61 +178,67 @@ __device__ __forceinline__ int value_swizzle(int row) {
 // Heads of D, the keys of a block split over G groups of waves.
 template <int D, int G>
 struct Shape {
-  static constexpr int kGroupWaves = kWaves / G, kRows = kWaveRows * kGroupWaves;  // query rows of a workgroup
-  static constexpr int kKeys = D == 256 ? 32 : 64;         // of a tile
+  static constexpr int kGroupWaves = kWaves / G, kRows = kWaveRows * kGroupWaves;  // (query row, head) pairs of a workgroup
+  static constexpr int kKeys = D == 256 ? 32 : 64;                                 // of a tile
   static constexpr int kRowBytes = 2 * D, kChunks = D / 8;
   static constexpr int kTileBytes = kKeys * kRowBytes;            // of K or V
   static constexpr int kLoads = kTileBytes / 1024 / kGroupWaves;  // 16-byte loads a lane, of K or V
   static constexpr int kLoadRows = 1024 / kRowBytes;              // rows of one load of a wave
+  static constexpr int kQueryBytes = kRows * kRowBytes;           // of a group's query rows
+  // (they come through the place of the second V and, where they are more, on)
+  static constexpr int kSpare = kQueryBytes > kTileBytes ? kQueryBytes - kTileBytes : 0;
 };
 
 template <int D, bool BF, int G>
-__global__ __launch_bounds__(kThreads, D * G >= 256 ? 1 : 2) void packed_attn_kernel(const PackedAttnArgs a, int slots) {
+__global__ __launch_bounds__(kThreads, D * G >= 256 ? 1 : 2) void packed_attn_kernel(const PackedAttnArgs a, int slots,
+                                                                                int heads_log2) {
   using S = Shape<D, G>;
-  constexpr int kKeys = S::kKeys, kSubs = kKeys / 32, kRowBytes = S::kRowBytes, kRows = S::kRows;
-  __shared__ __align__(1024) uint8_t lds_all[G][2][2][S::kTileBytes];  // [group][buffer][K, V]
+  constexpr int kKeys = S::kKeys, kSubs = kKeys / 32, kRowBytes = S::kRowBytes;
+  const int head_rows = 1 << (__builtin_ctz(S::kRows) - heads_log2);  // query rows of each of the workgroup's heads
+  __shared__ __align__(1024) uint8_t lds_all[G][4 * S::kTileBytes + S::kSpare];  // [group]: buffer 0's K, V, 1's K, V
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n32 = lane & 31, h = lane >> 5;
   const int part = wave / S::kGroupWaves, member = wave % S::kGroupWaves;  // group of waves, place in it
-  auto &lds = lds_all[part];
+  auto tile_of = [&](int buffer, int value) { return &lds_all[part][(2 * buffer + value) * S::kTileBytes]; };
 
   // Work: (slot, KV head) units from the last slot down -- a sequence's last
   // rows have the most keys -- dealt round the XCDs, the heads of a unit one
   // after another on one XCD, whose L2 then has the keys that they share.
-  const int group = a.nq / a.nkv;
+  const int group = a.nq / a.nkv, bundles = group >> heads_log2;
   const int r = blockIdx.x / kXcds;
-  const int unit = r / group * kXcds + blockIdx.x % kXcds;
+  const int unit = r / bundles * kXcds + blockIdx.x % kXcds;
   if (unit >= slots * a.nkv) return;
-  const int slot = slots - 1 - unit / a.nkv, kvh = unit % a.nkv, head = kvh * group + r % group;
+  const int slot = slots - 1 - unit / a.nkv, kvh = unit % a.nkv;
+  const int head = kvh * group + (r % bundles << heads_log2) + member % (1 << heads_log2);  // the wave's
 
   int seq, begin, end;
   {
     int lo = 0, n = a.sequences;  // the largest whose first block is not behind `slot`
     while (n > 64) {
       const int step = (n + 63) >> 6, at = lo + min(lane * step, n - 1);
-      const bool le = lane * step < n && packed_first_block(a.offsets[at], at, kRows) <= slot;
+      const bool le = lane * step < n && packed_first_block(a.offsets[at], at, head_rows) <= slot;
       const int c = max(__popcll(__ballot(le)), 1) - 1;
       lo += c * step;
       n = min(step, n - c * step);
     }
     const int at = lo + min(lane, n - 1), o0 = a.offsets[at], o1 = a.offsets[at + 1];
-    const bool le = lane < n && packed_first_block(o0, at, kRows) <= slot;
+    const bool le = lane < n && packed_first_block(o0, at, head_rows) <= slot;
     const int c = max(__popcll(__ballot(le)), 1) - 1;
     seq = lo + c;
     begin = __builtin_amdgcn_readlane(o0, c);
     end = min(__builtin_amdgcn_readlane(o1, c), a.tokens);
   }
   if (begin < 0 || begin >= end) return;
-  const int64_t row_at = (slot - packed_first_block(begin, seq, kRows)) * kRows;
+  const int64_t row_at = (slot - packed_first_block(begin, seq, head_rows)) * head_rows;
   const int len = end - begin;
   if (row_at < 0 || row_at >= len) return;
   const int row0 = (int)row_at;                         // the workgroup's first row
-  const int wave0 = row0 + kWaveRows * member;           // the wave's
+  const int wave0 = row0 + kWaveRows * (member >> heads_log2);           // the wave's
   const int row = wave0 + n32;                          // the lane's
   const int window = a.window > 0 ? a.window : 0x7fffffff;
   const int first = max(row - min(row, window - 1), 0);  // first key of the lane's row
   const int tile_first = max(row0 - min(row0, window - 1), 0) / kKeys * kKeys;
-  const int tile_stop = min(len, row0 + kRows);
+  const int tile_stop = min(len, row0 + head_rows);
 
   const uint8_t *kp = static_cast<const uint8_t *>(a.k) + ((int64_t)begin * a.k_stride + kvh * D) * 2;
   const uint8_t *vp = static_cast<const uint8_t *>(a.v) + ((int64_t)begin * a.v_stride + kvh * D) * 2;
@@ -222,7 +249,7 @@ __global__ __launch_bounds__(kThreads, D * G >= 256 ? 1 : 2) void packed_attn_ke
   constexpr int kTurn = S::kLoadRows * S::kGroupWaves;
   const int load_row = S::kLoadRows * member + lane / S::kChunks, load_chunk = lane % S::kChunks;
   const uint32_t k_row = (uint32_t)a.k_stride * 2, v_row = (uint32_t)a.v_stride * 2;
-  const uint32_t lds_at = (uint32_t)(uintptr_t)(lds_ptr)&lds[0][0][0] + 1024 * member;
+  const uint32_t lds_at = (uint32_t)(uintptr_t)(lds_ptr)tile_of(0, 0) + 1024 * member;
   // (the rows of one load of the group repeat the swizzles' after kKinds)
   constexpr int kKinds = kTurn >= 16 ? 1 : 16 / kTurn;
   static_assert(kTurn * kKinds % 16 == 0, "the swizzles' period");
@@ -253,12 +280,15 @@ __global__ __launch_bounds__(kThreads, D * G >= 256 ? 1 : 2) void packed_attn_ke
     load_rows(vp, v_row, v_at, key, lds_at + (buffer * 2 + 1) * S::kTileBytes);
   };
 
-  u32x4 q[D / 16];
-  {
-    const int64_t at = (int64_t)(begin + min(row, len - 1)) * a.q_stride + head * D + 8 * h;
+  // The wave's query rows (behind the sequence: its last) come through LDS, where
+  // the second values will be and on, so that a load is whole rows.
+  const uint8_t *own_q = tile_of(1, 1) + member * (kWaveRows * kRowBytes);
 #pragma unroll
-    for (int i = 0; i < D / 16; i++)
-      q[i] = *reinterpret_cast<const u32x4 *>(static_cast<const uint8_t *>(a.q) + (at + 16 * i) * 2);
+  for (int i = 0; i < kWaveRows; i += S::kLoadRows) {
+    const int rr = i + lane / S::kChunks;
+    const int64_t at = (int64_t)(begin + min(wave0 + rr, len - 1)) * a.q_stride + head * D;
+    load_to_lds(static_cast<const uint8_t *>(a.q) + at * 2 + 16 * (load_chunk ^ key_swizzle<D>(rr)),
+                (uint32_t)(uintptr_t)(lds_ptr)own_q + i * kRowBytes);
   }
   // Group `part` has the tiles part, part + G, ... : its tile i is key_of(i).
   const int tiles = (tile_stop - tile_first + kKeys - 1) / kKeys;
@@ -277,9 +307,10 @@ __global__ __launch_bounds__(kThreads, D * G >= 256 ? 1 : 2) void packed_attn_ke
     for (int i = 0; i < 16; i++) acc[t][i] = 0.0f;
   float m = -kInf, l = 0.0f;
 
+  u32x4 q[D / 16];
   // The steps of a tile.  scores: S^T of the keys in LDS.
   auto scores = [&](f32x16 (&s)[kSubs], int buffer) {
-    const uint8_t *kt = lds[buffer][0];
+    const uint8_t *kt = tile_of(buffer, 0);
     f32x16 odd;  // a second chain of products where there is one subtile
 #pragma unroll
     for (int i = 0; i < 16; i++) odd[i] = 0.0f;
@@ -362,7 +393,7 @@ __global__ __launch_bounds__(kThreads, D * G >= 256 ? 1 : 2) void packed_attn_ke
   // gather: O^T += V^T P^T with the values in LDS (check: keys may be masked).
   auto gather = [&](const u32x4 (&p)[2 * kSubs], int buffer, bool check, auto edge) {
     constexpr bool kMasked = decltype(edge)::value;
-    const uint8_t *vt = lds[buffer][1];
+    const uint8_t *vt = tile_of(buffer, 1);
     // V^T fragments: product jj's k index 8 h + i is key 16 jj + 4 h + i (i < 4)
     // and 16 jj + 8 + 4 h + i - 4; a lane of 16 reads 8 bytes of key row
     // (lane % 16) / 4, elements 4 (lane % 4) .. of its 16
@@ -447,11 +478,14 @@ __global__ __launch_bounds__(kThreads, D * G >= 256 ? 1 : 2) void packed_attn_ke
   };
   // Turns whose tiles every row of the workgroup sees whole.
   const int whole_first =
-      (max(row0 + kRows - min(row0 + kRows, window) - tile_first + kKeys - 1, 0) / kKeys + G - 1) / G;
+      (max(row0 + head_rows - min(row0 + head_rows, window) - tile_first + kKeys - 1, 0) / kKeys + G - 1) / G;
   const int whole_stop = (row0 + 1 - tile_first) / kKeys / G;
   f32x16 sa[kSubs], sb[kSubs];
   __builtin_amdgcn_s_waitcnt(kWaitLoads);
   __syncthreads();
+#pragma unroll
+  for (int i = 0; i < D / 16; i++)
+    q[i] = *reinterpret_cast<const u32x4 *>(own_q + n32 * kRowBytes + 16 * ((2 * i + h) ^ key_swizzle<D>(n32)));
   if (sees(0)) {
     scores(sa, 0);
     settle(sa, key_of(0), std::true_type{});
@@ -526,17 +560,55 @@ __global__ __launch_bounds__(kThreads, D * G >= 256 ? 1 : 2) void packed_attn_ke
     }
   }
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  if (row >= len) return;
-  const int64_t o = (int64_t)(begin + row) * a.out_stride + head * D;
+  // With one group the wave's rows leave through LDS, so that a store is whole
+  // rows and not 16 bytes of each: kSpan elements of them at a time, a row of 16
+  // bits or half a row of f32, in chunks that are XORed as the keys' are.  With
+  // two the launch is a few blocks whose end counts, and this costs more than it
+  // gives (77 rows of 8 / 2 heads of 256: 10.2 and 10.9 us).
+  if (G == 1) __syncthreads();  // no wave reads the tiles any more
+  uint8_t *own = reinterpret_cast<uint8_t *>(lds_all) + wave * (kWaveRows * kRowBytes);
+  static_assert(G > 1 || kWaves * kWaveRows * kRowBytes <= (int)sizeof(lds_all), "the rows fit the tiles' place");
+  // (the lane anew: addresses that the loads share would take registers through the walk)
+  int lane_now = lane;
+  asm volatile("" : "+v"(lane_now));
+  const int row_now = lane_now & 31, h_now = lane_now >> 5;
   auto store = [&](auto type) {
+    constexpr int kType = decltype(type)::value, kE = kType == kElemF32 ? 4 : 2, kSpan = kRowBytes / kE;
+    constexpr int kChunkMask = S::kChunks < 16 ? S::kChunks - 1 : 15;
+    if (G > 1) {
+      if (row >= len) return;
 #pragma unroll
-    for (int t = 0; t < D / 32; t++)
+      for (int t = 0; t < D / 32; t++)
 #pragma unroll
-      for (int b = 0; b < 4; b++) {
-        const float v[4] = {acc[t][4 * b] * inv, acc[t][4 * b + 1] * inv, acc[t][4 * b + 2] * inv,
-                            acc[t][4 * b + 3] * inv};
-        store4(a.out, o + 32 * t + 8 * b + 4 * h, decltype(type)::value, v);
+        for (int b = 0; b < 4; b++) {
+          const float v[4] = {acc[t][4 * b] * inv, acc[t][4 * b + 1] * inv, acc[t][4 * b + 2] * inv,
+                              acc[t][4 * b + 3] * inv};
+          store4(a.out, (int64_t)(begin + row) * a.out_stride + head * D + 32 * t + 8 * b + 4 * h, kType, v);
+        }
+      return;
+    }
+#pragma unroll
+    for (int from = 0; from < D; from += kSpan) {
+#pragma unroll
+      for (int t = from / 32; t < (from + kSpan) / 32; t++)
+#pragma unroll
+        for (int b = 0; b < 4; b++) {
+          const float v[4] = {acc[t][4 * b] * inv, acc[t][4 * b + 1] * inv, acc[t][4 * b + 2] * inv,
+                              acc[t][4 * b + 3] * inv};
+          const int at = (32 * t + 8 * b + 4 * h_now - from) * kE;  // bytes of the row
+          store4(own + row_now * kRowBytes + 16 * ((at >> 4) ^ (row_now & kChunkMask)) + (at & 15), 0, kType, v);
+        }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // one lane's writes are another's reads
+#pragma unroll
+      for (int i = 0; i < kWaveRows; i += S::kLoadRows) {
+        const int r = i + lane_now / S::kChunks, c = lane_now % S::kChunks;
+        const u32x4 w = *reinterpret_cast<const u32x4 *>(own + r * kRowBytes + 16 * (c ^ (r & kChunkMask)));
+        if (wave0 + r < len)
+          *reinterpret_cast<u32x4 *>(static_cast<uint8_t *>(a.out) +
+                                     ((int64_t)(begin + wave0 + r) * a.out_stride + head * D + from) * kE + 16 * c) = w;
       }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
   };
   if (a.out_type == kElemF32)
     store(std::integral_constant<int, kElemF32>{});
@@ -562,11 +634,17 @@ int groups_of(const PackedAttnArgs &a, int num_cus) {
   return 4 * blocks < (a.head_dim == 128 ? 3 : a.head_dim == 256 ? 5 : 8) * (int64_t)num_cus ? 2 : 1;
 }
 
+// log2 of the heads that a workgroup has: as many as divide a KV head's and its
+// waves (of a group of waves).
+int heads_log2_of(const PackedAttnArgs &a, int groups) {
+  const int group = a.nq / a.nkv;
+  return group % 4 == 0 && groups == 1 ? 2 : group % 2 == 0 ? 1 : 0;
+}
 int64_t slots_of(const PackedAttnArgs &a, int groups) {
-  return packed_blocks(a.tokens, a.sequences, kWaveRows * kWaves / groups);
+  return packed_blocks(a.tokens, a.sequences, (kWaveRows * kWaves / groups) >> heads_log2_of(a, groups));
 }
 int64_t grid_of(const PackedAttnArgs &a, int groups) {
-  return (slots_of(a, groups) * a.nkv + kXcds - 1) / kXcds * kXcds * (a.nq / a.nkv);
+  return (slots_of(a, groups) * a.nkv + kXcds - 1) / kXcds * kXcds * ((a.nq / a.nkv) >> heads_log2_of(a, groups));
 }
 
 template <int D, int G>
@@ -574,9 +652,9 @@ hipError_t launch(const PackedAttnArgs &a, hipStream_t s) {
   const unsigned grid = (unsigned)grid_of(a, G);
   const int slots = (int)slots_of(a, G);
   if (a.type == kElemBf16)
-    hipLaunchKernelGGL((packed_attn_kernel<D, true, G>), dim3(grid), dim3(kThreads), 0, s, a, slots);
+    hipLaunchKernelGGL((packed_attn_kernel<D, true, G>), dim3(grid), dim3(kThreads), 0, s, a, slots, heads_log2_of(a, G));
   else
-    hipLaunchKernelGGL((packed_attn_kernel<D, false, G>), dim3(grid), dim3(kThreads), 0, s, a, slots);
+    hipLaunchKernelGGL((packed_attn_kernel<D, false, G>), dim3(grid), dim3(kThreads), 0, s, a, slots, heads_log2_of(a, G));
   return hipGetLastError();
 }
 

@@ -682,3 +682,13 @@ def test_largest_and_smallest_scales(hip, S, D, scale):
     def zeros(q, k, v):
         q *= times
     run_packed(S, [1, 100, 65], 2, 1, D, "bf16", scale=scale, spoil=zeros, seed=D, window=40)
+
+
+@pytest.mark.parametrize("Hq,kv,D", [(4, 1, 64), (12, 1, 128), (8, 2, 256), (6, 1, 64), (2, 2, 256)])
+@pytest.mark.parametrize("out", ["f32", "f16"])
+def test_packed_heads_that_share_a_workgroup(hip, S, Hq, kv, D, out):
+    """Four, two and one heads a workgroup over its whole range of rows, in batches that fill the card (one walk over
+    the keys) and in small ones (two), with rows that end inside a block and a window that begins inside a tile."""
+    heads = -(-1400 // (Hq * 25)) * Hq  # blocks of 128 rows over 3200 rows past every limit of the split
+    run_packed(S, [1, 31, 32, 33, 2000, 0, 97, 1006], heads, heads // Hq * kv, D, "f16", out, window=75, seed=Hq, sample=60)
+    run_packed(S, [1, 31, 32, 33, 97], Hq, kv, D, "f16", out, window=40, seed=Hq, joined=True)
