@@ -5,23 +5,23 @@
 //
 // The matrix cores bound it (4 D flop a pair and head), with the vector unit
 // close behind: every pair costs one exponential, a quarter-rate instruction.
-// 16384 rows of 16 heads of 128, bf16: 1.1 TFLOP in 1004 us, 1096 TFLOP/s, at
+// 16384 rows of 16 heads of 128, bf16: 1.1 TFLOP in 996 us, 1104 TFLOP/s, at
 // which the card has lowered its clock to 1.6 GHz (a large library matrix
-// product reaches 1212); 15 prompts of 12345 rows, 32 heads: 111 GFLOP in 150 us,
-// 740 TFLOP/s, a quarter of their tiles being the diagonal's.
+// product reaches 1212); 15 prompts of 12345 rows, 32 heads: 111 GFLOP in 150
+// us, 740 TFLOP/s, a quarter of their tiles being the diagonal's.
 //
 // A workgroup is 32 query rows for each of its four waves -- 32 rows of four
 // heads that share their keys, 64 of two or 128 of one, by what the heads of a
 // group divide into -- and walks the keys in tiles of kKeys through LDS, double
 // buffered: the next tiles go from memory straight into LDS while one is worked
 // on.  The more heads, the fewer tiles of the diagonal, of a window's edge and
-// behind a prompt's end its waves wait through (15 prompts, four heads against
-// one: 171 -> 154 us; windows of 500 on 8000 rows 58 -> 55).  Query rows come in
-// and 16-bit and f32 rows leave through LDS, whole rows a load or store and not
-// 16 bytes of each (the same prompts to 150; 8 prompts of 2000 rows 22.3 -> 19.6,
-// 40 rows of heads of 128 6.0 -> 6.3).  Up to heads
-// of 128 two workgroups share a CU; the scores of the next tile are formed
-// ahead of this one's weights, so that a wave's products run under its
+// behind a prompt's end its waves wait through (8 prompts of 2000 rows, 32 / 8
+// heads of 128: one head 25.1 us, four 22.3; windows of 500 on 8000 rows 58.2 and
+// 56.0).  Query rows come in and, where blocks fill the card, output rows leave
+// through LDS, whole rows a load or store and not 16 bytes of each (the same
+// prompts to 19.6, the windows to 52.6; 40 rows of heads of 128 6.0 -> 6.3).
+// Up to heads of 128 two workgroups share a CU; the scores of the next tile are
+// formed ahead of this one's weights, so that a wave's products run under its
 // exponentials as well (heads of 256, one wave a SIMD: 192 -> 166 us on six
 // prompts of 9000 rows).  Tiles for heads of 256 are 32 keys, whose one
 // accumulator would chain sixteen products: even and odd ones go to one each
@@ -618,20 +618,26 @@ __global__ __launch_bounds__(kThreads, D * G >= 256 ? 1 : 2) void packed_attn_ke
     store(std::integral_constant<int, kElemBf16>{});
 }
 
-// Groups of waves that the keys of a block are split over.  A block of 128 rows
-// with its waves side by side reads each key once for the most rows, which is
-// best where the blocks fill the card.  Where they do not, the block with the
-// most keys is what a launch takes, and blocks of 64 rows with two groups walk
-// half of them each.  Measured with one group and two, one prompt: heads of 64,
-// 280 blocks 34.6 and 23.5 us, 658 92 and 96; heads of 128 (a CU then has one
-// workgroup), 160 blocks 46.1 and 35.3, 224 blocks 20.8 and 23.6; heads of 256,
-// 256 blocks 132 and 102, 304 158 and 152, 358 186 and 195.  Up to one tile of
-// rows there is nothing to split (40 rows: heads of 128 6.3 and 7.5, of 256 8.2
-// and 9.2, but of 64 5.7 and 5.3).
+// Groups of waves that the keys of a block are split over.  128 (row, head)
+// pairs with the waves side by side read each key once for the most rows, which
+// is best where the blocks fill the card.  Where they do not, the block with the
+// most keys is what a launch takes, and blocks of 64 with two groups walk half of
+// them each.  Blocks are counted from the rows, and two more for every further
+// prompt: it ends inside a block, and makes the longest walk shorter, of which
+// the split takes its half.  Measured with one group and two, us:
+//   heads of 64: one prompt, 280 blocks 36.8 and 22.5, 512 31.7 and 31.5, 672
+//     42.3 and 45.8; eight prompts, 704 9.1 and 10.2;
+//   heads of 128, whose CU then has one workgroup: one prompt, 224 blocks 59.9
+//     and 48.4 (8 heads) or 20.1 and 22.3 (32 heads), 288 77.1 and 79.3; three
+//     prompts, 224 31.9 and 25.9; six prompts, 352 15.0 and 18.9;
+//   heads of 256: one prompt, 256 blocks 132 and 102, 304 157 and 150, 352 186
+//     and 194; ten prompts, 240 18.0 and 16.7, 304 25.2 and 27.9.
+// Up to one tile of rows there is nothing to split (40 rows: heads of 128 6.3 and
+// 7.6, of 256 8.8 and 9.4, but of 64 5.7 and 5.3).
 int groups_of(const PackedAttnArgs &a, int num_cus) {
-  const int64_t blocks = ((int64_t)a.tokens / (kWaveRows * kWaves) + 1) * a.nq;
+  const int64_t blocks = ((int64_t)a.tokens / (kWaveRows * kWaves) + 2 * (int64_t)a.sequences - 1) * a.nq;
   if (a.head_dim > 64 && a.tokens <= 64) return 1;
-  return 4 * blocks < (a.head_dim == 128 ? 3 : a.head_dim == 256 ? 5 : 8) * (int64_t)num_cus ? 2 : 1;
+  return 8 * blocks < (a.head_dim == 64 ? 18 : a.head_dim == 128 ? 8 : 9) * (int64_t)num_cus ? 2 : 1;
 }
 
 // log2 of the heads that a workgroup has: as many as divide a KV head's and its
