@@ -40,7 +40,10 @@
 // and the normaliser adds the rounded ones, so that the weights of a row still
 // sum to one; scores, maximum, sums and output stay f32 until the end.  The
 // running maximum moves only when a tile passes it by more than 2^8 (p stays
-// below 2^8), so most tiles skip the rescaling.
+// below 2^8), so most tiles skip the rescaling.  f16's carry a factor 2^7
+// beside, which cancels: they stay below 2^15, and what is lost of a small one
+// in f16's subnormal steps is 2^-32 of the running maximum and not 2^-25, which
+// some thousands of keys behind a heavy one would add up to what f16 shows.
 //
 // Masked places are not read into the result whatever they hold: scores there
 // become -inf, and where a tile has masked keys its values' infinities and
@@ -61,6 +64,7 @@ constexpr int kXcds = 8;
 constexpr int kWaitLoads = 0x0f70;  // s_waitcnt vmcnt(0)
 constexpr float kLog2e = 1.44269504088896341f;
 constexpr float kLazy = 8.0f;
+constexpr float kBiasF16 = 7.0f;  // f16 weights carry 2^kBiasF16
 constexpr float kInf = __builtin_inff();
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -378,7 +382,7 @@ __global__ __launch_bounds__(kThreads, D * G >= 256 ? 1 : 2) void packed_attn_ke
   };
   // weigh: the probabilities, as the B operand of the second product.
   auto weigh = [&](const f32x16 (&s)[kSubs], u32x4 (&p)[2 * kSubs]) {
-    const float m_use = m == -kInf ? 0.0f : m;  // no key so far: exp2(-inf)
+    const float m_use = m == -kInf ? 0.0f : m - (BF ? 0.0f : kBiasF16);  // no key so far: exp2(-inf)
 #pragma unroll
     for (int u = 0; u < kSubs; u++)
 #pragma unroll

@@ -612,8 +612,9 @@ int32_t hp_hip_paged_attention_device(const hp_hip_paged_cache_t *cache, const h
  * over its rows max(0, i - sliding_window + 1) .. i (0: no window).  Rows
  * d_offsets[s] .. d_offsets[s + 1] - 1 (rising, [sequence_count + 1]) are
  * sequence s; rows behind the last are left as they were.  Queries, keys and
- * values are of one type, which the probabilities are rounded to as well;
- * scores, softmax statistics and sums are f32.  What masked places hold does
+ * values are of one type, which the probabilities are rounded to as well (f16:
+ * one below 2^-32 of its row's largest may count as 0); scores, softmax
+ * statistics and sums are f32.  What masked places hold does
  * not matter.  Token strides of their own let them lie in one projection's
  * rows. */
 typedef struct hp_hip_packed_attention {

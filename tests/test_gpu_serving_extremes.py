@@ -1,0 +1,97 @@
+"""The operators over several sequences where their numbers are extreme: weights far below the largest, scores and scales
+far from one, infinities among what counts; and the rules ahead of a sampler.
+
+Bounds are those of test_gpu_serving.py's head, with what a case changes about them beside it.  Scores that the cases
+below make are sums of one non-zero exact product, and far enough apart (or the same) that f32's rounding of them leaves
+every weight 0 or 1 to below f32's step.
+"""
+import numpy as np
+import pytest
+
+import test_gpu_serving as base
+from heliopause_amd import hip_kernels as H
+
+pytestmark = pytest.mark.gpu
+
+U, ELEM = base.U, base.ELEM
+dev, dtype_of, half_step, sync, values = base.dev, base.dtype_of, base.half_step, base.sync, base.values
+
+
+@pytest.fixture(scope="module")
+def S(oracle):
+    from oracle import serving
+
+    return serving
+
+
+def tensor(a, type):
+    return base._torch().from_numpy(np.ascontiguousarray(a, dtype=np.float32)).cuda().to(dtype_of(type))
+
+
+def packed(q, k, v, offsets, *, type, out=None, scale=1.0, window=0):
+    """q, k, v device tensors [rows][heads][D]: the output as float64."""
+    t = base._torch()
+    out = out or type
+    rows, heads, D = q.shape
+    got = t.full((rows, heads, D), 7.0, dtype=dtype_of(out), device="cuda")
+    off = dev(np.asarray(offsets, np.int32))
+    sync()
+    H.packed_attention_device(len(offsets) - 1, off.data_ptr(), rows, heads, k.shape[1], D, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                              ELEM[type], got.data_ptr(), ELEM[out], scale=scale, sliding_window=window)
+    sync()
+    return values(got)
+
+
+def paged(pool, q, *, q_type="f32", out="f32", scale=1.0, window=0):
+    t = base._torch()
+    heads = q.shape[1]
+    x = tensor(q, q_type)
+    got = t.full(tuple(x.shape), 7.0, dtype=dtype_of(out), device="cuda")
+    sync()
+    H.paged_attention_device(pool.cache(), heads, x.data_ptr(), ELEM[q_type], got.data_ptr(), ELEM[out], scale=scale, sliding_window=window)
+    sync()
+    return values(got)
+
+
+def place(pool, sequence, keys, vals):
+    """Rows [position][kv head][D] of a sequence into its pages (as stored)."""
+    t = base._torch()
+    for rows, to in ((keys, pool.keys), (vals, pool.values)):
+        x = t.from_numpy(np.ascontiguousarray(rows, dtype=np.float32)).cuda().to(to.dtype)
+        for p in range(0, len(rows), pool.page):
+            n = min(pool.page, len(rows) - p)
+            to[int(pool.pages[sequence, p // pool.page]), :, :n] = x[p:p + n].transpose(0, 1)
+
+
+# (D, heads, many rows) that take each form of the packed kernel: few blocks split their keys over two groups of waves,
+# those of 2800 rows do not.
+FORMS = [(64, 1, False), (64, 32, True), (128, 1, False), (128, 16, True), (256, 1, False), (256, 16, True)]
+
+
+# ---- small weights -------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("D,heads,many", FORMS)
+@pytest.mark.parametrize("type", ["f16", "bf16"])
+def test_packed_weights_far_below_the_largest(hip, S, type, D, heads, many):
+    """A first key that outweighs each of the others by 2^22 to 2^28, and so many others that they count: their values
+    are 1 and its value is 0, so the output is the share that they have.  An f16 weight is off by half a subnormal step
+    at most, 2^-32 of the running maximum; the others' sum by n of those."""
+    n = 6000
+    rng = np.random.default_rng(D)
+    k = np.zeros((n, 1, D))
+    k[0, 0, 0], k[1:, 0, 1] = 16.0, rng.integers(-32, 33, n - 1) / 16.0
+    q = np.zeros((n, heads, D))
+    q[:, :, 0], q[:, :, 1] = 25.0 * np.log(2.0) / 16.0, np.log(2.0)
+    v = np.ones((n, 1, D))
+    v[0] = 0.0
+    q, k, v = (tensor(x, type) for x in (q, k, v))
+    got = packed(q, k, v, [0, n], type=type, out="f32")
+    at = sorted({n - 1, n - 2, n // 2 + 7, 1000, 130, 33, 1, 0} | set(rng.integers(0, n, 6).tolist()))
+    ref = S.packed_attention(values(q), values(k), values(v), [0, n], 0, 1.0, set(at))
+    u = base._torch().finfo(dtype_of(type)).eps / 2
+    for row in at:
+        r, mass, size, keys = ref[row]
+        weight = 2 * (size * D * U + 2.0 ** -20) + 2 * (keys + 64) * U
+        bound = 1.01 * (mass * weight[:, None] + u * (mass + np.abs(r))) + half_step("f32", r) + (2.0 ** -32 * keys if type == "f16" else 0.0)
+        base.check(got[row], r, bound)
+    assert got[n - 1].min() > 2.0 ** -15  # (they do count)
