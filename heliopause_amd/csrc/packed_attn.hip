@@ -310,6 +310,15 @@ __global__ __launch_bounds__(kThreads, D * G >= 256 ? 1 : 2) void packed_attn_ke
 #pragma unroll
     for (int i = 0; i < 16; i++) acc[t][i] = 0.0f;
   float m = -kInf, l = 0.0f;
+  constexpr float kBias = BF ? 0.0f : kBiasF16;
+  // weigh's s * factor - m, in one rounding, is off from 0 at the maximum by what
+  // m's own rounding lost: nothing that counts below 2^22, but past 2^24 whole
+  // powers of two, at last an infinity or 0 for every key.  The scores of rows
+  // that far out become differences of rounded products, over the factor, as
+  // they are settled (on the way of the moving maximum, which costs every other
+  // batch the least: 1 %; a test of its own a tile 1 to 4 %).
+  float bar = -kInf;   // a score above it is settled apart: past m + kLazy, or any of such a row
+  float m_use = 0.0f;  // what weigh takes off (a row without a key so far: exp2(-inf) whatever it is)
 
   u32x4 q[D / 16];
   // The steps of a tile.  scores: S^T of the keys in LDS.
@@ -371,18 +380,28 @@ __global__ __launch_bounds__(kThreads, D * G >= 256 ? 1 : 2) void packed_attn_ke
     float x, y;
     halves(most, &x, &y);
     most = fmaxf(x, y) * factor;
-    if (__any(most > m + kLazy)) {
+    if (__any(most > bar)) {
       const float m_new = most > m + kLazy ? most : m;
       const float alpha = m_new == m ? 1.0f : __builtin_amdgcn_exp2f(m - m_new);
       m = m_new;
       l *= alpha;
 #pragma unroll
       for (int t = 0; t < D / 32; t++) acc[t] *= alpha;
+      const bool far = fabsf(m) >= 0x1p22f && m != -kInf;
+      bar = far ? -kInf : m + kLazy;
+      m_use = far ? -kBias : m == -kInf ? 0.0f : m - kBias;
+      if (__any(far)) {
+        const float back = 1.0f / factor;
+#pragma unroll
+        for (int u = 0; u < kSubs; u++)
+#pragma unroll
+          for (int i = 0; i < 16; i++) s[u][i] = far ? (s[u][i] * factor - m) * back : s[u][i];
+      }
     }
   };
-  // weigh: the probabilities, as the B operand of the second product.
+  // weigh: the probabilities, as the B operand of the second product, of scores
+  // that are settled.
   auto weigh = [&](const f32x16 (&s)[kSubs], u32x4 (&p)[2 * kSubs]) {
-    const float m_use = m == -kInf ? 0.0f : m - (BF ? 0.0f : kBiasF16);  // no key so far: exp2(-inf)
 #pragma unroll
     for (int u = 0; u < kSubs; u++)
 #pragma unroll

@@ -95,3 +95,41 @@ def test_packed_weights_far_below_the_largest(hip, S, type, D, heads, many):
         bound = 1.01 * (mass * weight[:, None] + u * (mass + np.abs(r))) + half_step("f32", r) + (2.0 ** -32 * keys if type == "f16" else 0.0)
         base.check(got[row], r, bound)
     assert got[n - 1].min() > 2.0 ** -15  # (they do count)
+
+
+# ---- large scores and scales ---------------------------------------------------------------------------------------------
+
+def ranked(rng, n, ties):
+    """n whole numbers 1 .. 200 (a key's score in steps), the largest so far twice here and there."""
+    x = rng.integers(1, 200, n).astype(np.float64)
+    for i in range(ties, n, ties):
+        x[i] = x[:i].max()
+    return x
+
+
+def of_the_best(scores, rows):
+    """Mean of the rows [key][D] whose score is the largest."""
+    return rows[scores == scores.max()].mean(0)
+
+
+@pytest.mark.parametrize("power", [20, 22, 23, 25, 26, 27, 28, 29, 32, 60, 110])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("type", ["f16", "bf16"])
+def test_packed_large_scores(hip, type, sign, power):
+    """Scores of about 2^power, above or below zero: the best key has the weight, or the best ones share it.  Off by the
+    weights' rounding (none: 1) and that of sums and quotient, 2^-20 of the value."""
+    rng = np.random.default_rng(power)
+    for D, heads, many in FORMS:
+        lengths = [1500, 1300] if many else [150, 70]
+        n = sum(lengths)
+        rank = np.concatenate([ranked(rng, m, 17) for m in lengths])
+        k, q = np.zeros((n, 1, D)), np.zeros((n, heads, D))
+        k[:, 0, 3] = rank if sign > 0 else 256 - rank
+        q[:, :, 3] = sign
+        v = rng.integers(-8, 9, (n, 1, D)).astype(np.float64)
+        got = packed(*(tensor(x, type) for x in (q, k, v)), [0, lengths[0], n], type=type, out="f32", scale=2.0 ** (power - 8), window=90)
+        for begin, rows in ((0, lengths[0]), (lengths[0], lengths[1])):
+            for i in range(0, rows, 1 if n < 300 else 37):
+                first = max(0, i - 89)
+                ref = of_the_best(rank[begin + first:begin + i + 1], v[begin + first:begin + i + 1, 0])
+                assert np.all(np.abs(got[begin + i] - ref) <= 2.0 ** -20 * 8), (D, i)
