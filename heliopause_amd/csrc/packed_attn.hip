@@ -582,7 +582,9 @@ __global__ __launch_bounds__(kThreads, D * G >= 256 ? 1 : 2) void packed_attn_ke
         for (int i = 0; i < 16; i++) acc[t][i] = acc[t][i] * f + from[64 * (16 * t + i)] * e;
     }
   }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  // (every row of a prompt has a key, itself: a sum of 0 is scores of -inf only,
+  // and 0 / 0 their softmax)
+  const float inv = 1.0f / l;
   // With one group the wave's rows leave through LDS, so that a store is whole
   // rows and not 16 bytes of each: kSpan elements of them at a time, a row of 16
   // bits or half a row of f32, in chunks that are XORed as the keys' are.  With

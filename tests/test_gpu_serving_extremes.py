@@ -133,3 +133,19 @@ def test_packed_large_scores(hip, type, sign, power):
                 first = max(0, i - 89)
                 ref = of_the_best(rank[begin + first:begin + i + 1], v[begin + first:begin + i + 1, 0])
                 assert np.all(np.abs(got[begin + i] - ref) <= 2.0 ** -20 * 8), (D, i)
+
+
+# ---- infinities that count ---------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("D,heads,many", FORMS)
+@pytest.mark.parametrize("type", ["f16", "bf16"])
+def test_packed_rows_whose_every_score_is_minus_infinity(hip, type, D, heads, many):
+    """Row 0 and those behind it up to the first finite score: softmax of nothing but -inf is NaN, not a row without
+    keys; later rows have the finite keys' values alone."""
+    n = 2800 if many else 100
+    k, q = np.zeros((n, 1, D)), np.ones((n, heads, D))
+    k[:3, 0, 1], k[50, 0, 2] = -np.inf, -np.inf
+    v = np.full((n, 1, D), 5.0)
+    v[:3] = v[50] = 3.0
+    got = packed(*(tensor(x, type) for x in (q, k, v)), [0, n], type=type, scale=0.125)
+    assert np.isnan(got[:3]).all() and np.all(got[3:] == 5.0)
