@@ -48,7 +48,8 @@
 // Masked places are not read into the result whatever they hold: scores there
 // become -inf, and where a tile has masked keys its values' infinities and
 // NaNs are taken out of the product (0 * inf) and added back for the rows
-// that do see them.
+// that do see them, as a tile without masked keys has them (a NaN where the
+// weight is 0).
 #include <type_traits>
 
 #include "hp_mfma.h"
@@ -413,8 +414,9 @@ __global__ __launch_bounds__(kThreads, D * G >= 256 ? 1 : 2) void packed_attn_ke
         p[2 * u + (w >> 2)][w & 3] = pair;
       }
   };
-  // gather: O^T += V^T P^T with the values in LDS (check: keys may be masked).
-  auto gather = [&](const u32x4 (&p)[2 * kSubs], int buffer, bool check, auto edge) {
+  // gather: O^T += V^T P^T with the values in LDS (check: keys may be masked; the
+  // tile is then the one at `key`).
+  auto gather = [&](u32x4 (&p)[2 * kSubs], int buffer, bool check, int key, auto edge) {
     constexpr bool kMasked = decltype(edge)::value;
     const uint8_t *vt = tile_of(buffer, 1);
     // V^T fragments: product jj's k index 8 h + i is key 16 jj + 4 h + i (i < 4)
@@ -460,8 +462,27 @@ __global__ __launch_bounds__(kThreads, D * G >= 256 ? 1 : 2) void packed_attn_ke
       for (int t = 0; t < D / 32; t++) acc[t] = mfma32<BF>(f[t], p[jj], acc[t]);
     }
     if (kMasked && odd) {
-      // what infinities and NaNs come to in the rows that see them: the weights
-      // of +inf, of -inf and of NaN, each as a product of its own
+      // what infinities and NaNs come to in the rows that see them, as in a tile
+      // without masked keys: themselves, or a NaN where a weight is 0.  Of a weight
+      // its kind is enough, 1 for one above 0, -128 for a 0 that is seen (more than
+      // all the tile's others), in a product for each of +inf, -inf and NaN
+      int to = row - key - 4 * h, from = first - key - 4 * h;
+      // (these formed here and the weights in l by now: kept, they would take
+      // registers from the walk)
+      asm volatile("" : "+v"(to), "+v"(from), "+v"(l));
+#pragma unroll
+      for (int jj = 0; jj < 2 * kSubs; jj++)
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+          uint32_t of = 0;
+#pragma unroll
+          for (int b = 0; b < 2; b++) {
+            const int j = 16 * jj + 8 * (w >> 1) + 2 * (w & 1) + b;
+            const uint32_t one = BF ? 0x3f80u : 0x3c00u, none = BF ? 0xc300u : 0xd800u;
+            of |= ((p[jj][w] >> (16 * b) & 0xffffu) != 0 ? one : j <= to && j >= from ? none : 0u) << (16 * b);
+          }
+          p[jj][w] = of;
+        }
 #pragma unroll 1
       for (int kind = 1; kind < 4; kind++) {
         const float add = kind == 1 ? kInf : kind == 2 ? -kInf : __builtin_nanf("");
@@ -478,7 +499,8 @@ __global__ __launch_bounds__(kThreads, D * G >= 256 ? 1 : 2) void packed_attn_ke
             weight = mfma32<BF>(f, p[jj], weight);
           }
 #pragma unroll
-          for (int i = 0; i < 16; i++) acc[t][i] += weight[i] > 0.0f ? add : 0.0f;
+          for (int i = 0; i < 16; i++)
+            acc[t][i] += weight[i] > 0.0f ? add : weight[i] < 0.0f ? __builtin_nanf("") : 0.0f;
         }
       }
     }
@@ -520,12 +542,12 @@ __global__ __launch_bounds__(kThreads, D * G >= 256 ? 1 : 2) void packed_attn_ke
       next_loads(i);
       scores(sb, 1);
       weigh(sa, p);
-      gather(p, 0, false, std::false_type{});
+      gather(p, 0, false, 0, std::false_type{});
       settle(sb, 0, std::false_type{});
       next_loads(i + 1);
       scores(sa, 0);
       weigh(sb, p);
-      gather(p, 1, false, std::false_type{});
+      gather(p, 1, false, 0, std::false_type{});
       settle(sa, 0, std::false_type{});
     }
     next_loads(i);
@@ -534,7 +556,7 @@ __global__ __launch_bounds__(kThreads, D * G >= 256 ? 1 : 2) void packed_attn_ke
     if (sees(i)) {
       u32x4 p[2 * kSubs];
       weigh(sa, p);
-      gather(p, i & 1, edge_at(key_of(i)), std::true_type{});
+      gather(p, i & 1, edge_at(key_of(i)), key_of(i), std::true_type{});
     }
     if (more) {
       settle(sb, key_of(i + 1), std::true_type{});

@@ -149,3 +149,25 @@ def test_packed_rows_whose_every_score_is_minus_infinity(hip, type, D, heads, ma
     v[:3] = v[50] = 3.0
     got = packed(*(tensor(x, type) for x in (q, k, v)), [0, n], type=type, scale=0.125)
     assert np.isnan(got[:3]).all() and np.all(got[3:] == 5.0)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("type", ["f16", "bf16"])
+@pytest.mark.parametrize("odd", [np.inf, -np.inf, np.nan])
+def test_packed_value_whose_weight_is_nothing(hip, type, D, odd):
+    """A value that is no number under a weight that rounds to 0: its column is no number for every row that sees it,
+    wherever the tiles and blocks lie (the rows ahead of it in the batch move them), and stays for those that do not."""
+    lead_of = {}
+    for heads, lead in ((1, 0), (1, 1), (1, 40), (1, 77), (32 if D == 64 else 16, 2403), (32 if D == 64 else 16, 2500)):
+        n = 300
+        k, q = np.zeros((lead + n, 1, D)), np.zeros((lead + n, heads, D))
+        k[lead, 0, 0], q[:, :, 0] = 30.0, 30.0     # the first key has the weight
+        v = np.full((lead + n, 1, D), 2.0)
+        v[lead + 100, 0, 6] = odd
+        offsets = [0, n] if lead == 0 else [0, lead, lead + n]
+        got = packed(*(tensor(x, type) for x in (q, k, v)), offsets, type=type)[lead:]
+        assert np.all(got[:100] == 2.0) and np.all(np.delete(got, 6, 2) == 2.0)
+        assert not np.isfinite(got[100:, :, 6]).any()
+        lead_of[heads, lead] = got[:, 0, 6]
+    first = lead_of[1, 0]
+    assert all(np.array_equal(first, x, equal_nan=True) for x in lead_of.values())
