@@ -366,7 +366,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(const PagedAttn
       if (q4 == 0) sh_most[wave][c16] = most;
     }
     __syncthreads();
-    float factor;  // of a score, to base 2
+    float factor, lift;  // of a score, to base 2: their product
     {
       float most = sh_most[0][c16];
 #pragma unroll
@@ -377,7 +377,14 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(const PagedAttn
       const int e = (int)(__builtin_bit_cast(uint32_t, most) >> 23) - 127;
       const int shift = most > 0.0f && e < 128 ? 4 - max(e, -100) : 0;
       const float up = __builtin_bit_cast(float, (uint32_t)(127 + shift) << 23);
-      factor = a.scale * (CT == kElemE4m3 ? a.c.key_scale : 1.0f) * kLog2e / up;
+      // (past f32's range where both the query and the scales are large: in two
+      // steps, so that a score of 0 stays 0 and the others leave f32 only where
+      // they do by themselves)
+      const double whole = (double)a.scale * (CT == kElemE4m3 ? a.c.key_scale : 1.0f) * kLog2e *
+                           __builtin_bit_cast(float, (uint32_t)(127 - shift) << 23);
+      const bool far = whole >= 0x1p126;
+      factor = (float)(far ? whole * 0x1p-126 : whole);
+      lift = far ? 0x1p126f : 1.0f;
       const bool rest = c16 >= kHeads;
 #pragma unroll
       for (int i = 0; i < kMine; i++) {
@@ -447,7 +454,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(const PagedAttn
 #pragma unroll
       for (int j = 0; j < kKeys; j++) {
         const float v = s[j >> 2][j & 3];
-        x[j] = (v + dpp_f32<kDppRor8>(v)) * factor;
+        x[j] = (v + dpp_f32<kDppRor8>(v)) * factor * lift;
       }
       if (edge) {  // the same for the wave
 #pragma unroll

@@ -135,6 +135,47 @@ def test_packed_large_scores(hip, type, sign, power):
                 assert np.all(np.abs(got[begin + i] - ref) <= 2.0 ** -20 * 8), (D, i)
 
 
+@pytest.mark.parametrize("size,scale", [(2.0 ** 13, 2.0 ** 120), (1e20, 2.0 ** 90), (2.0 ** 127, 64.0), (2.0 ** 127, 2.0 ** 120), (2.0 ** 100, 2.0 ** 20)])
+@pytest.mark.parametrize("type,q_type", [("f16", "f32"), ("bf16", "f32"), ("bf16", "bf16"), ("e4m3", "f32")])
+def test_paged_large_queries_at_large_scales(hip, type, q_type, size, scale):
+    """Keys of zeros score 0 whatever the query and the scale are, and share the weight; one key against the query's
+    direction then has none, one along it all (where its score is within f32)."""
+    rng = np.random.default_rng(1)
+    for D in (64, 128, 256):
+        lengths = [40, 300, 40, 1, 300]
+        pool = base.Pool(rng, lengths, 1, D, 16, type, scales=(1.0, 1.0))
+        q = np.full((len(lengths), 2, D), size)
+        refs = []
+        for s, n in enumerate(lengths):
+            k, v = np.zeros((n, 1, D)), rng.integers(-8, 9, (n, 1, D)).astype(np.float64)
+            refs.append(v[:, 0].mean(0))
+            if s == 1:
+                k[7, 0, 5] = -1.0
+                refs[-1] = np.delete(v[:, 0], 7, 0).mean(0)
+            if s == 4 and size * scale <= 2.0 ** 133:
+                k[299, 0, 5] = 2.0 ** -6
+                refs[-1] = v[299, 0]
+            place(pool, s, k, v)
+        got = paged(pool, q, q_type=q_type, scale=scale)
+        # (weights 1 in two parts, exact; sums of up to 300 whole numbers exact; the quotient)
+        assert np.all(np.abs(got - np.stack(refs)[:, None]) <= 2.0 ** -20 * 8), D
+
+
+def test_paged_scores_of_ordinary_size_from_far_factors(hip, S):
+    """bf16 keys of some 2^-125 under queries and a scale whose product is past f32's range."""
+    rng = np.random.default_rng(2)
+    lengths = [1, 40, 400]
+    pool = base.Pool(rng, lengths, 2, 128, 16, "bf16")
+    for s, n in enumerate(lengths):
+        place(pool, s, rng.uniform(1, 4, (n, 2, 128)) * rng.choice([-1, 1], (n, 2, 128)) * 2.0 ** -126, rng.standard_normal((n, 2, 128)))
+    q = np.zeros((3, 4, 128))
+    q[:, :, [3, 40, 77]] = rng.uniform(1, 2, (3, 4, 3)) * rng.choice([-1, 1], (3, 4, 3)) * 2.0 ** 101
+    got = paged(pool, q, scale=2.0 ** 30)
+    ref, mass, size, count = S.paged_attention(values(tensor(q, "f32")), values(pool.keys), values(pool.values), pool.lengths,
+                                               pool.pages, pool.page, pool.count, 0, 2.0 ** 30)
+    base.check(got, ref, base.paged_bound("f32", "bf16", ref, mass, size, count, 128))
+
+
 # ---- infinities that count ---------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("D,heads,many", FORMS)
