@@ -478,8 +478,11 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(const PagedAttn
 #pragma unroll
         for (int i = 0; i < kT; i++) acc[i] *= alpha;
       }
-      // a row without a key so far: exp2(-inf - 0) = 0
-      const float m_use = m_run == kNegInf ? 0.0f : m_run - kBias;
+      // a row without a key so far: exp2(-inf - 0) = 0.  From 2^27 on f32's steps
+      // are as large as the bias, and what is left of it could be more: 2^16 is
+      // past f16
+      float m_use = m_run == kNegInf ? 0.0f : m_run - kBias;
+      m_use = m_run - m_use > 15.0f ? m_run : m_use;
       uint32_t pf[kKeys / 2];
       const bool rest = c16 >= kHeads;
       uint32_t pb[kKeys];

@@ -135,6 +135,30 @@ def test_packed_large_scores(hip, type, sign, power):
                 assert np.all(np.abs(got[begin + i] - ref) <= 2.0 ** -20 * 8), (D, i)
 
 
+@pytest.mark.parametrize("power", [20, 22, 25, 26, 27, 28, 29, 32, 60, 110])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("type", ["f16", "bf16", "e4m3"])
+def test_paged_large_scores(hip, type, sign, power):
+    """The same over pages, whole and split over workgroups.  (e4m3 holds the whole numbers up to 16: ranks below that)"""
+    rng = np.random.default_rng(power)
+    for D in (64, 128, 256):
+        lengths = [1, 33, 150, 3000]
+        pool = base.Pool(rng, lengths, 1, D, 16, type, scales=(1.0, 1.0))
+        ranks = []
+        for s, n in enumerate(lengths):
+            rank = ranked(rng, n, 17)
+            rank = np.ceil(rank / 14.0) if type == "e4m3" else rank
+            k, v = np.zeros((n, 1, D)), rng.integers(-8, 9, (n, 1, D)).astype(np.float64)
+            k[:, 0, 3] = rank if sign > 0 else (16 if type == "e4m3" else 256) - rank
+            place(pool, s, k, v)
+            ranks.append((rank, v))
+        q = np.zeros((len(lengths), 3, D))
+        q[:, :, 3] = sign
+        got = paged(pool, q, scale=2.0 ** (power - (4 if type == "e4m3" else 8)))
+        for s, (rank, v) in enumerate(ranks):
+            assert np.all(np.abs(got[s] - of_the_best(rank, v[:, 0])) <= 2.0 ** -20 * 8), (D, s)
+
+
 @pytest.mark.parametrize("size,scale", [(2.0 ** 13, 2.0 ** 120), (1e20, 2.0 ** 90), (2.0 ** 127, 64.0), (2.0 ** 127, 2.0 ** 120), (2.0 ** 100, 2.0 ** 20)])
 @pytest.mark.parametrize("type,q_type", [("f16", "f32"), ("bf16", "f32"), ("bf16", "bf16"), ("e4m3", "f32")])
 def test_paged_large_queries_at_large_scales(hip, type, q_type, size, scale):
