@@ -29,7 +29,9 @@
 // cache's scales join the score's factor and the end.
 //
 // Masked keys (behind the length, before the window, on an absent page) get
-// score -inf and value zero, whatever their slots hold.
+// score -inf and value zero, whatever their slots hold.  A part of masked keys
+// only has the maximum -inf; one whose other keys all score -inf themselves the
+// lowest finite number: a row of nothing else is 0 / 0, not zeros.
 //
 // Split.  All (sequence, KV head) rows' steps of 128 keys (32 for each of the
 // four waves; heads of 256 half as many) lie end to end, and each workgroup
@@ -73,6 +75,7 @@ constexpr int kXcds = 8;  // workgroup i runs on XCD i % 8
 constexpr float kLog2e = 1.44269504088896341f;
 constexpr float kBias = 10.0f;  // p carries 2^kBias
 constexpr float kNegInf = -__builtin_inff();
+constexpr float kUnweighed = -3.40282346638528860e38f;  // the maximum of a part that has keys, all of which score -inf
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -140,6 +143,12 @@ __device__ __forceinline__ float column_max(float v) {
 __device__ __forceinline__ float column_sum(float v) {
   v += __shfl_xor(v, 16);
   return v + __shfl_xor(v, 32);
+}
+
+// A row's 1 / l (times the cache's scale): 0 without a key, NaN where nothing has
+// weight.
+__device__ __forceinline__ float row_scale(float m, float l, float value_scale) {
+  return m == kNegInf && l == 0.0f ? 0.0f : l == 0.0f ? __builtin_nanf("") : value_scale / l;
 }
 
 // Sum of v over the lanes up to this one.
@@ -277,6 +286,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(const PagedAttn
 #pragma unroll
     for (int t = 0; t < kT; t++) acc[t] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
     float m_run = kNegInf, l_part = 0.0f;
+    bool has_key = false;  // the lane has seen a key that is not masked
 
     // this wave's tiles: key .. key + kSub - 1 at key = begin + kStep i + kSub wave
     const int key0 = span.begin + (int)i0 * kStep + kSub * wave;
@@ -456,12 +466,14 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(const PagedAttn
         const float v = s[j >> 2][j & 3];
         x[j] = (v + dpp_f32<kDppRor8>(v)) * factor * lift;
       }
+      has_key = has_key || !edge;
       if (edge) {  // the same for the wave
 #pragma unroll
         for (int j = 0; j < kKeys; j++) {
           const int at_key = key + 16 * (j >> 2) + 4 * q4 + (j & 3);
           const bool off = at_key < span.first || at_key >= span.end || page[j >> 2] < 0;
           x[j] = off ? kNegInf : x[j];
+          has_key = has_key || !off;
 #pragma unroll
           for (int w = 0; w < T::kValueWords; w++) t.v[j][w] = off ? 0u : t.v[j][w];
         }
@@ -528,6 +540,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(const PagedAttn
     // the four waves' parts, joined in LDS.  Lane (q4, c): head c, elements
     // kT (4 q4 + r) + i
     const float l_run = column_sum(l_part);
+    if (__any(has_key)) m_run = fmaxf(m_run, kUnweighed);
 #pragma unroll
     for (int i = 0; i < kT; i++)
 #pragma unroll
@@ -568,7 +581,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(const PagedAttn
       }
       if (h >= live) continue;
       if (whole) {
-        const float inv = l == 0.0f ? 0.0f : (CT == kElemE4m3 ? a.c.value_scale : 1.0f) / l;
+        const float inv = row_scale(m, l, CT == kElemE4m3 ? a.c.value_scale : 1.0f);
 #pragma unroll
         for (int j = 0; j < 4; j++) o[j] *= inv;
         store4(a.out, seq * a.out_stride + (int64_t)(kvh * group + h0 + h) * D + 4 * d, a.out_type, o);
@@ -665,7 +678,7 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(const PagedAttnAr
     o[2] += f * v.z;
     o[3] += f * v.w;
   }
-  const float inv = l == 0.0f ? 0.0f : (a.c.type == kElemE4m3 ? a.c.value_scale : 1.0f) / l;
+  const float inv = row_scale(most, l, a.c.type == kElemE4m3 ? a.c.value_scale : 1.0f);
 #pragma unroll
   for (int j = 0; j < 4; j++) o[j] *= inv;
   store4(a.out, out, a.out_type, o);

@@ -591,10 +591,12 @@ int32_t hp_hip_paged_append_device(const hp_hip_paged_cache_t *cache, const hp_h
  * (head_count / head_count_kv).  Any query type goes with any cache type; the
  * sums are f32 and the products exact to some 2^-16 (bf16 pages) or 2^-22
  * (others) of the largest.  A sequence without a key (empty, or all its pages
- * absent) has zeros.  What masked places hold does not matter; an infinity or
- * NaN among the elements that count leaves no finite number in the outputs that
- * it reaches, and the others as they are.  Two launches, over scratch of the
- * stream's. */
+ * absent) has zeros.  What masked places hold does not matter.  A value's
+ * infinity or NaN that counts leaves no finite number in the outputs that it
+ * reaches, and the others as they are; a key's or a query's makes scores of it
+ * that are NaN or infinite (as one past f32's range is): -inf has no weight, and
+ * a head's output is NaN where another of these is among its scores or all are
+ * -inf.  Two launches, over scratch of the stream's. */
 typedef struct hp_hip_paged_attention {
   const void *d_q; /* [sequence_count][head_count][head_dim] of q_type */
   void *d_output;  /* [sequence_count][head_count][head_dim] of out_type */

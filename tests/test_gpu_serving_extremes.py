@@ -236,3 +236,46 @@ def test_packed_value_whose_weight_is_nothing(hip, type, D, odd):
         lead_of[heads, lead] = got[:, 0, 6]
     first = lead_of[1, 0]
     assert all(np.array_equal(first, x, equal_nan=True) for x in lead_of.values())
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_paged_rows_whose_every_score_is_minus_infinity(hip, D):
+    """f16 keys of -inf under queries of 1 + 2^-12, both of whose f16 parts are above zero: the scores are -inf.  Where
+    all are, the row is NaN; where one is not, its value; where there is no key, zeros.  Rows that one workgroup has
+    whole, and rows in many parts."""
+    lengths = [1, 40, 200, 5000, 40, 200, 5000, 5000, 70, 0, 5000]
+    pool = base.Pool(np.random.default_rng(4), lengths, 1, D, 16, "f16")
+    one = {4: 39, 5: 3, 6: 4999, 7: 2500}  # sequence: its one finite key
+    for s, n in enumerate(lengths):
+        if not n:
+            continue
+        k, v = np.zeros((n, 1, D)), np.full((n, 1, D), 3.0)
+        k[:, 0, 1] = -np.inf
+        if s in one:
+            k[one[s], 0, 1], v[one[s]] = 1.0, 5.0
+        place(pool, s, k, v)
+    pool.pages[8] = -1                      # no page at all
+    pool.pages[10, :300] = -1               # only the last keys are there, all of them -inf
+    pool.upload()
+    got = paged(pool, np.full((len(lengths), 11, D), 1.0 + 2.0 ** -12))
+    for s in range(len(lengths)):
+        if s in (8, 9):
+            assert np.all(got[s] == 0.0), s
+        elif s in one:
+            assert np.all(got[s] == 5.0), s
+        else:
+            assert np.isnan(got[s]).all(), s
+
+
+def test_paged_value_whose_weight_is_nothing(hip):
+    for type in ("f16", "bf16"):
+        pool = base.Pool(np.random.default_rng(3), [300, 300], 1, 64, 16, type)
+        for s in range(2):
+            k, v = np.zeros((300, 1, 64)), np.full((300, 1, 64), 2.0)
+            k[5, 0, 0] = 30.0
+            v[100 + 150 * s, 0, 6] = np.inf
+            place(pool, s, k, v)
+        q = np.zeros((2, 3, 64))
+        q[:, :, 0] = 30.0
+        got = paged(pool, q)
+        assert np.all(np.delete(got, 6, 2) == 2.0) and not np.isfinite(got[:, :, 6]).any()
