@@ -2987,6 +2987,7 @@ int32_t paged_attention_check(const hp_hip_paged_cache_t *cache, const hp_hip_pa
   if (!score_scale(p->scale) || p->scale * a->c.key_scale > 0x1p120f)
     return fail(HP_ERR_ARG, "scale (times the key scale) must be positive, up to 2^120");
   if (p->sliding_window < 0) return fail(HP_ERR_ARG, "sliding_window must not be negative");
+  if (p->reserved != 0) return fail(HP_ERR_ARG, "reserved field must be 0");
   const size_t row = (size_t)p->head_count * a->c.head_dim;
   if ((rc = row_stride(p->q_stride, row, elem_bytes(p->q_type), a->c.sequences, &a->q_stride)) != HP_OK) return rc;
   if ((rc = row_stride(p->output_stride, row, elem_bytes(p->out_type), a->c.sequences, &a->out_stride)) != HP_OK) return rc;
