@@ -3051,6 +3051,7 @@ int32_t logit_rules_check(const hp_hip_logit_rules_t *p, LogitRulesArgs *a) {
   if (p->rows > 65535) return fail(HP_ERR_SHAPE, "too many rows");
   if (p->n < 1 || p->n > most) return fail(HP_ERR_SHAPE, "n must be 1..2^30");
   if (p->history_stride > most || p->bias_stride > most) return fail(HP_ERR_SHAPE, "a list is too long");
+  if (!std::isfinite(p->softcap) || p->softcap < 0.0) return fail(HP_ERR_ARG, "softcap must be finite and not negative");
   const size_t words = (p->n + 31) / 32;
   const size_t logits = p->logits_stride ? p->logits_stride : p->n, output = p->output_stride ? p->output_stride : p->n;
   const size_t allowed = p->allowed_stride ? p->allowed_stride : words;
@@ -3082,7 +3083,8 @@ int32_t logit_rules_check(const hp_hip_logit_rules_t *p, LogitRulesArgs *a) {
                       (int64_t)p->bias_stride,
                       (int64_t)allowed,
                       (int)p->rows,
-                      (int)p->n};
+                      (int)p->n,
+                      p->softcap};
   return HP_OK;
 }
 

@@ -79,6 +79,7 @@ struct LogitRulesArgs {
   const uint32_t *allowed;
   int64_t logits_stride, out_stride, history_stride, bias_stride, allowed_stride;
   int rows, n;
+  double softcap;  // 0: none
 };
 hipError_t launch_logit_rules(const LogitRulesArgs &a, hipStream_t s);
 

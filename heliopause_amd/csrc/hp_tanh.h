@@ -139,4 +139,7 @@ __host__ __device__ inline double hp_tanh(double x) {
   return neg ? -z : z;
 }
 
+// The logit softcap of layers.ts:407-412, cap > 0.
+__device__ __forceinline__ float softcap_value(float v, double cap) { return (float)(hp_tanh((double)v / cap) * cap); }
+
 }  // namespace hp

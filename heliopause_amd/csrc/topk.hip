@@ -71,9 +71,7 @@ __device__ __forceinline__ uint32_t ord_bits(float v) {
   return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 
-__device__ __forceinline__ float softcap_value(float v, double cap) {
-  return cap > 0.0 ? (float)(hp_tanh((double)v / cap) * cap) : v;
-}
+__device__ __forceinline__ float capped(float v, double cap) { return cap > 0.0 ? softcap_value(v, cap) : v; }
 
 __device__ __forceinline__ uint64_t make_key(float v, uint32_t id) {
   return ((uint64_t)ord_bits(v) << 32) | (uint64_t)(0xFFFFFFFFu - id);
@@ -197,7 +195,7 @@ __device__ __forceinline__ void chunk_keys(const float *__restrict__ src, int n,
 #pragma unroll
   for (int i = 0; i < 4; i++) {
     const int id = base + i * kTopkThreads;
-    key[i] = id < n ? make_key(softcap_value(v[i], cap), (uint32_t)id) : 0;
+    key[i] = id < n ? make_key(capped(v[i], cap), (uint32_t)id) : 0;
   }
 }
 
@@ -314,7 +312,7 @@ __global__ __launch_bounds__(kTopkThreads) void topk_final_kernel(const float *_
       const uint32_t cid = 0xFFFFFFFFu - (uint32_t)mine;
       if (mine != 0 && (uint32_t)lane < want && cid < (uint32_t)n) {
         id = cid;
-        v = softcap_value(src[id], cap);
+        v = capped(src[id], cap);
       }
       ids[(size_t)row * k + lane] = id;
       vals[(size_t)row * k + lane] = v;

@@ -200,7 +200,8 @@ class HipLogitRules(ctypes.Structure):
                                                "d_prompt_lengths", "d_repetition", "d_frequency", "d_presence",
                                                "d_bias_ids", "d_bias_values", "d_bias_counts", "d_allowed")] + \
                [(n, _sz) for n in ("rows", "n", "logits_stride", "output_stride", "history_stride", "bias_stride",
-                                   "allowed_stride")]
+                                   "allowed_stride")] + \
+               [("softcap", ctypes.c_double)]
 
 
 def _declare_serving(L: ctypes.CDLL) -> None:
@@ -819,9 +820,10 @@ def logit_rules_device(rows: int, n: int, d_logits: int, d_output: int, *, d_his
                        d_repetition: int = 0, d_frequency: int = 0, d_presence: int = 0, d_bias_ids: int = 0,
                        d_bias_values: int = 0, d_bias_counts: int = 0, bias_stride: int = 0, d_allowed: int = 0,
                        allowed_stride: int = 0, logits_stride: int = 0, output_stride: int = 0,
-                       stream: int = 0) -> None:
-    """Penalties for repeated tokens, biases and the grammar's mask on [rows][n] logits (d_output may be d_logits)."""
+                       stream: int = 0, softcap: float = 0.0) -> None:
+    """Penalties for repeated tokens, biases and the grammar's mask on [rows][n] logits (d_output may be d_logits).  A
+    model's softcap is given here and the top-k behind gets 0: what is masked stays -inf."""
     p = HipLogitRules(d_logits, d_output, d_history, d_history_lengths, d_prompt_lengths, d_repetition, d_frequency,
                       d_presence, d_bias_ids, d_bias_values, d_bias_counts, d_allowed, rows, n, logits_stride,
-                      output_stride, history_stride, bias_stride, allowed_stride)
+                      output_stride, history_stride, bias_stride, allowed_stride, softcap)
     assertHipOk(lib().hp_hip_logit_rules_device(ctypes.byref(p), stream or None), "logit_rules")

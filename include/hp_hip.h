@@ -638,12 +638,16 @@ int32_t hp_hip_packed_attention_device(const hp_hip_packed_attention_t *attentio
 
 /* What a request changes about its logits ahead of hp_hip_topk_device: per row
  * and token, in f32 and in this order,
+ *   softcap * tanh(x / softcap)               softcap > 0: as hp_hip_topk_device forms it (layers.ts:407-412)
  *   x > 0 ? x / repetition : x * repetition   the token is in the row's history
  *   x - frequency * count                     count: its places in the history from
  *   x - presence, if count > 0                d_prompt_lengths[row] on
  *   x + bias                                  the last entry of the token in the row's list
  *   -inf                                      bit token % 32 of mask word token / 32 is 0
- * A row that the mask leaves nothing is all -inf.  Tokens outside 0 .. n - 1
+ * A row that the mask leaves nothing is all -inf (of such candidates
+ * hp_hip_sample_device takes the first).  The softcap of a model that has one is
+ * given here and hp_hip_topk_device gets 0: its own would be formed of what the
+ * rules leave, -inf a -softcap that can be sampled.  Tokens outside 0 .. n - 1
  * (padding) count nowhere.  Each array may be NULL where the rule is not used
  * (d_history with its lengths; the three bias arrays together).  d_output may
  * be d_logits. */
@@ -662,6 +666,7 @@ typedef struct hp_hip_logit_rules {
   size_t logits_stride, output_stride;          /* from row to row, below 2^32; 0: n */
   size_t history_stride, bias_stride;           /* up to 2^30; longer lengths count as these */
   size_t allowed_stride;                        /* words; 0: (n + 31) / 32 */
+  double softcap;                               /* finite; 0: none */
 } hp_hip_logit_rules_t;
 int32_t hp_hip_logit_rules_device(const hp_hip_logit_rules_t *rules, void *stream);
 

@@ -279,3 +279,78 @@ def test_paged_value_whose_weight_is_nothing(hip):
         q[:, :, 0] = 30.0
         got = paged(pool, q)
         assert np.all(np.delete(got, 6, 2) == 2.0) and not np.isfinite(got[:, :, 6]).any()
+
+
+# ---- the rules ahead of a sampler ------------------------------------------------------------------------------------------
+
+def capped(oracle, x, cap):
+    return np.array([oracle.softcap(float(v), cap) for v in np.asarray(x, np.float32).ravel()], np.float32).reshape(np.shape(x))
+
+
+@pytest.mark.parametrize("rows,n", [(1, 5), (3, 2049), (2, 6000)])
+@pytest.mark.parametrize("cap", [30.0, 0.7])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_rules_cap_the_logits_first(hip, oracle, S, rows, n, cap, in_place):
+    """To the bit: cap * tanh(logit / cap) as the top-k forms it, then the rules on that."""
+    t = base._torch()
+    rng = np.random.default_rng(n)
+    logits = (rng.standard_normal((rows, n)) * 40).astype(np.float32)
+    logits[0, :4] = np.inf, -np.inf, 0.0, np.nan
+    history = rng.integers(0, n, (rows, 50)).astype(np.int32)
+    told, r, f = np.full(rows, 50, np.int32), rng.uniform(0.8, 1.4, rows).astype(np.float32), rng.uniform(0, 1, rows).astype(np.float32)
+    ids, bias, counts = rng.integers(0, n, (rows, 3)).astype(np.int32), rng.standard_normal((rows, 3)).astype(np.float32), np.full(rows, 3, np.int32)
+    allowed = rng.integers(0, 2 ** 32, (rows, (n + 31) // 32), dtype=np.uint64).astype(np.uint32)
+    x = dev(logits)
+    out = x if in_place else t.zeros_like(x)
+    d = [dev(a) for a in (history, told, r, f, ids, bias, counts, allowed.view(np.int32))]
+    p = [a.data_ptr() for a in d]
+    sync()
+    H.logit_rules_device(rows, n, x.data_ptr(), out.data_ptr(), d_history=p[0], history_stride=50, d_history_lengths=p[1],
+                         d_repetition=p[2], d_frequency=p[3], d_bias_ids=p[4], d_bias_values=p[5], d_bias_counts=p[6], bias_stride=3,
+                         d_allowed=p[7], softcap=cap)
+    sync()
+    ref = S.logit_rules(capped(oracle, logits, cap), history, told, None, r, f, None, ids, bias, counts, allowed)
+    got = out.cpu().numpy()
+    assert np.array_equal(np.isnan(got), np.isnan(ref))
+    assert np.array_equal(got.view(np.uint32)[~np.isnan(ref)], ref.view(np.uint32)[~np.isnan(ref)])
+
+
+def test_masked_tokens_have_no_weight_under_a_softcap(hip, oracle):
+    """Rules with the cap, top-k without one, sampler: what the mask forbids is never a number again and is never
+    sampled, and where nothing is masked the candidates are those of the top-k's own cap, to the bit."""
+    t = base._torch()
+    rng = np.random.default_rng(5)
+    rows, n, k = 4, 5000, 40
+    logits = (rng.standard_normal((rows, n)) * 20).astype(np.float32)
+    allowed = np.full((rows, (n + 31) // 32), 0xFFFFFFFF, np.uint32)
+    few = {1: [17], 2: [3, 4999], 3: list(range(100, 130))}  # row: the tokens that its mask leaves
+    for row, tokens in few.items():
+        allowed[row] = 0
+        for i in tokens:
+            allowed[row, i // 32] |= np.uint32(1 << (i % 32))
+            logits[row, i] = -20.0 - i % 7
+    x, m = dev(logits), dev(allowed.view(np.int32))
+    ruled = t.zeros_like(x)
+    ids, vals = (t.zeros((2, rows, k), dtype=d, device="cuda") for d in (t.int32, t.float32))
+    state, tokens, kept = (t.zeros(c, dtype=t.int32, device="cuda") for c in (1, rows, rows))
+    probs = t.full((rows, k), -1.0, dtype=t.float64, device="cuda")
+    sync()
+    H.logit_rules_device(rows, n, x.data_ptr(), ruled.data_ptr(), d_allowed=m.data_ptr(), softcap=30.0)
+    L = H.lib()
+    H.assertHipOk(L.hp_hip_topk_device(ruled.data_ptr(), rows, n, k, 0.0, ids[0].data_ptr(), vals[0].data_ptr(), None), "topk")
+    H.assertHipOk(L.hp_hip_topk_device(x.data_ptr(), rows, n, k, 30.0, ids[1].data_ptr(), vals[1].data_ptr(), None), "topk")
+    drawn = [set() for _ in range(rows)]
+    for _ in range(200):
+        H.sample_device(ids[0].data_ptr(), vals[0].data_ptr(), rows, k, k, {"doSample": True, "topK": k, "temperature": 1.5, "topP": 1.0},
+                        state.data_ptr(), tokens.data_ptr(), probs.data_ptr(), kept.data_ptr(), 0)
+        sync()
+        for row, token in enumerate(tokens.tolist()):
+            drawn[row].add(token)
+    ids, vals, probs = ids.cpu().numpy(), vals.cpu().numpy(), probs.cpu().numpy()
+    assert np.array_equal(ids[0, 0], ids[1, 0]) and np.array_equal(vals[0, 0].view(np.uint32), vals[1, 0].view(np.uint32))
+    for row, left in few.items():
+        there = np.isfinite(vals[0, row])
+        assert sorted(ids[0, row][there]) == left and np.all(vals[0, row][~there] == -np.inf)
+        assert np.array_equal(vals[0, row][there], np.sort(capped(oracle, logits[row, left], 30.0))[::-1])
+        assert np.all(probs[row][~there] == 0.0) and abs(probs[row][there].sum() - 1.0) < 1e-12
+        assert drawn[row] <= set(left)
