@@ -269,11 +269,18 @@ _stream = None
 
 
 def _the_stream():
-    """The program's stream: every pass of this process is queued on it."""
+    """The stream that a pass is queued on: the current one, so that what comes before and after it in the program keeps
+    its order.  Torch's default stream has no handle that the framework's calls take (0 is the framework's own), so a
+    program on that one moves to a stream of its own, behind what it has queued."""
     global _stream
-    if _stream is None:
-        _stream = torch.cuda.Stream()
-    return _stream.cuda_stream
+    current = torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())  # (current_stream() takes 3 us of a call of 7)
+    if current == 0:
+        if _stream is None:
+            _stream = torch.cuda.Stream()
+        _stream.wait_stream(torch.cuda.current_stream())
+        torch.cuda.set_stream(_stream)
+        current = _stream.cuda_stream
+    return current
 
 
 def _p(t):
