@@ -107,13 +107,6 @@ __device__ __forceinline__ uint16_t bf16_bits(float v) { return __builtin_bit_ca
 __device__ __forceinline__ uint16_t f16_bits(float v) { return __builtin_bit_cast(uint16_t, (_Float16)v); }
 __device__ __forceinline__ float bf16_value(uint32_t bits16) { return __builtin_bit_cast(float, bits16 << 16); }
 
-// One element of an f32 / f16 / bf16 row as f32.
-__device__ __forceinline__ float load_elem(const void *p, int64_t i, int type) {
-  if (type == kElemF32) return static_cast<const float *>(p)[i];
-  const uint16_t b = static_cast<const uint16_t *>(p)[i];
-  return type == kElemF16 ? (float)__builtin_bit_cast(_Float16, b) : bf16_value(b);
-}
-
 // Four consecutive elements, rounded to nearest even where they leave in 16
 // bits (a value past the largest f16 becomes an infinity).
 __device__ __forceinline__ void store4(void *p, int64_t i, int type, const float (&v)[4]) {
