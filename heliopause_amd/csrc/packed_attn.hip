@@ -5,10 +5,12 @@
 //
 // The matrix cores bound it (4 D flop a pair and head), with the vector unit
 // close behind: every pair costs one exponential, a quarter-rate instruction.
-// 16384 rows of 16 heads of 128, bf16: 1.1 TFLOP in 996 us, 1104 TFLOP/s, at
-// which the card has lowered its clock to 1.6 GHz (a large library matrix
-// product reaches 1212); 15 prompts of 12345 rows, 32 heads: 111 GFLOP in 150
-// us, 740 TFLOP/s, a quarter of their tiles being the diagonal's.
+// 16384 rows of 16 heads of 128, bf16: 1.1 TFLOP in 1000 to 1080 us, 1020 to 1100
+// TFLOP/s, by the clock that the card's power leaves it (1190 us at 1.53 GHz, the
+// matrix cores busy 58 % of the cycles; a large library matrix product reaches
+// 1212); 15 prompts of 12345 rows, 32 heads: 111 GFLOP in 150 to 160 us, 690 to
+// 740 TFLOP/s (169 us at 1.96 GHz, 35 %), a quarter of their tiles being the
+// diagonal's.
 //
 // A workgroup is 32 query rows for each of its four waves -- 32 rows of four
 // heads that share their keys, 64 of two or 128 of one, by what the heads of a
@@ -16,8 +18,8 @@
 // buffered: the next tiles go from memory straight into LDS while one is worked
 // on.  The more heads, the fewer tiles of the diagonal, of a window's edge and
 // behind a prompt's end its waves wait through (8 prompts of 2000 rows, 32 / 8
-// heads of 128: one head 25.1 us, four 22.3; windows of 500 on 8000 rows 58.2 and
-// 56.0).  Query rows come in and, where blocks fill the card, output rows leave
+// heads of 128: one head 25.1 us, four 22.3; windows of 500 on 8000 rows of half as
+// many 58.2 and 56.0).  Query rows come in and, where blocks fill the card, output rows leave
 // through LDS, whole rows a load or store and not 16 bytes of each (the same
 // prompts to 19.6, the windows to 52.6; 40 rows of heads of 128 6.0 -> 6.3).
 // Up to heads of 128 two workgroups share a CU; the scores of the next tile are
@@ -38,12 +40,20 @@
 //
 // The probabilities are rounded to the operands' type for the second product
 // and the normaliser adds the rounded ones, so that the weights of a row still
-// sum to one; scores, maximum, sums and output stay f32 until the end.  The
-// running maximum moves only when a tile passes it by more than 2^8 (p stays
-// below 2^8), so most tiles skip the rescaling.  f16's carry a factor 2^7
-// beside, which cancels: they stay below 2^15, and what is lost of a small one
-// in f16's subnormal steps is 2^-32 of the running maximum and not 2^-25, which
-// some thousands of keys behind a heavy one would add up to what f16 shows.
+// sum to one; scores, maximum, sums and output stay f32 until the end.  One part
+// a weight is off by half a step of its type at most, also where outputs leave as
+// f32, and the steps of a row's keys average out: 16-bit outputs are 2.2e-4 (f16,
+// 77 rows of heads of 256) and 1.9e-3 (bf16, the batches above) of their size from
+// those of 64 bits, and would be 2.0e-4 and 1.7e-3 with f32 weights.  A second
+// part, which the one-token kernel has under its bytes, is a third product here:
+// 151 -> 196 us on the ragged batch, 1000 -> 1408 on the long prompt, 103 -> 132
+// on 4000 rows of heads of 256, 48 -> 71 on 6000 of heads of 64.
+//
+// The running maximum moves only when a tile passes it by more than 2^8 (p stays
+// below 2^8), so most tiles skip the rescaling.  f16 weights carry a factor 2^7
+// beside, which cancels: they stay below 2^15, and what is lost of a small one in
+// f16's subnormal steps is 2^-32 of the running maximum and not 2^-25, which some
+// thousands of keys behind a heavy one would add up to what f16 shows.
 //
 // Masked places are not read into the result whatever they hold: scores there
 // become -inf, and where a tile has masked keys its values' infinities and

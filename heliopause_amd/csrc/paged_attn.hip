@@ -2,9 +2,9 @@
 // pages: out_h = sum_j p_j v_j / sum_j p_j with p_j = exp(scale q_h . k_j - m)
 // over the last min(length, window) positions j of the sequence.
 //
-// Every key and value is read once per KV head for all query heads of its
-// group, so 2 (group) flop come on each 16-bit byte pair: the cache's bytes
-// bound it, and the matrix cores, which a group of eight leaves at a few
+// Every key and value is read once per KV head for up to eight query heads of its
+// group (a larger group reads them once for each eight), so 2 (group) flop come on
+// each 16-bit byte pair: the cache's bytes bound it, and the matrix cores, which a group of eight leaves at a few
 // percent, are used because they hand every key to all heads of the group at
 // once and leave the vector unit free.
 //
@@ -49,8 +49,8 @@
 //
 // 48 contexts up to 8192, 32 / 8 heads of 128, bf16: 660 MB in 108 us, 6.1 TB/s,
 // of which the merge launch is 5; two of 131072, f16: 419 MB in 69.5 us; 130
-// windows of 1024 of 8 / 2 heads of 256, e4m3: 121 MB in 33 us, five of the merge
-// and four until the first bytes come; one context of 4096: 8.4 MB in 12 us, two
+// windows of 1024 of 8 / 2 heads of 256, e4m3: 121 MB in 34 us, five of the merge
+// and four until the first bytes come; one context of 4096: 8.4 MB in 12.4 us, two
 // launches' latency.
 #include <type_traits>
 

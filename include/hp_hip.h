@@ -611,7 +611,10 @@ int32_t hp_hip_paged_attention_device(const hp_hip_paged_cache_t *cache, const h
                                       void *stream);
 
 /* Causal attention over whole prompts that lie end to end: row i of a sequence
- * over its rows max(0, i - sliding_window + 1) .. i (0: no window).  Rows
+ * over its rows max(0, i - sliding_window + 1) .. i (0: no window).  It reads no
+ * pages: rows of a sequence that goes on from tokens in its pages would not see
+ * those (they are appended and attended one token a call, by the paged
+ * attention).  Rows
  * d_offsets[s] .. d_offsets[s + 1] - 1 (rising, [sequence_count + 1]) are
  * sequence s; rows behind the last are left as they were.  Queries, keys and
  * values are of one type, which the probabilities are rounded to as well (f16:

@@ -68,7 +68,7 @@ def attend(q, k, v, scale):
         e = k @ q * scale
         p = np.exp(e - e.max())
         p /= p.sum()
-        # a weight of exactly 0 takes nothing of its value, whatever that is
+        # (a weight of exactly 0 makes a NaN of an infinite value)
         return p @ v, p @ np.abs(v), float((np.abs(k) @ np.abs(q)).max() * scale)
 
 
