@@ -4,9 +4,9 @@
 //
 // Every key and value is read once per KV head for up to eight query heads of its
 // group (a larger group reads them once for each eight), so 2 (group) flop come on
-// each 16-bit byte pair: the cache's bytes bound it, and the matrix cores, which a group of eight leaves at a few
-// percent, are used because they hand every key to all heads of the group at
-// once and leave the vector unit free.
+// each 16-bit byte pair: the cache's bytes bound it, and the matrix cores, which a
+// group of eight leaves at a few percent, are used because they hand every key to
+// all heads of the group at once and leave the vector unit free.
 //
 // Products.  A wave takes 32 keys at a time, v_mfma_f32_16x16x32:
 //   scores S^T = K Q^T, keys as the A rows, straight from the cache rows (a

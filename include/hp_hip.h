@@ -622,7 +622,8 @@ int32_t hp_hip_paged_attention_device(const hp_hip_paged_cache_t *cache, const h
  * statistics and sums are f32 (a score past f32's range is an infinity).  What
  * masked places hold does not matter; a value's infinity or NaN that counts
  * leaves no finite number where it reaches (NaN where its weight is 0), and a
- * row whose every score is -inf is NaN.  Token strides of their own let them lie in one projection's rows. */
+ * row whose every score is -inf is NaN.  Token strides of their own let them lie
+ * in one projection's rows. */
 typedef struct hp_hip_packed_attention {
   const void *d_q, *d_k, *d_v; /* [token][heads][head_dim] of type */
   void *d_output;              /* [token][head_count][head_dim] of out_type */
