@@ -500,7 +500,7 @@ def _block_scale(most, case):
         scale = most / MOST["i8"]
     else:  # the least power of two under which 448 reaches it: 448 = 0.875 * 2^9
         m, e = torch.frexp(most)
-        scale = torch.ldexp(torch.ones_like(most), torch.where(m <= 0.875, e - 9, e - 8))
+        scale = torch.ldexp(torch.ones_like(most), torch.where(m <= 0.875, e - 9, e - 8)) * (m > 0)
     return scale.clamp(SCALE_LOW, SCALE_HIGH)
 
 
