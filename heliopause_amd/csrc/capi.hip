@@ -2895,10 +2895,12 @@ int32_t heads_check(int32_t head_count, int32_t head_count_kv) {
   return HP_OK;
 }
 
-int32_t paged_cache_check(const hp_hip_paged_cache_t *c, PagedCache *out) {
+// (blocks: what is kept of the cache's blocks, for the entry points that take it)
+int32_t paged_cache_check(const hp_hip_paged_cache_t *c, PagedCache *out, const hp_hip_cache_blocks_t *blocks = nullptr) {
   if (!c) return fail(HP_ERR_ARG, "null pointer");
-  if (c->type != HP_ELEM_F16 && c->type != HP_ELEM_BF16 && c->type != HP_ELEM_E4M3)
-    return fail(HP_ERR_TYPE, "cache pages are f16, bf16 or e4m3");
+  if (c->type != HP_ELEM_F16 && c->type != HP_ELEM_BF16 && c->type != HP_ELEM_E4M3 && (c->type != HP_ELEM_I8 || !blocks))
+    return fail(HP_ERR_TYPE, "cache pages are f16, bf16 or e4m3 (with block scales i8 too)");
+  const bool scaled = blocks && (blocks->d_key_scales || blocks->d_value_scales);
   int32_t rc = head_dim_check(c->head_dim);
   if (rc != HP_OK) return rc;
   if (c->head_count_kv < 1 || c->head_count_kv > 65535) return fail(HP_ERR_HEADS, "head_count_kv must be 1..65535");
@@ -2908,7 +2910,7 @@ int32_t paged_cache_check(const hp_hip_paged_cache_t *c, PagedCache *out) {
   if (c->sequence_count < 0 || c->sequence_count > 65535) return fail(HP_ERR_SHAPE, "sequence_count must be 0..65535");
   if (c->pages_per_sequence < 1 || (int64_t)c->pages_per_sequence * c->page_size > (1 << 30))
     return fail(HP_ERR_SHAPE, "pages_per_sequence * page_size must be 1..2^30");
-  if (c->type == HP_ELEM_E4M3 && (!cache_scale(c->key_scale) || !cache_scale(c->value_scale)))
+  if (c->type == HP_ELEM_E4M3 && !scaled && (!cache_scale(c->key_scale) || !cache_scale(c->value_scale)))
     return fail(HP_ERR_ARG, "the scales of an e4m3 cache must be 2^-100 .. 2^100");
   int64_t stride = 0;
   rc = row_stride(c->page_stride, (size_t)c->head_count_kv * c->page_size * c->head_dim, elem_bytes(c->type),
@@ -2916,7 +2918,7 @@ int32_t paged_cache_check(const hp_hip_paged_cache_t *c, PagedCache *out) {
   if (rc != HP_OK) return rc;
   if (!c->d_keys || !c->d_values || !c->d_pages || !c->d_lengths) return fail(HP_ERR_ARG, "null pointer");
   if (!aligned16(c->d_keys) || !aligned16(c->d_values)) return fail(HP_ERR_ARG, "pages must start at 16-byte boundaries");
-  const bool e4m3 = c->type == HP_ELEM_E4M3;
+  const bool e4m3 = c->type == HP_ELEM_E4M3 && !scaled;
   *out = PagedCache{c->d_keys,
                     c->d_values,
                     c->d_pages,
@@ -2934,9 +2936,30 @@ int32_t paged_cache_check(const hp_hip_paged_cache_t *c, PagedCache *out) {
   return HP_OK;
 }
 
-int32_t paged_append_check(const hp_hip_paged_cache_t *cache, const hp_hip_paged_append_t *p, PagedAppendArgs *a) {
+// Whose scales and bounds: `scaled` pages need their scales, `bounded` ones their bounds.
+int32_t cache_blocks_check(const hp_hip_paged_cache_t *c, const hp_hip_cache_blocks_t *b, bool bounded, PagedCache *cache,
+                           CacheBlocks *out) {
+  if (!b) return fail(HP_ERR_ARG, "null pointer");
+  int32_t rc = paged_cache_check(c, cache, b);
+  if (rc != HP_OK) return rc;
+  if (b->block_size < 16 || b->block_size > 128 || (b->block_size & (b->block_size - 1)) != 0 || b->block_size > c->page_size)
+    return fail(HP_ERR_SHAPE, "block_size must be a power of two, 16..128, up to page_size");
+  if (b->reserved != 0) return fail(HP_ERR_ARG, "reserved field must be 0");
+  if (!b->d_key_scales != !b->d_value_scales) return fail(HP_ERR_ARG, "keys and values both have scales, or neither");
+  if (c->type == HP_ELEM_I8 && !b->d_key_scales) return fail(HP_ERR_ARG, "i8 pages have block scales");
+  if (elem_bytes(c->type) != 1 && b->d_key_scales) return fail(HP_ERR_TYPE, "16-bit pages have no block scales");
+  if (bounded && !b->d_key_bounds) return fail(HP_ERR_ARG, "null pointer");
+  if (!aligned16(b->d_key_bounds) || reinterpret_cast<uintptr_t>(b->d_key_scales) % 4 != 0 ||
+      reinterpret_cast<uintptr_t>(b->d_value_scales) % 4 != 0)
+    return fail(HP_ERR_ARG, "misaligned pointer");
+  *out = CacheBlocks{b->d_key_scales, b->d_value_scales, b->d_key_bounds, __builtin_ctz((unsigned)b->block_size)};
+  return HP_OK;
+}
+
+int32_t paged_append_check(const hp_hip_paged_cache_t *cache, const hp_hip_paged_append_t *p, PagedAppendArgs *a,
+                           const hp_hip_cache_blocks_t *blocks = nullptr) {
   if (!p) return fail(HP_ERR_ARG, "null pointer");
-  int32_t rc = paged_cache_check(cache, &a->c);
+  int32_t rc = paged_cache_check(cache, &a->c, blocks);
   if (rc != HP_OK) return rc;
   if (!activation_type(p->out_type)) return fail(HP_ERR_TYPE, "outputs are f32, f16 or bf16");
   if (p->d_q || p->head_count != 0) rc = heads_check(p->head_count, a->c.nkv);
@@ -2977,9 +3000,10 @@ int32_t paged_append_check(const hp_hip_paged_cache_t *cache, const hp_hip_paged
   return HP_OK;
 }
 
-int32_t paged_attention_check(const hp_hip_paged_cache_t *cache, const hp_hip_paged_attention_t *p, PagedAttnArgs *a) {
+int32_t paged_attention_check(const hp_hip_paged_cache_t *cache, const hp_hip_paged_attention_t *p, PagedAttnArgs *a,
+                              const hp_hip_cache_blocks_t *blocks = nullptr) {
   if (!p) return fail(HP_ERR_ARG, "null pointer");
-  int32_t rc = paged_cache_check(cache, &a->c);
+  int32_t rc = paged_cache_check(cache, &a->c, blocks);
   if (rc == HP_OK) rc = heads_check(p->head_count, a->c.nkv);
   if (rc != HP_OK) return rc;
   if (!activation_type(p->q_type) || !activation_type(p->out_type))
@@ -3003,6 +3027,105 @@ int32_t paged_attention_check(const hp_hip_paged_cache_t *cache, const hp_hip_pa
   a->scale = p->scale;
   if (paged_attn_most_steps(*a) >> 31)
     return fail(HP_ERR_SHAPE, "sequences * heads * table positions are more than the kernel counts");
+  return HP_OK;
+}
+
+int32_t block_append_check(const hp_hip_paged_cache_t *cache, const hp_hip_cache_blocks_t *blocks,
+                           const hp_hip_paged_append_t *p, PagedAppendArgs *a, CacheBlocks *b) {
+  int32_t rc = cache_blocks_check(cache, blocks, false, &a->c, b);
+  if (rc != HP_OK) return rc;
+  if (elem_bytes(a->c.type) != 1) return fail(HP_ERR_TYPE, "16-bit pages have no block scales");
+  if (!b->key_scales) return fail(HP_ERR_ARG, "null pointer");
+  if ((rc = paged_append_check(cache, p, a, blocks)) != HP_OK) return rc;
+  if (a->c.sequences == 0 || p->token_count == 0) return HP_OK;
+  return block_append_fits(*a, *b) ? HP_OK : fail(HP_ERR_SHAPE, "too many tokens and heads for one launch");
+}
+
+int32_t block_bounds_check(const hp_hip_paged_cache_t *cache, const hp_hip_cache_blocks_t *blocks, const int32_t *d_offsets,
+                           size_t token_count, BlockBoundsArgs *a) {
+  int32_t rc = cache_blocks_check(cache, blocks, true, &a->c, &a->b);
+  if (rc != HP_OK) return rc;
+  if (token_count > (1u << 23)) return fail(HP_ERR_SHAPE, "too many tokens");
+  if (!d_offsets && token_count != (size_t)a->c.sequences)
+    return fail(HP_ERR_SHAPE, "without offsets there is one token a sequence");
+  a->offsets = d_offsets;
+  a->tokens = (int)token_count;
+  return block_bounds_fits(*a) ? HP_OK : fail(HP_ERR_SHAPE, "too many tokens and heads for one launch");
+}
+
+int32_t block_select_check(const hp_hip_paged_cache_t *cache, const hp_hip_cache_blocks_t *blocks,
+                           const hp_hip_block_select_t *p, BlockSelectArgs *a) {
+  if (!p) return fail(HP_ERR_ARG, "null pointer");
+  int32_t rc = cache_blocks_check(cache, blocks, true, &a->c, &a->b);
+  if (rc == HP_OK) rc = heads_check(p->head_count, a->c.nkv);
+  if (rc != HP_OK) return rc;
+  if (!activation_type(p->q_type)) return fail(HP_ERR_TYPE, "queries are f32, f16 or bf16");
+  if (p->budget < 1 || p->budget > (1 << 20)) return fail(HP_ERR_SHAPE, "budget must be 1..2^20");
+  if (p->first_blocks < 0 || p->last_blocks < 0 || (int64_t)p->first_blocks + p->last_blocks > p->budget)
+    return fail(HP_ERR_SHAPE, "first_blocks and last_blocks must not be negative, nor together more than the budget");
+  if (p->reserved != 0) return fail(HP_ERR_ARG, "reserved field must be 0");
+  const size_t row = (size_t)p->head_count * a->c.head_dim;
+  if ((rc = row_stride(p->q_stride, row, elem_bytes(p->q_type), a->c.sequences, &a->q_stride)) != HP_OK) return rc;
+  if (a->c.sequences == 0) return HP_OK;
+  if (!p->d_q || !p->d_selected) return fail(HP_ERR_ARG, "null pointer");
+  if (!aligned16(p->d_q)) return fail(HP_ERR_ARG, "rows must start at 16-byte boundaries");
+  a->q = p->d_q;
+  a->selected = p->d_selected;
+  a->counts = p->d_counts;
+  a->nq = p->head_count;
+  a->q_type = p->q_type;
+  a->budget = p->budget;
+  a->first_blocks = p->first_blocks;
+  a->last_blocks = p->last_blocks;
+  return block_select_fits(*a) ? HP_OK : fail(HP_ERR_SHAPE, "sequences * heads * blocks are more than one launch takes");
+}
+
+int32_t block_attention_check(const hp_hip_paged_cache_t *cache, const hp_hip_cache_blocks_t *blocks,
+                              const hp_hip_paged_attention_t *p, const int32_t *d_selected, const int32_t *d_counts,
+                              int32_t budget, PagedAttnArgs *a) {
+  CacheBlocks b{};
+  int32_t rc = cache_blocks_check(cache, blocks, false, &a->c, &b);
+  if (rc != HP_OK) return rc;
+  if (!d_selected && !b.key_scales)
+    return fail(HP_ERR_ARG, "without scales and selected blocks it is hp_hip_paged_attention_device's");
+  if (!d_selected && (d_counts || budget != 0)) return fail(HP_ERR_ARG, "counts and budget go with selected blocks");
+  if (d_selected && (budget < 1 || budget > (1 << 20))) return fail(HP_ERR_SHAPE, "budget must be 1..2^20");
+  if (d_selected && p && p->sliding_window != 0) return fail(HP_ERR_ARG, "selected blocks have no sliding window");
+  a->key_scales = b.key_scales;
+  a->value_scales = b.value_scales;
+  a->selected = d_selected;
+  a->counts = d_counts;
+  a->block_shift = b.shift;
+  a->budget = budget;
+  return paged_attention_check(cache, p, a, blocks);
+}
+
+int32_t page_plan_check(const hp_hip_page_plan_t *p, PagePlanArgs *a) {
+  if (!p) return fail(HP_ERR_ARG, "null pointer");
+  if (p->sequence_count < 0 || p->sequence_count > 65535) return fail(HP_ERR_SHAPE, "sequence_count must be 0..65535");
+  if (p->page_size < 16 || p->page_size > 4096 || (p->page_size & (p->page_size - 1)) != 0)
+    return fail(HP_ERR_SHAPE, "page_size must be a power of two, 16..4096");
+  if (p->page_count < 1) return fail(HP_ERR_SHAPE, "page_count must be positive");
+  if (p->pages_per_sequence < 1 || (int64_t)p->pages_per_sequence * p->page_size > (1 << 30))
+    return fail(HP_ERR_SHAPE, "pages_per_sequence * page_size must be 1..2^30");
+  if ((int64_t)p->pages_per_sequence * p->sequence_count >> 31) return fail(HP_ERR_SHAPE, "the table is too large");
+  if (p->token_count > (1u << 30)) return fail(HP_ERR_SHAPE, "too many tokens");
+  if (!p->d_new_tokens && p->token_count > (size_t)p->sequence_count)
+    return fail(HP_ERR_SHAPE, "without new token counts there is one token a sequence");
+  if (p->sequence_count == 0) return HP_OK;
+  if (!p->d_pages || !p->d_lengths || !p->d_lengths_out || !p->d_free || !p->d_free_count)
+    return fail(HP_ERR_ARG, "null pointer");
+  for (const void *ptr : {(const void *)p->d_pages, (const void *)p->d_lengths, (const void *)p->d_new_tokens,
+                          (const void *)p->d_keep_from, (const void *)p->d_lengths_out, (const void *)p->d_free,
+                          (const void *)p->d_free_count, (const void *)p->d_offsets, (const void *)p->d_missing,
+                          (const void *)p->d_sequences, (const void *)p->d_positions})
+    if (reinterpret_cast<uintptr_t>(ptr) % 4 != 0) return fail(HP_ERR_ARG, "misaligned pointer");
+  if (reinterpret_cast<uintptr_t>(p->d_slots) % 8 != 0) return fail(HP_ERR_ARG, "misaligned pointer");
+  const bool maps = p->d_sequences || p->d_positions || p->d_slots;
+  *a = PagePlanArgs{p->d_pages,     p->d_lengths, p->d_new_tokens,    p->d_keep_from, p->d_lengths_out,
+                    p->d_free,      p->d_free_count, p->d_offsets,    p->d_missing,   p->d_sequences,
+                    p->d_positions, p->d_slots,   p->sequence_count,  p->pages_per_sequence,
+                    __builtin_ctz((unsigned)p->page_size), p->page_count, maps ? (int)p->token_count : 0};
   return HP_OK;
 }
 
@@ -3121,6 +3244,93 @@ int32_t hp_hip_paged_attention_device(const hp_hip_paged_cache_t *cache, const h
         a.partials = static_cast<float *>(scratch);
         hipEvent_t e = prof_begin(strm);
         HP_HIP_TRY(launch_paged_attn(a, groups, strm));
+        prof_end(HP_KERNEL_ATTENTION, e, strm);
+        s.launches += 2;
+        return HP_OK;
+      });
+}
+
+int32_t hp_hip_page_plan_device(const hp_hip_page_plan_t *plan, void *stream) {
+  PagePlanArgs a{};
+  return serving_call(
+      stream, [&] { return page_plan_check(plan, &a); },
+      [&](State &s, hipStream_t strm) -> int32_t {
+        if (a.sequences == 0) return HP_OK;
+        void *scratch = nullptr;
+        int32_t rc = stream_scratch(strm, kScratchPlan, page_plan_scratch_bytes(a), &scratch);
+        if (rc != HP_OK) return rc;
+        hipEvent_t e = prof_begin(strm);
+        HP_HIP_TRY(launch_page_plan(a, scratch, strm));
+        prof_end(HP_KERNEL_ATTENTION, e, strm);
+        s.launches += 3 + (a.keep_from != nullptr) + (a.rows > 0);
+        return HP_OK;
+      });
+}
+
+int32_t hp_hip_block_append_device(const hp_hip_paged_cache_t *cache, const hp_hip_cache_blocks_t *blocks,
+                                   const hp_hip_paged_append_t *append, void *stream) {
+  PagedAppendArgs a{};
+  CacheBlocks b{};
+  return serving_call(
+      stream, [&] { return block_append_check(cache, blocks, append, &a, &b); },
+      [&](State &s, hipStream_t strm) -> int32_t {
+        if (a.c.sequences == 0 || a.tokens == 0) return HP_OK;
+        hipEvent_t e = prof_begin(strm);
+        HP_HIP_TRY(launch_block_append(a, b, s.num_cus, strm));
+        prof_end(HP_KERNEL_ATTENTION, e, strm);
+        s.launches++;
+        return HP_OK;
+      });
+}
+
+int32_t hp_hip_block_bounds_device(const hp_hip_paged_cache_t *cache, const hp_hip_cache_blocks_t *blocks,
+                                   const int32_t *d_offsets, size_t token_count, void *stream) {
+  BlockBoundsArgs a{};
+  return serving_call(
+      stream, [&] { return block_bounds_check(cache, blocks, d_offsets, token_count, &a); },
+      [&](State &s, hipStream_t strm) -> int32_t {
+        if (a.c.sequences == 0 || a.tokens == 0) return HP_OK;
+        hipEvent_t e = prof_begin(strm);
+        HP_HIP_TRY(launch_block_bounds(a, strm));
+        prof_end(HP_KERNEL_ATTENTION, e, strm);
+        s.launches++;
+        return HP_OK;
+      });
+}
+
+int32_t hp_hip_block_select_device(const hp_hip_paged_cache_t *cache, const hp_hip_cache_blocks_t *blocks,
+                                   const hp_hip_block_select_t *select, void *stream) {
+  BlockSelectArgs a{};
+  return serving_call(
+      stream, [&] { return block_select_check(cache, blocks, select, &a); },
+      [&](State &s, hipStream_t strm) -> int32_t {
+        if (a.c.sequences == 0) return HP_OK;
+        void *scratch = nullptr;
+        int32_t rc = stream_scratch(strm, kScratchSelect, block_select_scratch_bytes(a), &scratch);
+        if (rc != HP_OK) return rc;
+        hipEvent_t e = prof_begin(strm);
+        HP_HIP_TRY(launch_block_select(a, scratch, s.num_cus, strm));
+        prof_end(HP_KERNEL_ATTENTION, e, strm);
+        s.launches += 2;
+        return HP_OK;
+      });
+}
+
+int32_t hp_hip_block_attention_device(const hp_hip_paged_cache_t *cache, const hp_hip_cache_blocks_t *blocks,
+                                      const hp_hip_paged_attention_t *attention, const int32_t *d_selected,
+                                      const int32_t *d_counts, int32_t budget, void *stream) {
+  PagedAttnArgs a{};
+  return serving_call(
+      stream, [&] { return block_attention_check(cache, blocks, attention, d_selected, d_counts, budget, &a); },
+      [&](State &s, hipStream_t strm) -> int32_t {
+        if (a.c.sequences == 0) return HP_OK;
+        const int groups = paged_attn_groups(a, s.num_cus);
+        void *scratch = nullptr;
+        int32_t rc = stream_scratch(strm, kScratchPaged, paged_attn_scratch_bytes(a, groups), &scratch);
+        if (rc != HP_OK) return rc;
+        a.partials = static_cast<float *>(scratch);
+        hipEvent_t e = prof_begin(strm);
+        HP_HIP_TRY(launch_block_attn(a, groups, strm));
         prof_end(HP_KERNEL_ATTENTION, e, strm);
         s.launches += 2;
         return HP_OK;

@@ -61,4 +61,48 @@ HP_PAGES_FN uint32_t share_of(uint32_t total, uint32_t t, uint32_t shares) {
 HP_PAGES_FN int64_t packed_first_block(int offset, int s, int rows) { return (offset > 0 ? offset : 0) / rows + (int64_t)s; }
 HP_PAGES_FN int64_t packed_blocks(int64_t tokens, int64_t sequences, int rows) { return tokens / rows + 1 + sequences; }
 
+// Blocks of `block` positions (a power of two) that new tokens lie in.  Sequence
+// s's slots begin here and end where the next one's begin: rows offset .. end -
+// 1 of it touch at most (rows - 1) / block + 2 blocks, whatever position they
+// begin at, and with no sum over the sequences before it there are that many.
+HP_PAGES_FN int64_t touched_first(int offset, int s, int block) { return (offset > 0 ? offset : 0) / block + 2 * (int64_t)s; }
+HP_PAGES_FN int64_t touched_blocks(int64_t tokens, int64_t sequences, int block) { return tokens / block + 2 * sequences; }
+
+// The new tokens of a sequence of `length` tokens, the last `rows` of them, in
+// the i-th block that they touch: positions first .. end - 1, none where the
+// block is behind the last or outside the table.
+struct NewInBlock {
+  int block, first, end;
+};
+HP_PAGES_FN NewInBlock new_in_block(int length, int64_t rows, int64_t i, int block_shift, int64_t table_keys) {
+  NewInBlock n = {0, 0, 0};
+  const int64_t all = length > 0 ? length : 0, begin = rows >= all ? 0 : rows > 0 ? all - rows : all;
+  const int64_t b = (begin >> block_shift) + i, at = b << block_shift;
+  const int64_t first = at > begin ? at : begin, stop = at + ((int64_t)1 << block_shift), end = stop < all ? stop : all;
+  if (i < 0 || first >= end || at >= table_keys) return n;
+  n.block = (int)b;
+  n.first = (int)first;
+  n.end = (int)end;
+  return n;
+}
+
+// A step's plan for one sequence: table entries 0 .. back - 1 are given back;
+// the new tokens' positions begin at `old`, and of the entries first .. last -
+// 1, whose positions are all new, those that name no page get one.
+struct PlanSpan {
+  int old, back, first, last;
+  int64_t fresh;  // new tokens
+};
+HP_PAGES_FN PlanSpan plan_span(int length, int64_t fresh, int keep_from, int page_shift, int width) {
+  PlanSpan p;
+  p.old = keep_from < 0 || length < 0 ? 0 : length;
+  const int64_t gone = keep_from < 0 ? width : keep_from >> page_shift, page = (int64_t)1 << page_shift;
+  p.back = gone < width ? (int)gone : width;
+  p.fresh = fresh > 0 ? fresh : 0;
+  const int64_t first = ((int64_t)p.old + page - 1) >> page_shift, last = ((int64_t)p.old + p.fresh + page - 1) >> page_shift;
+  p.first = first < width ? (int)first : width;
+  p.last = last < width ? (int)last : width;
+  return p;
+}
+
 }  // namespace hp

@@ -43,7 +43,9 @@ enum ScratchKind {
   kScratchParts = 5,    // block-range sums of a prefill launch that a norm launch adds
   kScratchFused = 6,    // exchange arena and control words of the persistent decode step (zeroed when allocated)
   kScratchPaged = 7,    // row parts of the paged attention
-  kScratchKinds = 8
+  kScratchPlan = 8,     // counts and sums of a page plan
+  kScratchSelect = 9,   // scores of a block selection
+  kScratchKinds = 10
 };
 
 enum ScratchStatus { kScratchOk = 0, kScratchCapturing = 1, kScratchNoMemory = 2, kScratchZeroFailed = 3 };

@@ -13,8 +13,10 @@
 namespace hp {
 
 // HP_ELEM_* of include/hp_hip.h
-constexpr int kElemF32 = 0, kElemF16 = 1, kElemBf16 = 2, kElemE4m3 = 3;
-inline int elem_bytes(int type) { return type == kElemF32 ? 4 : type == kElemE4m3 ? 1 : 2; }
+constexpr int kElemF32 = 0, kElemF16 = 1, kElemBf16 = 2, kElemE4m3 = 3, kElemI8 = 4;
+__host__ __device__ constexpr int elem_bytes(int type) {
+  return type == kElemF32 ? 4 : type == kElemE4m3 || type == kElemI8 ? 1 : 2;
+}
 
 // The pages of a batch: key row (page p, head h, slot i) at element
 // p * page_stride + (h * page_size + i) * head_dim.
@@ -47,15 +49,65 @@ struct PagedAttnArgs {
   int nq, q_type, out_type, window;
   float scale;
   float *partials;  // paged_attn_scratch_bytes
+  // block_attn.hip: a scale of each block and KV head, [page][kv head][block]; the
+  // blocks to attend to, [sequence][kv head][budget], and how many
+  const float *key_scales, *value_scales;
+  const int *selected, *counts;
+  int block_shift, budget;
 };
 // Shares of a launch's keys, which the scratch goes by (the lengths are on the
 // device, so neither depends on them).
 int paged_attn_groups(const PagedAttnArgs &a, int num_cus);
 size_t paged_attn_scratch_bytes(const PagedAttnArgs &a, int groups);
 hipError_t launch_paged_attn(const PagedAttnArgs &a, int groups, hipStream_t s);
+hipError_t launch_block_attn(const PagedAttnArgs &a, int groups, hipStream_t s);
 // Steps of a batch whose sequences fill their tables; the kernel counts them
 // in 32 bits.
 uint64_t paged_attn_most_steps(const PagedAttnArgs &a);
+
+// What is kept of a cache's blocks of 1 << shift positions: for each page, KV head
+// and block of the page a scale of the keys and one of the values, and the bounds
+// of the keys (bf16: head_dim least, head_dim largest elements).
+struct CacheBlocks {
+  float *key_scales, *value_scales;
+  uint16_t *key_bounds;
+  int shift;
+};
+
+// Whether the launch's grid is within what a launch takes.
+bool block_append_fits(const PagedAppendArgs &a, const CacheBlocks &b);
+hipError_t launch_block_append(const PagedAppendArgs &a, const CacheBlocks &b, int num_cus, hipStream_t s);
+
+struct BlockBoundsArgs {
+  PagedCache c;
+  CacheBlocks b;
+  const int *offsets;  // null: row s is sequence s's
+  int tokens;
+};
+bool block_bounds_fits(const BlockBoundsArgs &a);
+hipError_t launch_block_bounds(const BlockBoundsArgs &a, hipStream_t s);
+
+struct BlockSelectArgs {
+  PagedCache c;
+  CacheBlocks b;
+  const void *q;
+  int64_t q_stride;
+  int *selected, *counts;  // [sequence][kv head][budget], [sequence][kv head]
+  int nq, q_type, budget, first_blocks, last_blocks;
+};
+bool block_select_fits(const BlockSelectArgs &a);
+size_t block_select_scratch_bytes(const BlockSelectArgs &a);
+hipError_t launch_block_select(const BlockSelectArgs &a, void *scratch, int num_cus, hipStream_t s);
+
+struct PagePlanArgs {
+  int *pages;  // [sequences][width]
+  const int *lengths, *fresh, *keep_from;  // fresh null: a token for each sequence that has some
+  int *lengths_out, *free, *free_count, *offsets, *missing, *sequence_of, *positions;
+  int64_t *slots;
+  int sequences, width, page_shift, page_count, rows;
+};
+size_t page_plan_scratch_bytes(const PagePlanArgs &a);
+hipError_t launch_page_plan(const PagePlanArgs &a, void *scratch, hipStream_t s);
 
 struct PackedAttnArgs {
   const void *q, *k, *v;

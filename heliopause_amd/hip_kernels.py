@@ -204,16 +204,44 @@ class HipLogitRules(ctypes.Structure):
                [("softcap", ctypes.c_double)]
 
 
+class HipCacheBlocks(ctypes.Structure):
+    """hp_hip_cache_blocks_t: what is kept of a cache's blocks."""
+    _fields_ = [("block_size", ctypes.c_int32), ("reserved", ctypes.c_int32)] + \
+               [(n, ctypes.c_void_p) for n in ("d_key_scales", "d_value_scales", "d_key_bounds")]
+
+
+class HipBlockSelect(ctypes.Structure):
+    """hp_hip_block_select_t: which blocks a token of every sequence attends to."""
+    _fields_ = [("d_q", ctypes.c_void_p), ("q_stride", _sz), ("d_selected", ctypes.c_void_p),
+                ("d_counts", ctypes.c_void_p)] + \
+               [(n, ctypes.c_int32) for n in ("head_count", "q_type", "budget", "first_blocks", "last_blocks", "reserved")]
+
+
+class HipPagePlan(ctypes.Structure):
+    """hp_hip_page_plan_t: a step's page tables and slot maps from the requests' lengths."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("d_pages", "d_lengths", "d_new_tokens", "d_keep_from", "d_lengths_out",
+                                               "d_free", "d_free_count", "d_offsets", "d_missing", "d_sequences",
+                                               "d_positions", "d_slots")] + \
+               [("token_count", _sz)] + \
+               [(n, ctypes.c_int32) for n in ("sequence_count", "pages_per_sequence", "page_size", "page_count")]
+
+
 def _declare_serving(L: ctypes.CDLL) -> None:
     """Entry points of several sequences at once."""
     vp = ctypes.c_void_p
-    cache = ctypes.POINTER(HipPagedCache)
+    cache, blocks = ctypes.POINTER(HipPagedCache), ctypes.POINTER(HipCacheBlocks)
+    L.hp_hip_page_plan_device.argtypes = [ctypes.POINTER(HipPagePlan), vp]
+    L.hp_hip_block_append_device.argtypes = [cache, blocks, ctypes.POINTER(HipPagedAppend), vp]
+    L.hp_hip_block_bounds_device.argtypes = [cache, blocks, vp, _sz, vp]
+    L.hp_hip_block_select_device.argtypes = [cache, blocks, ctypes.POINTER(HipBlockSelect), vp]
+    L.hp_hip_block_attention_device.argtypes = [cache, blocks, ctypes.POINTER(HipPagedAttention), vp, vp, ctypes.c_int32, vp]
     L.hp_hip_paged_append_device.argtypes = [cache, ctypes.POINTER(HipPagedAppend), vp]
     L.hp_hip_paged_attention_device.argtypes = [cache, ctypes.POINTER(HipPagedAttention), vp]
     L.hp_hip_packed_attention_device.argtypes = [ctypes.POINTER(HipPackedAttention), vp]
     L.hp_hip_logit_rules_device.argtypes = [ctypes.POINTER(HipLogitRules), vp]
     for name in ("hp_hip_paged_append_device", "hp_hip_paged_attention_device", "hp_hip_packed_attention_device",
-                 "hp_hip_logit_rules_device"):
+                 "hp_hip_logit_rules_device", "hp_hip_page_plan_device", "hp_hip_block_append_device",
+                 "hp_hip_block_bounds_device", "hp_hip_block_select_device", "hp_hip_block_attention_device"):
         getattr(L, name).restype = ctypes.c_int32
 
 
@@ -769,7 +797,7 @@ def decode_layers_device(layers: Sequence[HipDecodeLayer], d_hidden: int, d_posi
 
 # ---- several sequences at once (device pointers; asynchronous on ``stream``; no counterpart in the reference) ----------
 
-HP_ELEM_F32, HP_ELEM_F16, HP_ELEM_BF16, HP_ELEM_E4M3 = 0, 1, 2, 3
+HP_ELEM_F32, HP_ELEM_F16, HP_ELEM_BF16, HP_ELEM_E4M3, HP_ELEM_I8 = 0, 1, 2, 3, 4
 
 
 def paged_cache(d_keys: int, d_values: int, type: int, *, page_count: int, page_size: int, head_count_kv: int,
@@ -827,3 +855,65 @@ def logit_rules_device(rows: int, n: int, d_logits: int, d_output: int, *, d_his
                       d_presence, d_bias_ids, d_bias_values, d_bias_counts, d_allowed, rows, n, logits_stride,
                       output_stride, history_stride, bias_stride, allowed_stride, softcap)
     assertHipOk(lib().hp_hip_logit_rules_device(ctypes.byref(p), stream or None), "logit_rules")
+
+
+# ---- long contexts (device pointers; asynchronous on ``stream``; no counterpart in the reference) -----------------------
+
+def page_plan_device(sequence_count: int, pages_per_sequence: int, page_size: int, page_count: int, d_pages: int,
+                     d_lengths: int, d_lengths_out: int, d_free: int, d_free_count: int, *, d_new_tokens: int = 0,
+                     d_keep_from: int = 0, d_offsets: int = 0, d_missing: int = 0, token_count: int = 0,
+                     d_sequences: int = 0, d_positions: int = 0, d_slots: int = 0, stream: int = 0) -> None:
+    """A step's page tables, lengths, row offsets and slot maps from the requests' lengths (d_new_tokens 0: one token
+    for each sequence that has tokens): pages that are no longer needed go back on the stack of free ones, new ones come
+    off it."""
+    p = HipPagePlan(d_pages, d_lengths, d_new_tokens, d_keep_from, d_lengths_out, d_free, d_free_count, d_offsets,
+                    d_missing, d_sequences, d_positions, d_slots, token_count, sequence_count, pages_per_sequence,
+                    page_size, page_count)
+    assertHipOk(lib().hp_hip_page_plan_device(ctypes.byref(p), stream or None), "page_plan")
+
+
+def cache_blocks(block_size: int, *, d_key_scales: int = 0, d_value_scales: int = 0, d_key_bounds: int = 0) -> HipCacheBlocks:
+    """hp_hip_cache_blocks_t: scales [page][kv head][block] and key bounds [page][kv head][block][2][head_dim] of a
+    paged cache's blocks."""
+    return HipCacheBlocks(block_size, 0, d_key_scales, d_value_scales, d_key_bounds)
+
+
+def block_append_device(cache: HipPagedCache, blocks: HipCacheBlocks, token_count: int, head_count: int, d_q: int,
+                        d_k: int, d_v: int, d_q_out: int, out_type: int, *, d_offsets: int = 0, d_q_norm: int = 0,
+                        d_k_norm: int = 0, norm_values: bool = False, epsilon: float = 1e-6, rope_dims: int = 0,
+                        rope_freq_base: float = 10000.0, d_rope_freq_factors: int = 0, q_stride: int = 0,
+                        k_stride: int = 0, v_stride: int = 0, d_k_out: int = 0, d_v_out: int = 0,
+                        stream: int = 0) -> None:
+    """paged_append_device into pages of 8 bits with a scale for each block and KV head."""
+    p = HipPagedAppend(d_q, d_k, d_v, q_stride, k_stride, v_stride, d_offsets, d_q_norm, d_k_norm,
+                       d_rope_freq_factors, d_q_out, d_k_out, d_v_out, token_count, head_count, out_type,
+                       1 if norm_values else 0, rope_dims, rope_freq_base, epsilon)
+    assertHipOk(lib().hp_hip_block_append_device(ctypes.byref(cache), ctypes.byref(blocks), ctypes.byref(p),
+                                                 stream or None), "block_append")
+
+
+def block_bounds_device(cache: HipPagedCache, blocks: HipCacheBlocks, token_count: int, *, d_offsets: int = 0,
+                        stream: int = 0) -> None:
+    """The key bounds of the blocks that the new tokens of an append lie in, formed anew."""
+    assertHipOk(lib().hp_hip_block_bounds_device(ctypes.byref(cache), ctypes.byref(blocks), d_offsets or None, token_count,
+                                                 stream or None), "block_bounds")
+
+
+def block_select_device(cache: HipPagedCache, blocks: HipCacheBlocks, head_count: int, d_q: int, q_type: int, budget: int,
+                        d_selected: int, d_counts: int = 0, *, first_blocks: int = 0, last_blocks: int = 1,
+                        q_stride: int = 0, stream: int = 0) -> None:
+    """The blocks, up to ``budget`` of each sequence and KV head, that the last token's queries could score highest in."""
+    p = HipBlockSelect(d_q, q_stride, d_selected, d_counts, head_count, q_type, budget, first_blocks, last_blocks, 0)
+    assertHipOk(lib().hp_hip_block_select_device(ctypes.byref(cache), ctypes.byref(blocks), ctypes.byref(p),
+                                                 stream or None), "block_select")
+
+
+def block_attention_device(cache: HipPagedCache, blocks: HipCacheBlocks, head_count: int, d_q: int, q_type: int,
+                           d_output: int, out_type: int, *, scale: float = 1.0, sliding_window: int = 0,
+                           d_selected: int = 0, d_counts: int = 0, budget: int = 0, q_stride: int = 0,
+                           output_stride: int = 0, stream: int = 0) -> None:
+    """paged_attention_device over pages whose blocks have scales, over the selected blocks only, or both."""
+    p = HipPagedAttention(d_q, d_output, q_stride, output_stride, head_count, q_type, out_type, sliding_window, scale, 0)
+    assertHipOk(lib().hp_hip_block_attention_device(ctypes.byref(cache), ctypes.byref(blocks), ctypes.byref(p),
+                                                    d_selected or None, d_counts or None, budget, stream or None),
+                "block_attention")

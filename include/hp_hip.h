@@ -528,6 +528,7 @@ int32_t hp_hip_set_fused_trace(uint64_t *d_stamps, size_t len);
 #define HP_ELEM_F16 1
 #define HP_ELEM_BF16 2
 #define HP_ELEM_E4M3 3 /* OCP fp8, cache pages only: value = stored * scale */
+#define HP_ELEM_I8 4   /* -127 .. 127, cache pages whose blocks have scales (hp_hip_cache_blocks_t) only */
 
 /* A pool of pages and what a batch's sequences hold in it.  Position i of
  * sequence s is slot i % page_size of page d_pages[s * pages_per_sequence + i /
@@ -673,6 +674,119 @@ typedef struct hp_hip_logit_rules {
   double softcap;                               /* finite; 0: none */
 } hp_hip_logit_rules_t;
 int32_t hp_hip_logit_rules_device(const hp_hip_logit_rules_t *rules, void *stream);
+
+/* ---- Long contexts ---------------------------------------------------------
+ * The rules of "Several sequences at once" hold here too.  Pages are dealt and
+ * taken back on the device; pages of 8 bits have a scale for each block of
+ * positions and KV head; a token's attention may keep to the blocks that a bound
+ * of their scores selects. */
+
+/* A step's page tables, lengths, row offsets and slot maps from the requests'
+ * lengths.  The free pages are a stack: the next to be dealt is
+ * d_free[*d_free_count - 1].  In this order:
+ *   - a sequence with d_keep_from[s] < 0 is over: every page that its row of the
+ *     table names goes back and its length counts as 0; with k >= 0 the pages
+ *     wholly before position k go back.  Their entries become -1;
+ *   - the new tokens' pages, those all of whose positions are new and whose entry
+ *     names no page, are dealt, in order of sequence and position.  When there
+ *     is none left they stay -1: rows appended there are dropped and their
+ *     positions left out of the attention; d_missing[s] counts them;
+ *   - d_lengths_out[s] (may be d_lengths) is the length with the new tokens,
+ *     d_offsets the sums of the new tokens (the packed rows of
+ *     hp_hip_paged_append_device), and row t of the maps is the t-th new token:
+ *     its sequence, position, and slot page * page_size + position % page_size.
+ *     Rows behind the last are -1, a slot without a page too.
+ * A step that lacks pages can be taken again once some are free: with the
+ * lengths as they were, pages dealt before are found in the table.  A page that
+ * two rows of the table name must not go back through both; the stack holds
+ * d_free's page_count entries at most, what goes back beyond is lost.  Up to four
+ * launches, over scratch of the stream's. */
+typedef struct hp_hip_page_plan {
+  int32_t *d_pages;              /* [sequence_count][pages_per_sequence] */
+  const int32_t *d_lengths;      /* [sequence_count]; below 1: empty */
+  const int32_t *d_new_tokens;   /* [sequence_count]; NULL: one for each sequence that has tokens, as row s */
+  const int32_t *d_keep_from;    /* [sequence_count]; NULL: no page goes back */
+  int32_t *d_lengths_out;        /* [sequence_count] */
+  int32_t *d_free, *d_free_count; /* [page_count], [1] */
+  int32_t *d_offsets;            /* [sequence_count + 1], or NULL */
+  int32_t *d_missing;            /* [sequence_count], or NULL */
+  int32_t *d_sequences, *d_positions; /* [token_count], or NULL */
+  int64_t *d_slots;              /* [token_count], or NULL */
+  size_t token_count;            /* rows of the maps, up to 2^30; 0: none.  Without d_new_tokens up to sequence_count */
+  int32_t sequence_count;        /* up to 65535; 0: the call does nothing */
+  int32_t pages_per_sequence;    /* pages_per_sequence * page_size <= 2^30, * sequence_count < 2^31 */
+  int32_t page_size;             /* a power of two, 16 .. 4096 */
+  int32_t page_count;
+} hp_hip_page_plan_t;
+int32_t hp_hip_page_plan_device(const hp_hip_page_plan_t *plan, void *stream);
+
+/* What is kept of a cache's blocks: block_size consecutive positions of a page.
+ * Entry (page * head_count_kv + head) * (page_size / block_size) + block of each
+ * array is of that page, KV head and block of the page. */
+typedef struct hp_hip_cache_blocks {
+  int32_t block_size; /* a power of two, 16 .. 128, up to page_size */
+  int32_t reserved;   /* 0 */
+  float *d_key_scales, *d_value_scales; /* value = stored * scale; 0, or 2^-100 .. 2^100.  HP_ELEM_I8 pages have them,
+                                           HP_ELEM_E4M3 pages may (key_scale and value_scale are not used then), others
+                                           have NULL */
+  uint16_t *d_key_bounds; /* bf16 [entry][2][head_dim]: the least and the largest elements of the block's keys; NULL
+                             where none are used.  At a 16-byte boundary */
+} hp_hip_cache_blocks_t;
+
+/* hp_hip_paged_append_device into pages whose blocks have scales.  With A the
+ * largest magnitude among the call's rows of a block and KV head (keys and values
+ * each for themselves): a block that begins with this call has the scale A / 127
+ * (i8) or the least power of two with A <= 448 scale (e4m3).  One begun before
+ * keeps its scale as long as A is within it; otherwise the scale becomes that of
+ * A, i8's at least 1.25 times what it was, and what the block holds is rounded to
+ * the new one.  Scales stay within 2^-100 .. 2^100, what is past them saturates.
+ * An infinity or NaN makes the block's scale NaN until the block begins anew.
+ * d_k_out and d_v_out have the rows before they are rounded to 8 bits.  The
+ * angles' sines and cosines are f32's, of turns reduced in 64 bits. */
+int32_t hp_hip_block_append_device(const hp_hip_paged_cache_t *cache, const hp_hip_cache_blocks_t *blocks,
+                                   const hp_hip_paged_append_t *append, void *stream);
+
+/* Forms d_key_bounds anew for every block that holds one of the new tokens, over
+ * all its keys before the sequence's end: the tokens of a hp_hip_paged_append_device
+ * or hp_hip_block_append_device call, with its d_offsets and token_count, once it
+ * has been queued.  Bounds are rounded outward; a NaN among a block's keys counts
+ * as the smallest and the largest finite number. */
+int32_t hp_hip_block_bounds_device(const hp_hip_paged_cache_t *cache, const hp_hip_cache_blocks_t *blocks,
+                                   const int32_t *d_offsets, size_t token_count, void *stream);
+
+/* The blocks that one token of every sequence, the last, attends to: of the
+ * sequence's blocks those with the largest scores, up to `budget`, in rising
+ * order.  A block's score is the largest over the query heads of a KV head of
+ * sum_d max(q_d least_d, q_d largest_d), which no key within the bounds exceeds;
+ * it is formed in 64 bits, and of equal scores the block that comes first is
+ * taken.  The first_blocks first and last_blocks last blocks are always taken,
+ * and count.  Blocks on absent pages are not.  An infinite query element counts
+ * as the largest finite number, a NaN as 0.  Two launches, over scratch of the
+ * stream's. */
+typedef struct hp_hip_block_select {
+  const void *d_q;      /* [sequence_count][head_count][head_dim] of q_type */
+  size_t q_stride;      /* from sequence to sequence */
+  int32_t *d_selected;  /* [sequence_count][head_count_kv][budget], -1 behind the last */
+  int32_t *d_counts;    /* [sequence_count][head_count_kv], or NULL */
+  int32_t head_count;
+  int32_t q_type;       /* HP_ELEM_F32, HP_ELEM_F16 or HP_ELEM_BF16 */
+  int32_t budget;       /* 1 .. 2^20 */
+  int32_t first_blocks, last_blocks; /* together up to budget */
+  int32_t reserved;     /* 0 */
+} hp_hip_block_select_t;
+int32_t hp_hip_block_select_device(const hp_hip_paged_cache_t *cache, const hp_hip_cache_blocks_t *blocks,
+                                   const hp_hip_block_select_t *select, void *stream);
+
+/* hp_hip_paged_attention_device over pages whose blocks have scales, over the
+ * selected blocks only, or both.  d_selected (NULL: whole sequences, which then
+ * have block scales) has `budget` block numbers of each sequence and KV head, of
+ * which the first d_counts count (NULL: all; others than the sequence's blocks
+ * are left out); a block named twice counts twice.  sliding_window is 0 with it.
+ * Bounds are not used here.  Products are exact to some 2^-22 of the largest
+ * (bf16 pages 2^-16); a NaN scale makes NaN what its block has weight in. */
+int32_t hp_hip_block_attention_device(const hp_hip_paged_cache_t *cache, const hp_hip_cache_blocks_t *blocks,
+                                      const hp_hip_paged_attention_t *attention, const int32_t *d_selected,
+                                      const int32_t *d_counts, int32_t budget, void *stream);
 
 #ifdef __cplusplus
 }
