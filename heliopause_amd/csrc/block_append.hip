@@ -2,7 +2,7 @@
 // a scale for each KV head: head norms and position rotation as
 // paged_append.hip has them, then per block and head with A the largest
 // magnitude among the call's rows in it
-//   i8:   s' = A / 127          e4m3: s' = the least power of two with A <= 448 s'
+//   i8:   s' = A (1 / 127)      e4m3: s' = the least power of two with A <= 448 s'
 // held within 2^-100 .. 2^100, and x is stored as round(x / s').  A block that
 // was begun before the call keeps its scale s while A <= M s (M = 127 or 448);
 // otherwise the scale grows to s' (i8: at least 1.25 s, so that growing again
@@ -55,7 +55,7 @@ template <int CT>
 __device__ __forceinline__ float fresh_scale(float most) {
   float s;
   if (CT == kElemI8) {
-    s = most / 127.0f;
+    s = most * (1.0f / 127.0f);
   } else {
     int e;
     const float m = frexpf(most, &e);

@@ -735,7 +735,7 @@ typedef struct hp_hip_cache_blocks {
 
 /* hp_hip_paged_append_device into pages whose blocks have scales.  With A the
  * largest magnitude among the call's rows of a block and KV head (keys and values
- * each for themselves): a block that begins with this call has the scale A / 127
+ * each for themselves): a block that begins with this call has the scale A * (1 / 127)
  * (i8) or the least power of two with A <= 448 scale (e4m3).  One begun before
  * keeps its scale as long as A is within it; otherwise the scale becomes that of
  * A, i8's at least 1.25 times what it was, and what the block holds is rounded to
