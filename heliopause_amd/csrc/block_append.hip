@@ -201,19 +201,7 @@ __global__ __launch_bounds__(NT) void block_append_kernel(const PagedAppendArgs 
   int seq = slot, row_end;
   NewInBlock n;
   if (a.offsets) {
-    const int S = a.c.sequences;
-    int lo = 0, left = S;  // the largest sequence whose first slot is not behind this one
-    const int lane = tid & 63;
-    while (left > 64) {
-      const int step = (left + 63) >> 6, i = lo + min(lane * step, left - 1);
-      const bool le = lane * step < left && touched_first(a.offsets[i], i, 1 << b.shift) <= slot;
-      const int c = max(__popcll(__ballot(le)), 1) - 1;
-      lo += c * step;
-      left = min(step, left - c * step);
-    }
-    const int i = lo + min(lane, left - 1);
-    const bool le = lane < left && touched_first(a.offsets[i], i, 1 << b.shift) <= slot;
-    seq = lo + max(__popcll(__ballot(le)), 1) - 1;
+    seq = touched_sequence(a.offsets, a.c.sequences, slot, 1 << b.shift);
     const int begin = a.offsets[seq];
     row_end = a.offsets[seq + 1];
     n = new_in_block(a.c.lengths[seq], (int64_t)row_end - begin, slot - touched_first(begin, seq, 1 << b.shift), b.shift,

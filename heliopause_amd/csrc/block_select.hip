@@ -13,10 +13,17 @@
 // its negative part, so that a term is two fused products of which one adds 0.
 // A score becomes a 64-bit key that sorts the same way.
 //
-// Pick.  One workgroup per (sequence, KV head): the digits of the budget-th
-// largest key, 8 bits at a time below the bits that all keys share, by counting
-// in LDS; then the blocks above it, and of those equal to it the first ones, in
-// their order.
+// Pick.  One workgroup per (sequence, KV head), the keys in its registers where
+// they fit: the digits of the budget-th largest key, 8 bits at a time below the
+// bits that all keys share, by counting in LDS, until 64 or fewer are left, which
+// a wave ranks; then the blocks above it, and of those equal to it the first
+// ones, in their order.
+//
+// Not kept: scores by the matrix cores in parts of bf16 (10.5 us for 12.0 on 24
+// contexts, 12.8 for 14.4 on two of 262144), with the blocks that their error
+// leaves open scored in 64 bits by the pick, which then took 12.4 and 18.9 us for
+// 7.2 and 10.8.
+#include "hp_mfma.h"
 #include "hp_serving.h"
 #include "hp_wave.h"
 
@@ -38,67 +45,90 @@ __device__ __forceinline__ uint16_t outward(float x) {
   return (uint16_t)((bits + (away ? 0xffffu : 0u)) >> 16);
 }
 
-// One wave per (touched block, KV head): 16 bytes of a row a lane.
-constexpr int kBoundWaves = 4;
-
+// 16 bytes of a row a lane.  The least and largest are f16's in pairs, two rows
+// an instruction (v_pk_minimum3_f16), which keep a NaN: f16 keys as they are, e4m3
+// as the halves that they are, i8 as the halves 1152 + q, whose order is theirs;
+// bf16 as f32.  Few blocks: a workgroup has a (touched block, KV head), all of its
+// loads on their way at once, and the waves' parts are joined in LDS.  Many: a wave
+// has it.  (One block of 64 rows, 2 heads of 256, f16: 3.5 us, with a wave each 7.2;
+// 100000 rows in blocks of 32, e4m3: 57 MB in 12.8 us, with a workgroup each 36.)
 template <int CT>
-__device__ __forceinline__ void elements(const uint4 &w, float (&v)[16 / elem_bytes(CT)]) {
-  const uint32_t d[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-  for (int i = 0; i < 16 / elem_bytes(CT); i++) {
-    if (CT == kElemF16)
-      v[i] = (float)__builtin_bit_cast(_Float16, (uint16_t)(d[i / 2] >> (16 * (i & 1))));
-    else if (CT == kElemBf16)
-      v[i] = bf16_value(d[i / 2] >> (16 * (i & 1)) & 0xffffu);
-    else if (CT == kElemI8)
-      v[i] = (float)(int8_t)(d[i / 4] >> (8 * (i & 3)));
-    else
-      v[i] = (i & 3) == 0   ? __builtin_amdgcn_cvt_f32_fp8(d[i / 4], 0)
-             : (i & 3) == 1 ? __builtin_amdgcn_cvt_f32_fp8(d[i / 4], 1)
-             : (i & 3) == 2 ? __builtin_amdgcn_cvt_f32_fp8(d[i / 4], 2)
-                            : __builtin_amdgcn_cvt_f32_fp8(d[i / 4], 3);
+struct Extremes {
+  using V = half2v;
+  static constexpr int kPer = 16 / elem_bytes(CT), kN = kPer / 2;  // elements of a lane, registers
+  static __device__ __forceinline__ V most(bool up) {
+    const _Float16 v = (_Float16)(up ? -kInf : kInf);
+    return V{v, v};
   }
-}
+  static __device__ __forceinline__ void of(const uint4 &w, V (&v)[kN]) {
+    const uint32_t d[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      if (CT == kElemF16) {
+        v[i] = as_h2(d[i]);
+      } else if (CT == kElemI8) {
+        v[2 * i % kN] = magic_pair<kSel01>(d[i] ^ 0x80808080u);
+        v[(2 * i + 1) % kN] = magic_pair<kSel23>(d[i] ^ 0x80808080u);
+      } else {
+        v[2 * i % kN] = __builtin_bit_cast(half2v, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(d[i], 1.0f, false));
+        v[(2 * i + 1) % kN] = __builtin_bit_cast(half2v, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(d[i], 1.0f, true));
+      }
+    }
+  }
+  static __device__ __forceinline__ float value(const V (&v)[kN], int j) {
+    return (float)v[j / 2][j & 1] - (CT == kElemI8 ? 1152.0f : 0.0f);
+  }
+};
+template <>
+struct Extremes<kElemBf16> {
+  using V = float;
+  static constexpr int kPer = 8, kN = 8;
+  static __device__ __forceinline__ V most(bool up) { return up ? -kInf : kInf; }
+  static __device__ __forceinline__ void of(const uint4 &w, V (&v)[kN]) {
+    const uint32_t d[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      v[2 * i] = bf16_value(d[i] & 0xffffu);
+      v[2 * i + 1] = __builtin_bit_cast(float, d[i] & 0xffff0000u);
+    }
+  }
+  static __device__ __forceinline__ float value(const V (&v)[kN], int j) { return v[j]; }
+};
 
-template <int D, int CT>
-__global__ __launch_bounds__(64 * kBoundWaves) void block_bounds_kernel(const BlockBoundsArgs a, int units) {
-  constexpr int kE = elem_bytes(CT), kPer = 16 / kE, kLanes = D / kPer, kRows = 64 / kLanes, kDeep = 8;
-  const int lane = threadIdx.x & 63, unit = blockIdx.x * kBoundWaves + (threadIdx.x >> 6);
+template <int D, int CT, int WAVES>
+__global__ __launch_bounds__(256) void block_bounds_kernel(const BlockBoundsArgs a, int units) {
+  using E = Extremes<CT>;
+  using V = typename E::V;
+  constexpr int kE = elem_bytes(CT), kPer = E::kPer, kN = E::kN, kLanes = D / kPer, kRows = 64 / kLanes * WAVES;
+  constexpr int kDeep = WAVES == 1 ? 8 : 4;  // loads of a lane at a time
+  __shared__ V sh[WAVES == 1 ? 1 : 2][WAVES][WAVES == 1 ? 1 : kLanes][kN];
+  const int tid = threadIdx.x % (64 * WAVES), lane = threadIdx.x & 63, wave = WAVES == 1 ? 0 : threadIdx.x >> 6;
+  const int unit = WAVES == 1 ? blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
   if (unit >= units) return;
   const int h = unit % a.c.nkv, slot = unit / a.c.nkv;
   int seq = slot;
   NewInBlock n;
   const int64_t table_keys = (int64_t)a.c.width << a.c.page_shift;
   if (a.offsets) {
-    int lo = 0, left = a.c.sequences;  // the largest sequence whose first slot is not behind this one
-    while (left > 64) {
-      const int step = (left + 63) >> 6, i = lo + min(lane * step, left - 1);
-      const bool le = lane * step < left && touched_first(a.offsets[i], i, 1 << a.b.shift) <= slot;
-      const int c = max(__popcll(__ballot(le)), 1) - 1;
-      lo += c * step;
-      left = min(step, left - c * step);
-    }
-    const int i = lo + min(lane, left - 1);
-    const bool le = lane < left && touched_first(a.offsets[i], i, 1 << a.b.shift) <= slot;
-    seq = lo + max(__popcll(__ballot(le)), 1) - 1;
+    seq = touched_sequence(a.offsets, a.c.sequences, slot, 1 << a.b.shift);
     const int begin = a.offsets[seq];
     n = new_in_block(a.c.lengths[seq], (int64_t)a.offsets[seq + 1] - begin,
                      slot - touched_first(begin, seq, 1 << a.b.shift), a.b.shift, table_keys);
   } else {
     n = new_in_block(a.c.lengths[seq], 1, 0, a.b.shift, table_keys);
   }
-  if (n.end <= n.first) return;
+  if (n.end <= n.first) return;  // (the same for the unit's waves)
   const int page = page_or_none(a.c.pages[(int64_t)seq * a.c.width + (n.first >> a.c.page_shift)], a.c.page_count);
   if (page < 0) return;
   const int in_page = n.block & ((1 << (a.c.page_shift - a.b.shift)) - 1), live = n.end - (n.block << a.b.shift);
   const int64_t block_at = (((int64_t)page * a.c.nkv + h) << (a.c.page_shift - a.b.shift)) + in_page;
   const uint8_t *rows = static_cast<const uint8_t *>(a.c.keys) +
                         (page * a.c.page_stride + (((int64_t)h << a.c.page_shift) + ((int64_t)in_page << a.b.shift)) * D) * kE;
-  const int col = lane % kLanes, sub = lane / kLanes;
-  float lo[kPer], hi[kPer];
+  const float scale = a.b.key_scales ? a.b.key_scales[block_at] : CT == kElemE4m3 ? a.c.key_scale : 1.0f;
+  const int col = lane % kLanes, sub = tid / kLanes;
+  V lo[kN], hi[kN];
 #pragma unroll
-  for (int i = 0; i < kPer; i++) lo[i] = kInf, hi[i] = -kInf;
-  bool odd = false;  // a NaN is among the lane's elements
+  for (int i = 0; i < kN; i++) lo[i] = E::most(false), hi[i] = E::most(true);
   for (int r0 = 0; r0 < live; r0 += kRows * kDeep) {
     uint4 w[kDeep];
 #pragma unroll
@@ -107,76 +137,122 @@ __global__ __launch_bounds__(64 * kBoundWaves) void block_bounds_kernel(const Bl
       w[i] = *reinterpret_cast<const uint4 *>(rows + ((int64_t)r * D + col * kPer) * kE);
     }
 #pragma unroll
-    for (int i = 0; i < kDeep; i++) {
-      float v[kPer];
-      elements<CT>(w[i], v);
+    for (int i = 0; i < kDeep; i += 2) {
+      V u[kN], v[kN];
+      E::of(w[i], u);
+      E::of(w[i + 1], v);
 #pragma unroll
-      for (int j = 0; j < kPer; j++) {
-        lo[j] = fminf(lo[j], v[j]);
-        hi[j] = fmaxf(hi[j], v[j]);
-        odd = odd || v[j] != v[j];
+      for (int j = 0; j < kN; j++) {
+        lo[j] = __builtin_elementwise_minimum(__builtin_elementwise_minimum(lo[j], u[j]), v[j]);
+        hi[j] = __builtin_elementwise_maximum(__builtin_elementwise_maximum(hi[j], u[j]), v[j]);
       }
     }
   }
-  if (__any(odd)) {  // rare: which elements
-#pragma unroll
-    for (int j = 0; j < kPer; j++) {
-      bool is = false;
-      for (int r = sub; r < live; r += kRows) {
-        float v[kPer];
-        elements<CT>(*reinterpret_cast<const uint4 *>(rows + ((int64_t)r * D + col * kPer) * kE), v);
-        is = is || v[j] != v[j];
-      }
-      lo[j] = is ? -kInf : lo[j];
-      hi[j] = is ? kInf : hi[j];
-    }
-  }
-  const float scale = a.b.key_scales ? a.b.key_scales[block_at] : CT == kElemE4m3 ? a.c.key_scale : 1.0f;
 #pragma unroll
   for (int m = kLanes; m < 64; m *= 2) {
 #pragma unroll
-    for (int j = 0; j < kPer; j++) {
-      lo[j] = fminf(lo[j], __shfl_xor(lo[j], m));
-      hi[j] = fmaxf(hi[j], __shfl_xor(hi[j], m));
+    for (int j = 0; j < kN; j++) {
+      const int x = __builtin_bit_cast(int, lo[j]), y = __builtin_bit_cast(int, hi[j]);
+      lo[j] = __builtin_elementwise_minimum(lo[j], __builtin_bit_cast(V, __shfl_xor(x, m)));
+      hi[j] = __builtin_elementwise_maximum(hi[j], __builtin_bit_cast(V, __shfl_xor(y, m)));
     }
   }
-  if (sub != 0) return;
+  if (WAVES > 1) {
+    if (lane < kLanes) {
+#pragma unroll
+      for (int j = 0; j < kN; j++) {
+        sh[0][wave][lane % kLanes][j] = lo[j];
+        sh[WAVES == 1 ? 0 : 1][wave][lane % kLanes][j] = hi[j];
+      }
+    }
+    __syncthreads();
+    if (wave != 0) return;
+#pragma unroll
+    for (int w = 1; w < WAVES; w++)
+#pragma unroll
+      for (int j = 0; j < kN; j++) {
+        lo[j] = __builtin_elementwise_minimum(lo[j], sh[0][w][col][j]);
+        hi[j] = __builtin_elementwise_maximum(hi[j], sh[WAVES == 1 ? 0 : 1][w][col][j]);
+      }
+  }
+  if (lane >= kLanes) return;
   uint16_t *out = a.b.key_bounds + block_at * 2 * D + col * kPer;
 #pragma unroll
   for (int j = 0; j < kPer; j += 8) {
     uint32_t l[4], u[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-      l[i] = outward<false>(lo[j + 2 * i] * scale) | (uint32_t)outward<false>(lo[j + 2 * i + 1] * scale) << 16;
-      u[i] = outward<true>(hi[j + 2 * i] * scale) | (uint32_t)outward<true>(hi[j + 2 * i + 1] * scale) << 16;
+      l[i] = outward<false>(E::value(lo, j + 2 * i) * scale) | (uint32_t)outward<false>(E::value(lo, j + 2 * i + 1) * scale) << 16;
+      u[i] = outward<true>(E::value(hi, j + 2 * i) * scale) | (uint32_t)outward<true>(E::value(hi, j + 2 * i + 1) * scale) << 16;
     }
     *reinterpret_cast<uint4 *>(out + j) = make_uint4(l[0], l[1], l[2], l[3]);
     *reinterpret_cast<uint4 *>(out + D + j) = make_uint4(u[0], u[1], u[2], u[3]);
   }
 }
 
+template <int D, int CT>
+hipError_t launch_bounds(const BlockBoundsArgs &a, int slots, int num_cus, hipStream_t s) {
+  const int units = slots * a.c.nkv;
+  if (units <= 4 * num_cus)
+    hipLaunchKernelGGL((block_bounds_kernel<D, CT, 4>), dim3(units), dim3(256), 0, s, a, units);
+  else
+    hipLaunchKernelGGL((block_bounds_kernel<D, CT, 1>), dim3((units + 3) / 4), dim3(256), 0, s, a, units);
+  return hipGetLastError();
+}
+
 template <int D>
-hipError_t launch_bounds_type(const BlockBoundsArgs &a, int units, hipStream_t s) {
-  const dim3 grid((units + kBoundWaves - 1) / kBoundWaves), threads(64 * kBoundWaves);
+hipError_t launch_bounds_type(const BlockBoundsArgs &a, int slots, int num_cus, hipStream_t s) {
   switch (a.c.type) {
-    case kElemF16: hipLaunchKernelGGL((block_bounds_kernel<D, kElemF16>), grid, threads, 0, s, a, units); break;
-    case kElemBf16: hipLaunchKernelGGL((block_bounds_kernel<D, kElemBf16>), grid, threads, 0, s, a, units); break;
-    case kElemE4m3: hipLaunchKernelGGL((block_bounds_kernel<D, kElemE4m3>), grid, threads, 0, s, a, units); break;
-    case kElemI8: hipLaunchKernelGGL((block_bounds_kernel<D, kElemI8>), grid, threads, 0, s, a, units); break;
+    case kElemF16: return launch_bounds<D, kElemF16>(a, slots, num_cus, s);
+    case kElemBf16: return launch_bounds<D, kElemBf16>(a, slots, num_cus, s);
+    case kElemE4m3: return launch_bounds<D, kElemE4m3>(a, slots, num_cus, s);
+    case kElemI8: return launch_bounds<D, kElemI8>(a, slots, num_cus, s);
     default: return hipErrorInvalidValue;
   }
-  return hipGetLastError();
 }
 
 // ---- scores ------------------------------------------------------------------
 
 constexpr int kScoreWaves = 4;
-constexpr int kHeadsAtOnce = 4;  // whose queries a lane holds: 8 elements, both parts, 64 bits
-constexpr uint64_t kAlways = ~0ull;  // a key of a block that is taken whatever its score; 0: none to take
 
+// Keys that sort as the scores do.  0: no block to take; all ones: a block that
+// is taken whatever its score.
+constexpr uint64_t kAlways = ~0ull;
 __device__ __forceinline__ uint64_t key_of(double score) {
   const uint64_t bits = __builtin_bit_cast(uint64_t, score + 0.0);  // (-0 is 0)
   return bits ^ ((int64_t)bits < 0 ? ~0ull : 1ull << 63);
+}
+
+__device__ __forceinline__ int table_blocks_of(const BlockSelectArgs &a) {
+  return (int)(((int64_t)a.c.width << a.c.page_shift) >> a.b.shift);
+}
+__device__ __forceinline__ int blocks_of(const BlockSelectArgs &a, int length) {
+  return length > 0 ? (int)min(((int64_t)length + (1 << a.b.shift) - 1) >> a.b.shift, (int64_t)table_blocks_of(a)) : 0;
+}
+// Bounds of block b of a sequence on `page` for KV head h.
+__device__ __forceinline__ const uint16_t *bounds_of(const BlockSelectArgs &a, int page, int h, int b, int head_dim) {
+  const int in_page = a.c.page_shift - a.b.shift;
+  return a.b.key_bounds + ((((int64_t)page * a.c.nkv + h) << in_page) + (b & ((1 << in_page) - 1))) * 2 * head_dim;
+}
+
+// Eight elements of a query row from element i on: a NaN is 0, an infinity the
+// largest number.
+__device__ __forceinline__ void query_part(const BlockSelectArgs &a, int64_t i, float (&v)[8]) {
+  if (a.q_type == kElemF32) {
+    const float4 *p = reinterpret_cast<const float4 *>(static_cast<const float *>(a.q) + i);
+    const float4 x = p[0], y = p[1];
+    v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w, v[4] = y.x, v[5] = y.y, v[6] = y.z, v[7] = y.w;
+  } else {
+    const uint4 x = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(a.q) + i);
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const uint32_t b = w[j / 2] >> (16 * (j & 1)) & 0xffffu;
+      v[j] = a.q_type == kElemF16 ? (float)__builtin_bit_cast(_Float16, (uint16_t)b) : bf16_value(b);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 8; j++) v[j] = v[j] != v[j] ? 0.0f : fminf(fmaxf(v[j], -kF32Most), kF32Most);
 }
 
 // Sum over the L lanes of a row (8, 16 or 32).
@@ -190,231 +266,363 @@ __device__ __forceinline__ double row_sum(double v) {
   return v;
 }
 
-__device__ __forceinline__ float query_element(const BlockSelectArgs &a, int64_t i) {
-  const float v = a.q_type == kElemF32   ? static_cast<const float *>(a.q)[i]
-                  : a.q_type == kElemF16 ? (float)static_cast<const _Float16 *>(a.q)[i]
-                                         : bf16_value(static_cast<const uint16_t *>(a.q)[i]);
-  return v != v ? 0.0f : fminf(fmaxf(v, -kF32Most), kF32Most);
-}
-
-// D / 8 lanes have a block's bounds, 8 elements each; a workgroup `per` blocks
-// of a (sequence, KV head).
-template <int D>
+// D / 8 lanes have a block's bounds, 8 elements each, and HEADS of the group's
+// queries at a time; a workgroup has `per` blocks of a (sequence, KV head).  The
+// next block's bounds are on their way while one is worked on, and the table's
+// entry of the one after it.
+template <int D, int HEADS>
 __global__ __launch_bounds__(64 * kScoreWaves) void block_score_kernel(const BlockSelectArgs a, uint64_t *__restrict__ keys,
                                                                        int per, int chunks) {
-  constexpr int kLanes = D / 8, kRows = 64 / kLanes;
+  constexpr int kLanes = D / 8, kRows = 64 / kLanes, kStep = kScoreWaves * kRows;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane % kLanes, sub = lane / kLanes;
   const int row = blockIdx.x / chunks, seq = row / a.c.nkv, h = row - seq * a.c.nkv;
-  const int table_blocks = (int)(((int64_t)a.c.width << a.c.page_shift) >> a.b.shift);
-  const int length = a.c.lengths[seq];
-  const int blocks = length > 0 ? min((int)(((int64_t)length + (1 << a.b.shift) - 1) >> a.b.shift), table_blocks) : 0;
-  const int begin = blockIdx.x % chunks * per, end = min(begin + per, blocks);
-  if (begin >= end) return;
   const int group = a.nq / a.c.nkv, in_page = a.c.page_shift - a.b.shift;
-  const int *table = a.c.pages + (int64_t)seq * a.c.width;
   const int64_t q0 = seq * a.q_stride + (int64_t)h * group * D + 8 * l;
-  for (int g0 = 0; g0 < group; g0 += kHeadsAtOnce) {
-    double up[kHeadsAtOnce][8], down[kHeadsAtOnce][8];
+  const int *table = a.c.pages + (int64_t)seq * a.c.width;
+  const int blocks = blocks_of(a, a.c.lengths[seq]);
+  const int begin = blockIdx.x % chunks * per + wave * kRows, end = min((int)(blockIdx.x % chunks) * per + per, blocks), last = end - 1;
+  if (begin >= end) return;
+  for (int g0 = 0; g0 < group; g0 += HEADS) {
+    int b0 = begin;
+    int entry = table[min(b0 + sub, last) >> in_page], entry_next = table[min(b0 + sub + kStep, last) >> in_page];
+    double up[HEADS][8], down[HEADS][8];
 #pragma unroll
-    for (int g = 0; g < kHeadsAtOnce; g++)
+    for (int g = 0; g < HEADS; g++) {  // (a head beyond the group: the last one's again)
+      float q[8];
+      query_part(a, q0 + (int64_t)min(g0 + g, group - 1) * D, q);
 #pragma unroll
-      for (int j = 0; j < 8; j++) {  // (a head beyond the group: the last one's again)
-        const float v = query_element(a, q0 + (int64_t)min(g0 + g, group - 1) * D + j);
-        up[g][j] = fmaxf(v, 0.0f);
-        down[g][j] = fminf(v, 0.0f);
+      for (int j = 0; j < 8; j++) {
+        up[g][j] = fmaxf(q[j], 0.0f);
+        down[g][j] = fminf(q[j], 0.0f);
       }
-    for (int b0 = begin + wave * kRows; b0 < end; b0 += kScoreWaves * kRows) {
-      const int b = min(b0 + sub, end - 1);
-      const int page = page_or_none(table[b >> in_page], a.c.page_count);
-      const uint16_t *bound = a.b.key_bounds +
-                              ((((int64_t)max(page, 0) * a.c.nkv + h) << in_page) + (b & ((1 << in_page) - 1))) * 2 * D + 8 * l;
-      const uint4 lo = *reinterpret_cast<const uint4 *>(bound), hi = *reinterpret_cast<const uint4 *>(bound + D);
+    }
+    const uint16_t *bound = bounds_of(a, max(page_or_none(entry, a.c.page_count), 0), h, min(b0 + sub, last), D) + 8 * l;
+    uint4 lo = *reinterpret_cast<const uint4 *>(bound), hi = *reinterpret_cast<const uint4 *>(bound + D);
+    for (; b0 < end; b0 += kStep) {
+      const int b = b0 + sub;
+      const bool absent = page_or_none(entry, a.c.page_count) < 0;
       const uint32_t low[4] = {lo.x, lo.y, lo.z, lo.w}, high[4] = {hi.x, hi.y, hi.z, hi.w};
-      double sum[kHeadsAtOnce];
+      bound = bounds_of(a, max(page_or_none(entry_next, a.c.page_count), 0), h, min(b + kStep, last), D) + 8 * l;
+      entry = entry_next;
+      entry_next = table[min(b + 2 * kStep, last) >> in_page];
+      lo = *reinterpret_cast<const uint4 *>(bound);
+      hi = *reinterpret_cast<const uint4 *>(bound + D);
+      double sum[HEADS];
 #pragma unroll
-      for (int g = 0; g < kHeadsAtOnce; g++) sum[g] = 0.0;
+      for (int g = 0; g < HEADS; g++) sum[g] = 0.0;
 #pragma unroll
       for (int j = 0; j < 8; j++) {
         const double x = (double)bf16_value(low[j / 2] >> (16 * (j & 1)) & 0xffffu);
         const double y = (double)bf16_value(high[j / 2] >> (16 * (j & 1)) & 0xffffu);
 #pragma unroll
-        for (int g = 0; g < kHeadsAtOnce; g++) sum[g] = fma(up[g][j], y, fma(down[g][j], x, sum[g]));
+        for (int g = 0; g < HEADS; g++) sum[g] = fma(up[g][j], y, fma(down[g][j], x, sum[g]));
       }
       double best = row_sum<kLanes>(sum[0]);
 #pragma unroll
-      for (int g = 1; g < kHeadsAtOnce; g++) best = fmax(best, row_sum<kLanes>(sum[g]));
-      if (l != 0 || b0 + sub >= end) continue;
-      uint64_t *key = keys + (int64_t)row * table_blocks + b;
+      for (int g = 1; g < HEADS; g++) best = fmax(best, row_sum<kLanes>(sum[g]));
+      if (l != 0 || b >= end) continue;
+      uint64_t *key = keys + (int64_t)row * table_blocks_of(a) + b;
       uint64_t k = key_of(best);
       if (g0 > 0) k = max(k, *key);  // (this lane's own of the heads before)
       if (b < a.first_blocks || b >= blocks - a.last_blocks) k = kAlways;
-      *key = page < 0 ? 0 : k;
+      *key = absent ? 0 : k;
     }
   }
 }
 
 // ---- pick --------------------------------------------------------------------
 
-constexpr int kPickThreads = 1024, kPickWaves = kPickThreads / 64;
+constexpr int kPickKeys = 8;     // of a thread, in registers where these are enough
+constexpr int kPickAtOnce = 64;  // keys that one wave ranks by comparing all with all
 
-__device__ __forceinline__ uint64_t wave_or(uint64_t v) {
-#pragma unroll
-  for (int m = 1; m < 64; m *= 2) v |= __shfl_xor(v, m);
-  return v;
-}
-__device__ __forceinline__ uint64_t wave_and(uint64_t v) {
-#pragma unroll
-  for (int m = 1; m < 64; m *= 2) v &= __shfl_xor(v, m);
-  return v;
+__device__ __forceinline__ uint64_t lane_key(uint64_t k, int lane) {
+  return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(k >> 32), lane) << 32 |
+         (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)k, lane);
 }
 
-__global__ __launch_bounds__(kPickThreads) void block_pick_kernel(const BlockSelectArgs a, const uint64_t *__restrict__ keys) {
-  __shared__ uint64_t sh_or[kPickWaves], sh_and[kPickWaves];
-  __shared__ int sh_live[kPickWaves], sh_always[kPickWaves];
-  __shared__ int sh_bins[256];
-  __shared__ int sh_digit, sh_need, sh_in;
+// A row's keys in a workgroup's sweeps: in registers (HELD, up to NT * kPickKeys),
+// or read in each.
+template <int NT, bool HELD>
+struct Keys {
+  const uint64_t *key;
+  int n;
+  uint64_t held[HELD ? kPickKeys : 1];
+  __device__ __forceinline__ Keys(const uint64_t *k, int count) : key(k), n(count) {
+    if (HELD) {
+#pragma unroll
+      for (int j = 0; j < kPickKeys; j++) held[j % (HELD ? kPickKeys : 1)] = j * NT + (int)threadIdx.x < n ? key[j * NT + threadIdx.x] : 0;
+    }
+  }
+  template <class F>
+  __device__ __forceinline__ void each(F f) const {  // f(key, place); behind the last: a key of 0
+    if (HELD) {
+#pragma unroll
+      for (int j = 0; j < kPickKeys; j++)
+        if (j * NT < n) f(held[j % (HELD ? kPickKeys : 1)], j * NT + (int)threadIdx.x);
+    } else {
+      for (int i = threadIdx.x; i < n; i += NT) f(key[i], i);
+    }
+  }
+};
+
+// What the sweeps of a workgroup share.
+template <int NT>
+struct PickShared {
+  static constexpr int kWaves = NT / 64;
+  uint64_t any[kWaves], all[kWaves], key[kPickAtOnce], least;
+  int first[kWaves], second[kWaves], bins[256], at[kPickAtOnce], counts[kPickKeys * kWaves + 1];
+  int digit, need, in, last, found;
+};
+
+// The need-th of the keys other than 0 and kAlways in the order (larger key, lower
+// place), of which there are `in` >= need >= 1 and which have the bits `all` and no
+// others than `any`: its key and place.  Digits of eight bits below those that all
+// share, counted in LDS, until a wave can compare what is left.
+template <int NT, bool HELD>
+__device__ void nth_key(PickShared<NT> &sh, const Keys<NT, HELD> &keys, uint64_t any, uint64_t all, int in, int need,
+                        uint64_t *at_key, int *at_place) {
+  constexpr int kWaves = NT / 64;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int row = blockIdx.x, seq = row / a.c.nkv;
-  const int table_blocks = (int)(((int64_t)a.c.width << a.c.page_shift) >> a.b.shift);
-  const int length = a.c.lengths[seq];
-  const int n = length > 0 ? min((int)(((int64_t)length + (1 << a.b.shift) - 1) >> a.b.shift), table_blocks) : 0;
-  const uint64_t *key = keys + (int64_t)row * table_blocks;
+  const uint64_t differ = any ^ all;
+  int shift = differ ? 64 - __builtin_clzll(differ) : 0;  // they agree in the bits from here on
+  uint64_t least = shift < 64 ? all >> shift << shift : 0;
+  auto among = [&](uint64_t k) { return k != 0 && k != kAlways && (shift == 64 || k >> shift == least >> shift); };
+  while (shift > 0 && in > kPickAtOnce) {
+    const int low = max(shift - 8, 0), digits = (1 << (shift - low)) - 1;
+    keys.each([&](uint64_t k, int) {
+      if (among(k)) atomicAdd(&sh.bins[(int)(k >> low) & digits], 1);
+    });
+    __syncthreads();
+    if (wave == 0) {  // from the largest digit down: four a lane
+      int c[4], sum = 0;
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        sum += c[j] = sh.bins[255 - 4 * lane - j];
+        sh.bins[255 - 4 * lane - j] = 0;
+      }
+      int to = sum;
+#pragma unroll
+      for (int d = 1; d < 64; d *= 2) {
+        const int o = __shfl_up(to, d);
+        to += lane >= d ? o : 0;
+      }
+      int before = to - sum;
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        if (before < need && need <= before + c[j]) {  // one lane's one digit
+          sh.digit = 255 - 4 * lane - j;
+          sh.need = need - before;
+          sh.in = c[j];
+        }
+        before += c[j];
+      }
+    }
+    __syncthreads();
+    least |= (uint64_t)sh.digit << low;
+    need = sh.need;
+    in = sh.in;
+    shift = low;
+  }
+  if (in <= kPickAtOnce) {  // the rank of each: how many are ahead of it
+    keys.each([&](uint64_t k, int i) {
+      if (among(k)) {
+        const int at = atomicAdd(&sh.found, 1);
+        sh.key[at] = k;
+        sh.at[at] = i;
+      }
+    });
+    __syncthreads();
+    if (wave == 0) {
+      const uint64_t k = lane < in ? sh.key[lane] : 0;
+      const int i = lane < in ? sh.at[lane] : 0x7fffffff;
+      int ahead = 0;
+      for (int j = 0; j < in; j++) {
+        const uint64_t other = lane_key(k, j);
+        ahead += other > k || (other == k && __builtin_amdgcn_readlane(i, j) < i);
+      }
+      if (lane < in && ahead == need - 1) {
+        sh.least = k;
+        sh.last = i;
+      }
+    }
+  } else {  // all alike: the place of the need-th
+    int seen = 0;
+    for (int i0 = 0; i0 < keys.n && seen < need; i0 += NT) {
+      const bool is = i0 + tid < keys.n && keys.key[i0 + tid] == least;
+      const uint64_t mask = __ballot(is);
+      __syncthreads();
+      if (lane == 0) sh.first[wave] = __popcll(mask);
+      __syncthreads();
+      int rank = seen + __popcll(mask & ((1ull << lane) - 1));
+#pragma unroll
+      for (int w = 0; w < kWaves; w++) {
+        rank += w < wave ? sh.first[w] : 0;
+        seen += sh.first[w];
+      }
+      if (is && rank == need - 1) {
+        sh.least = least;
+        sh.last = i0 + tid;
+      }
+    }
+  }
+  __syncthreads();
+  *at_key = sh.least;
+  *at_place = sh.last;
+}
 
-  // how many there are, and the bits in which the others' keys differ
-  uint64_t any = 0, all = ~0ull;
+// The places that `taken` says, in their order, and -1 behind them.
+template <int NT, bool HELD, class Taken>
+__device__ void put_places(PickShared<NT> &sh, const Keys<NT, HELD> &keys, Taken taken, int budget, int *__restrict__ out,
+                           int *count) {
+  constexpr int kWaves = NT / 64;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  int total = 0;
+  if (HELD) {
+    uint64_t masks[kPickKeys];
+#pragma unroll
+    for (int j = 0; j < kPickKeys; j++) {
+      masks[j] = __ballot(j * NT + tid < keys.n && taken(keys.held[j % (HELD ? kPickKeys : 1)], j * NT + tid));
+      if (lane == 0) sh.counts[j * kWaves + wave] = __popcll(masks[j]);
+    }
+    __syncthreads();
+    if (wave == 0) {
+      constexpr int kAll = kPickKeys * kWaves, kPer = (kAll + 63) / 64;
+      int c[kPer], sum = 0;
+#pragma unroll
+      for (int j = 0; j < kPer; j++) sum += c[j] = lane * kPer + j < kAll ? sh.counts[lane * kPer + j] : 0;
+      int to = sum;
+#pragma unroll
+      for (int d = 1; d < 64; d *= 2) {
+        const int o = __shfl_up(to, d);
+        to += lane >= d ? o : 0;
+      }
+      int before = to - sum;
+#pragma unroll
+      for (int j = 0; j < kPer; j++) {
+        if (lane * kPer + j < kAll) sh.counts[lane * kPer + j] = before;
+        before += c[j];
+      }
+      if (lane == 63) sh.counts[kAll] = to;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kPickKeys; j++) {
+      const int at = sh.counts[j * kWaves + wave] + __popcll(masks[j] & ((1ull << lane) - 1));
+      if ((masks[j] >> lane & 1) != 0 && at < budget) out[at] = j * NT + tid;
+    }
+    total = sh.counts[kPickKeys * kWaves];
+  } else {
+    for (int i0 = 0; i0 < keys.n && total < budget; i0 += NT) {
+      const bool is = i0 + tid < keys.n && taken(keys.key[i0 + tid], i0 + tid);
+      const uint64_t mask = __ballot(is);
+      __syncthreads();
+      if (lane == 0) sh.first[wave] = __popcll(mask);
+      __syncthreads();
+      int at = total + __popcll(mask & ((1ull << lane) - 1));
+#pragma unroll
+      for (int w = 0; w < kWaves; w++) {
+        at += w < wave ? sh.first[w] : 0;
+        total += sh.first[w];
+      }
+      if (is && at < budget) out[at] = i0 + tid;
+    }
+  }
+  total = min(total, budget);
+  for (int i = total + tid; i < budget; i += NT) out[i] = -1;
+  if (tid == 0 && count) *count = total;
+}
+
+// One (sequence, KV head).
+template <int NT, bool HELD>
+__device__ void pick(const BlockSelectArgs &a, const uint64_t *key, int n, int *out, int *count) {
+  __shared__ PickShared<NT> sh;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const Keys<NT, HELD> keys(key, n);
+  // how many there are, and the bits in which the scored ones differ
   int live = 0, always = 0;
-  for (int i = tid; i < n; i += kPickThreads) {
-    const uint64_t k = key[i];
+  uint64_t any = 0, all = ~0ull;
+  keys.each([&](uint64_t k, int) {
     live += k != 0;
     always += k == kAlways;
     if (k != 0 && k != kAlways) {
       any |= k;
       all &= k;
     }
-  }
-  any = wave_or(any);
-  all = wave_and(all);
+  });
 #pragma unroll
   for (int m = 1; m < 64; m *= 2) {
     live += __shfl_xor(live, m);
     always += __shfl_xor(always, m);
+    any |= __shfl_xor(any, m);
+    all &= __shfl_xor(all, m);
   }
   if (lane == 0) {
-    sh_or[wave] = any;
-    sh_and[wave] = all;
-    sh_live[wave] = live;
-    sh_always[wave] = always;
+    sh.first[wave] = live;
+    sh.second[wave] = always;
+    sh.any[wave] = any;
+    sh.all[wave] = all;
   }
+  if (tid < 256) sh.bins[tid] = 0;
+  if (tid == 0) sh.found = 0;
   __syncthreads();
   live = always = 0;
-  for (int w = 0; w < kPickWaves; w++) {
-    any |= sh_or[w];
-    all &= sh_and[w];
-    live += sh_live[w];
-    always += sh_always[w];
+#pragma unroll
+  for (int w = 0; w < NT / 64; w++) {
+    live += sh.first[w];
+    always += sh.second[w];
+    any |= sh.any[w];
+    all &= sh.all[w];
   }
-  __syncthreads();  // (the counts' places are used again)
+  __syncthreads();  // (the places are used again)
 
-  // the threshold: keys above `least | low bits` are taken, and `need` of those
-  // whose bits from `shift` on are its own
-  int need = a.budget - always, shift = 64;
-  uint64_t least = 0;
-  const bool whole = live <= a.budget;  // (the same for the workgroup)
-  if (!whole && need > 0) {
-    const uint64_t differ = any ^ all;
-    shift = differ ? 64 - __builtin_clzll(differ) : 0;  // the bits from here on are the same
-    least = shift < 64 ? all >> shift << shift : 0;
-    int in = live - always;
-    while (shift > 0 && in > need) {
-      const int low = max(shift - 8, 0), bits = shift - low;
-      for (int i = tid; i < 256; i += kPickThreads) sh_bins[i] = 0;
-      __syncthreads();
-      for (int i = tid; i < n; i += kPickThreads) {
-        const uint64_t k = key[i];
-        if (k != 0 && k != kAlways && (shift == 64 || k >> shift == least >> shift))
-          atomicAdd(&sh_bins[(k >> low) & ((1 << bits) - 1)], 1);
-      }
-      __syncthreads();
-      if (wave == 0) {  // from the largest digit down: four a lane
-        int c[4], sum = 0;
-#pragma unroll
-        for (int j = 0; j < 4; j++) sum += c[j] = sh_bins[255 - 4 * lane - j];
-        int to = sum;
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-          const int o = __shfl_up(to, d);
-          to += lane >= d ? o : 0;
-        }
-        int before = to - sum;
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-          if (before < need && need <= before + c[j]) {  // one lane's one digit
-            sh_digit = 255 - 4 * lane - j;
-            sh_need = need - before;
-            sh_in = c[j];
-          }
-          before += c[j];
-        }
-      }
-      __syncthreads();
-      least |= (uint64_t)sh_digit << low;
-      need = sh_need;
-      in = sh_in;
-      shift = low;
-      __syncthreads();
-    }
-    if (in <= need) need = in;
-  }
+  // taken: keys above `least`, and those equal to it up to place `last`
+  uint64_t least = live <= a.budget ? 0 : kAlways - 1;
+  int last = -1;
+  if (live > a.budget && a.budget > always) nth_key(sh, keys, any, all, live - always, a.budget - always, &least, &last);
+  put_places(sh, keys, [&](uint64_t k, int i) { return k > least || (k == least && i <= last); }, a.budget, out, count);
+}
 
-  // in their order
-  int *out = a.selected + (int64_t)row * a.budget;
-  int taken = 0, equal = 0;  // up to the blocks at hand, by the whole workgroup
-  for (int i0 = 0; i0 < n && taken < a.budget; i0 += kPickThreads) {
-    const int i = i0 + tid;
-    const uint64_t k = i < n ? key[i] : 0;
-    const bool other = k != 0 && k != kAlways;
-    const bool same = !whole && need > 0 && other && (shift == 64 || k >> shift == least >> shift);
-    const bool above = k == kAlways || (whole && k != 0) || (!whole && need > 0 && other && !same && k > least);
-    const uint64_t same_mask = __ballot(same);
-    if (lane == 0) sh_live[wave] = __popcll(same_mask);
-    __syncthreads();
-    int rank = equal + __popcll(same_mask & ((1ull << lane) - 1)), sames = 0;
-    for (int w = 0; w < kPickWaves; w++) {
-      rank += w < wave ? sh_live[w] : 0;
-      sames += sh_live[w];
-    }
-    const bool take = above || (same && rank < need);
-    const uint64_t mask = __ballot(take);
-    if (lane == 0) sh_always[wave] = __popcll(mask);
-    __syncthreads();
-    int at = taken + __popcll(mask & ((1ull << lane) - 1)), takes = 0;
-    for (int w = 0; w < kPickWaves; w++) {
-      at += w < wave ? sh_always[w] : 0;
-      takes += sh_always[w];
-    }
-    if (take && at < a.budget) out[at] = i;
-    taken += takes;
-    equal += sames;
-  }
-  taken = min(taken, a.budget);
-  for (int i = taken + tid; i < a.budget; i += kPickThreads) out[i] = -1;
-  if (tid == 0 && a.counts) a.counts[row] = taken;
+template <int NT>
+__global__ __launch_bounds__(NT) void block_pick_kernel(const BlockSelectArgs a, const uint64_t *__restrict__ keys) {
+  const int row = blockIdx.x, n = blocks_of(a, a.c.lengths[row / a.c.nkv]);
+  const uint64_t *key = keys + (int64_t)row * table_blocks_of(a);
+  int *out = a.selected + (int64_t)row * a.budget, *count = a.counts ? a.counts + row : nullptr;
+  if (n <= NT * kPickKeys)
+    pick<NT, true>(a, key, n, out, count);
+  else
+    pick<NT, false>(a, key, n, out, count);
+}
+
+template <int D>
+void launch_scores(const BlockSelectArgs &a, uint64_t *keys, int grid, int per, int chunks, hipStream_t s) {
+  const int group = a.nq / a.c.nkv;
+  if (group == 1)
+    hipLaunchKernelGGL((block_score_kernel<D, 1>), dim3(grid), dim3(64 * kScoreWaves), 0, s, a, keys, per, chunks);
+  else if (group == 2)
+    hipLaunchKernelGGL((block_score_kernel<D, 2>), dim3(grid), dim3(64 * kScoreWaves), 0, s, a, keys, per, chunks);
+  else
+    hipLaunchKernelGGL((block_score_kernel<D, 4>), dim3(grid), dim3(64 * kScoreWaves), 0, s, a, keys, per, chunks);
 }
 
 template <int D>
 hipError_t launch_select_width(const BlockSelectArgs &a, uint64_t *keys, int num_cus, hipStream_t s) {
   constexpr int kRows = 64 / (D / 8) * kScoreWaves;  // blocks of a workgroup at once
   const int64_t rows = (int64_t)a.c.sequences * a.c.nkv, table_blocks = ((int64_t)a.c.width << a.c.page_shift) >> a.b.shift;
-  // eight workgroups a CU where there are as many blocks
-  int64_t per = (rows * table_blocks + 8 * num_cus - 1) / (8 * num_cus);
+  // four workgroups a CU where there are as many blocks (24 contexts up to 32768
+  // in blocks of 64, 8 KV heads of 128, groups of 4: 12.0 us, eight 14.6, sixteen
+  // 17.4; two of 262144 in blocks of 32, 4 KV heads: 14.4, 15.4, 17.0; two heads at
+  // a time in place of four 14.9 and 16.4, one 21.4 and 20.0)
+  int64_t per = (rows * table_blocks + 4 * num_cus - 1) / (4 * num_cus);
   per = (per + kRows - 1) / kRows * kRows;
-  per = per < kRows ? kRows : per > 32 * kRows ? 32 * kRows : per;
+  per = per < kRows ? kRows : per > 64 * kRows ? 64 * kRows : per;
   const int64_t chunks = (table_blocks + per - 1) / per;
-  hipLaunchKernelGGL(block_score_kernel<D>, dim3((unsigned)(rows * chunks)), dim3(64 * kScoreWaves), 0, s, a, keys,
-                     (int)per, (int)chunks);
+  launch_scores<D>(a, keys, (int)(rows * chunks), (int)per, (int)chunks, s);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(block_pick_kernel, dim3((unsigned)rows), dim3(kPickThreads), 0, s, a, keys);
+  if (table_blocks <= 256 * kPickKeys)
+    hipLaunchKernelGGL(block_pick_kernel<256>, dim3((unsigned)rows), dim3(256), 0, s, a, keys);
+  else
+    hipLaunchKernelGGL(block_pick_kernel<1024>, dim3((unsigned)rows), dim3(1024), 0, s, a, keys);
   return hipGetLastError();
 }
 
@@ -425,15 +633,14 @@ bool block_bounds_fits(const BlockBoundsArgs &a) {
   return !((slots * a.c.nkv) >> 31);
 }
 
-hipError_t launch_block_bounds(const BlockBoundsArgs &a, hipStream_t s) {
+hipError_t launch_block_bounds(const BlockBoundsArgs &a, int num_cus, hipStream_t s) {
   if (a.tokens < 1 || a.c.nkv < 1 || !a.b.key_bounds || a.b.shift < 4 || a.b.shift > a.c.page_shift || !block_bounds_fits(a))
     return hipErrorInvalidValue;
   const int64_t slots = a.offsets ? touched_blocks(a.tokens, a.c.sequences, 1 << a.b.shift) : a.c.sequences;
-  const int units = (int)(slots * a.c.nkv);
   switch (a.c.head_dim) {
-    case 64: return launch_bounds_type<64>(a, units, s);
-    case 128: return launch_bounds_type<128>(a, units, s);
-    case 256: return launch_bounds_type<256>(a, units, s);
+    case 64: return launch_bounds_type<64>(a, (int)slots, num_cus, s);
+    case 128: return launch_bounds_type<128>(a, (int)slots, num_cus, s);
+    case 256: return launch_bounds_type<256>(a, (int)slots, num_cus, s);
     default: return hipErrorInvalidValue;
   }
 }

@@ -3257,12 +3257,15 @@ int32_t hp_hip_page_plan_device(const hp_hip_page_plan_t *plan, void *stream) {
       [&](State &s, hipStream_t strm) -> int32_t {
         if (a.sequences == 0) return HP_OK;
         void *scratch = nullptr;
-        int32_t rc = stream_scratch(strm, kScratchPlan, page_plan_scratch_bytes(a), &scratch);
-        if (rc != HP_OK) return rc;
+        const bool small = page_plan_is_small(a);
+        if (!small) {
+          int32_t rc = stream_scratch(strm, kScratchPlan, page_plan_scratch_bytes(a), &scratch);
+          if (rc != HP_OK) return rc;
+        }
         hipEvent_t e = prof_begin(strm);
         HP_HIP_TRY(launch_page_plan(a, scratch, strm));
         prof_end(HP_KERNEL_ATTENTION, e, strm);
-        s.launches += 3 + (a.keep_from != nullptr) + (a.rows > 0);
+        s.launches += small ? 1 : 3 + (a.keep_from != nullptr);
         return HP_OK;
       });
 }
@@ -3291,7 +3294,7 @@ int32_t hp_hip_block_bounds_device(const hp_hip_paged_cache_t *cache, const hp_h
       [&](State &s, hipStream_t strm) -> int32_t {
         if (a.c.sequences == 0 || a.tokens == 0) return HP_OK;
         hipEvent_t e = prof_begin(strm);
-        HP_HIP_TRY(launch_block_bounds(a, strm));
+        HP_HIP_TRY(launch_block_bounds(a, s.num_cus, strm));
         prof_end(HP_KERNEL_ATTENTION, e, strm);
         s.launches++;
         return HP_OK;

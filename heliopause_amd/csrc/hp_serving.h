@@ -85,7 +85,7 @@ struct BlockBoundsArgs {
   int tokens;
 };
 bool block_bounds_fits(const BlockBoundsArgs &a);
-hipError_t launch_block_bounds(const BlockBoundsArgs &a, hipStream_t s);
+hipError_t launch_block_bounds(const BlockBoundsArgs &a, int num_cus, hipStream_t s);
 
 struct BlockSelectArgs {
   PagedCache c;
@@ -106,6 +106,7 @@ struct PagePlanArgs {
   int64_t *slots;
   int sequences, width, page_shift, page_count, rows;
 };
+bool page_plan_is_small(const PagePlanArgs &a);  // one launch, no scratch
 size_t page_plan_scratch_bytes(const PagePlanArgs &a);
 hipError_t launch_page_plan(const PagePlanArgs &a, void *scratch, hipStream_t s);
 
@@ -150,6 +151,23 @@ __device__ __forceinline__ int packed_sequence_of(const int *__restrict__ offset
   }
   const bool le = lane < n && offsets[lo + 1 + min(lane, max(n - 1, 0))] <= t;
   return lo + __popcll(__ballot(le));
+}
+
+// The sequence whose touched blocks (hp_pages.h) have slot `slot`, by a whole
+// wave: the largest s in 0 .. n - 1 whose first slot is not behind it.
+__device__ __forceinline__ int touched_sequence(const int *__restrict__ offsets, int n, int slot, int block) {
+  const int lane = threadIdx.x & 63;
+  int lo = 0;
+  while (n > 64) {
+    const int step = (n + 63) >> 6, i = lo + min(lane * step, n - 1);
+    const bool le = lane * step < n && touched_first(offsets[i], i, block) <= slot;
+    const int c = max(__popcll(__ballot(le)), 1) - 1;
+    lo += c * step;
+    n = min(step, n - c * step);
+  }
+  const int i = lo + min(lane, n - 1);
+  const bool le = lane < n && touched_first(offsets[i], i, block) <= slot;
+  return lo + max(__popcll(__ballot(le)), 1) - 1;
 }
 
 // DPP rotation of each 16-lane row by eight: lane c gets lane c ^ 8's value.

@@ -29,7 +29,10 @@ uint64_t paged_attn_most_steps(const PagedAttnArgs &a) {
 
 int paged_attn_groups(const PagedAttnArgs &a, int num_cus) {
   const uint64_t most = paged_attn_most_steps(a);
-  const int room = 2 * num_cus / blocks_of(a.nq, a.c.nkv);  // two workgroups a CU
+  // two workgroups a CU; block_attn.hip's of 8 bits, which have half the bytes on
+  // their way in as many keys, as many as the registers hold
+  const int each = elem_bytes(a.c.type) == 1 && (a.key_scales || a.selected) ? a.c.head_dim == 64 ? 4 : a.c.head_dim == 128 ? 3 : 2 : 2;
+  const int room = each * num_cus / blocks_of(a.nq, a.c.nkv);
   return most < (uint64_t)room ? (int)most : room < 1 ? 1 : room;
 }
 

@@ -700,7 +700,7 @@ int32_t hp_hip_logit_rules_device(const hp_hip_logit_rules_t *rules, void *strea
  * lengths as they were, pages dealt before are found in the table.  A page that
  * two rows of the table name must not go back through both; the stack holds
  * d_free's page_count entries at most, what goes back beyond is lost.  Up to four
- * launches, over scratch of the stream's. */
+ * launches, over scratch of the stream's; one where it is small. */
 typedef struct hp_hip_page_plan {
   int32_t *d_pages;              /* [sequence_count][pages_per_sequence] */
   const int32_t *d_lengths;      /* [sequence_count]; below 1: empty */

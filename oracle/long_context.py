@@ -111,7 +111,7 @@ def select(q, bound, lengths, pages, page_size, page_count, block, budget, first
                     continue
                 lo, hi = bound[page, h, b % per].astype(np.float64)
                 rows = q[s, h * (H // kv):(h + 1) * (H // kv)]
-                score = max(float(np.sum(np.maximum(r * lo, r * hi))) for r in rows)
+                score = max(math.fsum(np.maximum(r * lo, r * hi)) for r in rows)
                 scores.append((-math.inf if b < first or b >= n - last else -score, b))
             got.append(sorted(b for _, b in sorted(scores)[:budget]))
     return got

@@ -576,6 +576,41 @@ def test_select_from_many(hip, L, blocks):
         run_select(L, pool, 2, max(budget, 2), 1, 1, rng)
 
 
+@pytest.mark.parametrize("blocks", [300, 3000, 20000])
+@pytest.mark.parametrize("alike", ["all", "few", "nearly"])
+def test_select_where_many_are_alike(hip, L, blocks, alike):
+    """Blocks of equal bounds, of a few kinds, and of bounds of which one element differs by the last bit of bf16 under a
+    query element of 2^-20: all within what single precision can tell apart."""
+    t = _torch()
+    rng = np.random.default_rng(blocks)
+    pool = bounded(Pool(rng, [16 * blocks], 1, 64, 128, 16, "i8", extra=0), rng)
+    b = pool.bounds.float().cpu().numpy()
+    flat = np.empty((blocks, 2, 64), np.float32)
+    kinds = rng.integers(0, {"all": 1, "few": 5, "nearly": 1}[alike], blocks)
+    flat[:] = b[pool.pages[0, 0], 0, :1]
+    flat[:, :, 5] += kinds[:, None] * np.float32(0.5)
+    if alike == "nearly":
+        flat[:, :, 9] = (1 + rng.integers(0, 100, blocks)[:, None] * 2.0 ** -7).astype(np.float32)
+    for i in range(blocks):
+        b[pool.pages[0, i // 8], 0, i % 8] = flat[i]
+    pool.bounds = t.from_numpy(b).cuda().to(t.bfloat16)
+    q = rng.standard_normal((1, 2, 64)).astype(np.float32)
+    q[:, :, 9] = 2.0 ** -20
+    for budget in (1, 70, 299):
+        run_select(L, pool, 2, budget, 0, 1, q=dev(q))
+
+
+@pytest.mark.parametrize("times", [2.0 ** 100, 2.0 ** -120, 3e38, 1e-45])
+def test_select_of_large_and_small_numbers(hip, L, times):
+    """Scores past f32's range and below its normal numbers."""
+    rng = np.random.default_rng(3)
+    pool = bounded(Pool(rng, [3000, 40], 2, 128, 64, 32, "i8"), rng)
+    big = bounded(Pool(rng, [3000, 40], 2, 128, 64, 32, "i8"), rng, spread=1e36)
+    q = (np.clip(rng.standard_normal((2, 6, 128)), -1, 1) * times).astype(np.float32)
+    for p in (pool, big):
+        run_select(L, p, 6, 20, 1, 1, q=dev(q))
+
+
 def test_select_ties_and_odd_scores(hip, L):
     """Equal scores go to the first blocks; zeros of both signs are equal; scores that differ in their last bits only;
     infinite and NaN queries; the largest bounds."""
