@@ -251,25 +251,62 @@ __device__ __forceinline__ void query_part(const BlockSelectArgs &a, int64_t i, 
       v[j] = a.q_type == kElemF16 ? (float)__builtin_bit_cast(_Float16, (uint16_t)b) : bf16_value(b);
     }
   }
+  float odd = 0.0f;  // a NaN where an element is not finite
 #pragma unroll
-  for (int j = 0; j < 8; j++) v[j] = v[j] != v[j] ? 0.0f : fminf(fmaxf(v[j], -kF32Most), kF32Most);
+  for (int j = 0; j < 8; j++) odd += v[j] * 0.0f;
+  if (odd != 0.0f) {  // (NaN)
+#pragma unroll
+    for (int j = 0; j < 8; j++) v[j] = v[j] != v[j] ? 0.0f : fminf(fmaxf(v[j], -kF32Most), kF32Most);
+  }
 }
 
-// Sum over the L lanes of a row (8, 16 or 32).
-template <int L>
-__device__ __forceinline__ double row_sum(double v) {
-  v += dpp_f64<kDppXor1>(v);
-  v += dpp_f64<kDppXor2>(v);
-  v += dpp_f64<kDppRowHalfMirror>(v);
-  if (L >= 16) v += dpp_f64<kDppRowMirror>(v);
-  if (L >= 32) v += __shfl_xor(v, 16);
-  return v;
+// A permutation of each 16-lane row that has a source for every lane.
+template <int CTRL>
+__device__ __forceinline__ uint32_t permuted(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
+}
+template <int CTRL>
+__device__ __forceinline__ double permuted(double v) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  return __builtin_bit_cast(double, (uint64_t)permuted<CTRL>((uint32_t)(b >> 32)) << 32 | permuted<CTRL>((uint32_t)b));
+}
+constexpr int kDppRor4 = 0x124, kDppReverse = 0x1B;  // quad_perm [3,2,1,0]
+
+// Of two sums of every lane, x's over the lane and its partner in the lanes whose
+// bit of `odd` is clear, y's in the others.
+template <int CTRL>
+__device__ __forceinline__ double joined(double x, double y, bool odd) {
+  const double keep = odd ? y : x, send = odd ? x : y;
+  return keep + permuted<CTRL>(send);
+}
+
+// Largest of the HEADS sums over the L lanes of a row (8, 16 or 32).  The lanes
+// first share the sums out, so that each step has half as many.
+template <int L, int HEADS>
+__device__ __forceinline__ double largest_sum(const double (&v)[HEADS], int lane) {
+  double s;
+  if (HEADS == 4) {
+    s = joined<kDppXor2>(joined<kDppXor1>(v[0], v[1 % HEADS], lane & 1), joined<kDppXor1>(v[2 % HEADS], v[3 % HEADS], lane & 1), lane & 2);
+  } else {
+    s = HEADS == 2 ? joined<kDppXor1>(v[0], v[1 % HEADS], lane & 1) : v[0] + permuted<kDppXor1>(v[0]);
+    s += permuted<kDppXor2>(s);
+  }
+  if (L == 8) {
+    s += permuted<kDppReverse>(permuted<kDppRowHalfMirror>(s));  // lane ^ 4
+  } else {
+    s += permuted<kDppRor8>(s);
+    s += permuted<kDppRor4>(s);
+    if (L == 32) s += __shfl_xor(s, 16);
+  }
+  if (HEADS >= 2) s = fmax(s, permuted<kDppXor1>(s));
+  if (HEADS == 4) s = fmax(s, permuted<kDppXor2>(s));
+  return s;
 }
 
 // D / 8 lanes have a block's bounds, 8 elements each, and HEADS of the group's
 // queries at a time; a workgroup has `per` blocks of a (sequence, KV head).  The
 // next block's bounds are on their way while one is worked on, and the table's
-// entry of the one after it.
+// entry of the one after it (four turns ahead: the same or slower).
 template <int D, int HEADS>
 __global__ __launch_bounds__(64 * kScoreWaves) void block_score_kernel(const BlockSelectArgs a, uint64_t *__restrict__ keys,
                                                                        int per, int chunks) {
@@ -283,8 +320,7 @@ __global__ __launch_bounds__(64 * kScoreWaves) void block_score_kernel(const Blo
   const int begin = blockIdx.x % chunks * per + wave * kRows, end = min((int)(blockIdx.x % chunks) * per + per, blocks), last = end - 1;
   if (begin >= end) return;
   for (int g0 = 0; g0 < group; g0 += HEADS) {
-    int b0 = begin;
-    int entry = table[min(b0 + sub, last) >> in_page], entry_next = table[min(b0 + sub + kStep, last) >> in_page];
+    int entry = table[min(begin + sub, last) >> in_page], entry_next = table[min(begin + sub + kStep, last) >> in_page];
     double up[HEADS][8], down[HEADS][8];
 #pragma unroll
     for (int g = 0; g < HEADS; g++) {  // (a head beyond the group: the last one's again)
@@ -296,9 +332,9 @@ __global__ __launch_bounds__(64 * kScoreWaves) void block_score_kernel(const Blo
         down[g][j] = fminf(q[j], 0.0f);
       }
     }
-    const uint16_t *bound = bounds_of(a, max(page_or_none(entry, a.c.page_count), 0), h, min(b0 + sub, last), D) + 8 * l;
+    const uint16_t *bound = bounds_of(a, max(page_or_none(entry, a.c.page_count), 0), h, min(begin + sub, last), D) + 8 * l;
     uint4 lo = *reinterpret_cast<const uint4 *>(bound), hi = *reinterpret_cast<const uint4 *>(bound + D);
-    for (; b0 < end; b0 += kStep) {
+    for (int b0 = begin; b0 < end; b0 += kStep) {
       const int b = b0 + sub;
       const bool absent = page_or_none(entry, a.c.page_count) < 0;
       const uint32_t low[4] = {lo.x, lo.y, lo.z, lo.w}, high[4] = {hi.x, hi.y, hi.z, hi.w};
@@ -317,9 +353,7 @@ __global__ __launch_bounds__(64 * kScoreWaves) void block_score_kernel(const Blo
 #pragma unroll
         for (int g = 0; g < HEADS; g++) sum[g] = fma(up[g][j], y, fma(down[g][j], x, sum[g]));
       }
-      double best = row_sum<kLanes>(sum[0]);
-#pragma unroll
-      for (int g = 1; g < HEADS; g++) best = fmax(best, row_sum<kLanes>(sum[g]));
+      const double best = largest_sum<kLanes>(sum, lane);
       if (l != 0 || b >= end) continue;
       uint64_t *key = keys + (int64_t)row * table_blocks_of(a) + b;
       uint64_t k = key_of(best);
@@ -333,6 +367,10 @@ __global__ __launch_bounds__(64 * kScoreWaves) void block_score_kernel(const Blo
 // ---- pick --------------------------------------------------------------------
 
 constexpr int kPickKeys = 8;     // of a thread, in registers where these are enough
+template <int NT>
+constexpr int digit_bits() {  // (so that one digit mostly leaves few enough)
+  return NT > 256 ? 11 : 8;
+}
 constexpr int kPickAtOnce = 64;  // keys that one wave ranks by comparing all with all
 
 __device__ __forceinline__ uint64_t lane_key(uint64_t k, int lane) {
@@ -369,15 +407,42 @@ struct Keys {
 template <int NT>
 struct PickShared {
   static constexpr int kWaves = NT / 64;
+  static constexpr int kBins = 1 << digit_bits<NT>(), kEach = kBins / NT;  // of a thread
   uint64_t any[kWaves], all[kWaves], key[kPickAtOnce], least;
-  int first[kWaves], second[kWaves], bins[256], at[kPickAtOnce], counts[kPickKeys * kWaves + 1];
+  int first[kWaves], second[kWaves], bins[kBins], at[kPickAtOnce], counts[kPickKeys * kWaves + 1];
   int digit, need, in, last, found;
 };
 
+// The bits that some, and that all, of a wave's lanes have.
+template <int CTRL>
+__device__ __forceinline__ void join_bits(uint32_t (&any)[2], uint32_t (&all)[2]) {
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    any[i] |= permuted<CTRL>(any[i]);
+    all[i] &= permuted<CTRL>(all[i]);
+  }
+}
+__device__ __forceinline__ void wave_bits(uint64_t &some, uint64_t &every) {
+  uint32_t any[2] = {(uint32_t)some, (uint32_t)(some >> 32)}, all[2] = {(uint32_t)every, (uint32_t)(every >> 32)};
+  join_bits<kDppXor1>(any, all);
+  join_bits<kDppXor2>(any, all);
+  join_bits<kDppRowHalfMirror>(any, all);
+  join_bits<kDppRowMirror>(any, all);
+  uint32_t o[2], a[2];
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    auto lane = [](uint32_t v, int l) { return (uint32_t)__builtin_amdgcn_readlane((int)v, l); };
+    o[i] = lane(any[i], 0) | lane(any[i], 16) | lane(any[i], 32) | lane(any[i], 48);
+    a[i] = lane(all[i], 0) & lane(all[i], 16) & lane(all[i], 32) & lane(all[i], 48);
+  }
+  some = (uint64_t)o[1] << 32 | o[0];
+  every = (uint64_t)a[1] << 32 | a[0];
+}
+
 // The need-th of the keys other than 0 and kAlways in the order (larger key, lower
 // place), of which there are `in` >= need >= 1 and which have the bits `all` and no
-// others than `any`: its key and place.  Digits of eight bits below those that all
-// share, counted in LDS, until a wave can compare what is left.
+// others than `any`: its key and place.  Digits below the bits that all share,
+// counted in LDS, until a wave can compare what is left.
 template <int NT, bool HELD>
 __device__ void nth_key(PickShared<NT> &sh, const Keys<NT, HELD> &keys, uint64_t any, uint64_t all, int in, int need,
                         uint64_t *at_key, int *at_place) {
@@ -388,34 +453,33 @@ __device__ void nth_key(PickShared<NT> &sh, const Keys<NT, HELD> &keys, uint64_t
   uint64_t least = shift < 64 ? all >> shift << shift : 0;
   auto among = [&](uint64_t k) { return k != 0 && k != kAlways && (shift == 64 || k >> shift == least >> shift); };
   while (shift > 0 && in > kPickAtOnce) {
-    const int low = max(shift - 8, 0), digits = (1 << (shift - low)) - 1;
+    using S = PickShared<NT>;
+    const int low = max(shift - digit_bits<NT>(), 0), digits = (1 << (shift - low)) - 1;
     keys.each([&](uint64_t k, int) {
       if (among(k)) atomicAdd(&sh.bins[(int)(k >> low) & digits], 1);
     });
     __syncthreads();
-    if (wave == 0) {  // from the largest digit down: four a lane
-      int c[4], sum = 0;
+    // from the largest digit down
+    int c[S::kEach], sum = 0;
 #pragma unroll
-      for (int j = 0; j < 4; j++) {
-        sum += c[j] = sh.bins[255 - 4 * lane - j];
-        sh.bins[255 - 4 * lane - j] = 0;
-      }
-      int to = sum;
+    for (int j = 0; j < S::kEach; j++) {
+      sum += c[j] = sh.bins[S::kBins - 1 - S::kEach * tid - j];
+      sh.bins[S::kBins - 1 - S::kEach * tid - j] = 0;
+    }
+    const int to = (int)wave_scan((uint32_t)sum);
+    if (lane == 63) sh.first[wave] = to;
+    __syncthreads();
+    int before = to - sum;
 #pragma unroll
-      for (int d = 1; d < 64; d *= 2) {
-        const int o = __shfl_up(to, d);
-        to += lane >= d ? o : 0;
-      }
-      int before = to - sum;
+    for (int w = 0; w < kWaves; w++) before += w < wave ? sh.first[w] : 0;
 #pragma unroll
-      for (int j = 0; j < 4; j++) {
-        if (before < need && need <= before + c[j]) {  // one lane's one digit
-          sh.digit = 255 - 4 * lane - j;
-          sh.need = need - before;
-          sh.in = c[j];
-        }
-        before += c[j];
+    for (int j = 0; j < S::kEach; j++) {
+      if (before < need && need <= before + c[j]) {  // one thread's one digit
+        sh.digit = S::kBins - 1 - S::kEach * tid - j;
+        sh.need = need - before;
+        sh.in = c[j];
       }
+      before += c[j];
     }
     __syncthreads();
     least |= (uint64_t)sh.digit << low;
@@ -490,12 +554,7 @@ __device__ void put_places(PickShared<NT> &sh, const Keys<NT, HELD> &keys, Taken
       int c[kPer], sum = 0;
 #pragma unroll
       for (int j = 0; j < kPer; j++) sum += c[j] = lane * kPer + j < kAll ? sh.counts[lane * kPer + j] : 0;
-      int to = sum;
-#pragma unroll
-      for (int d = 1; d < 64; d *= 2) {
-        const int o = __shfl_up(to, d);
-        to += lane >= d ? o : 0;
-      }
+      const int to = (int)wave_scan((uint32_t)sum);
       int before = to - sum;
 #pragma unroll
       for (int j = 0; j < kPer; j++) {
@@ -539,22 +598,20 @@ __device__ void pick(const BlockSelectArgs &a, const uint64_t *key, int n, int *
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const Keys<NT, HELD> keys(key, n);
   // how many there are, and the bits in which the scored ones differ
-  int live = 0, always = 0;
+  int live = 0, always = 0;  // (a wave's)
   uint64_t any = 0, all = ~0ull;
   keys.each([&](uint64_t k, int) {
-    live += k != 0;
-    always += k == kAlways;
+    live += __popcll(__ballot(k != 0));
+    always += __popcll(__ballot(k == kAlways));
     if (k != 0 && k != kAlways) {
       any |= k;
       all &= k;
     }
   });
-#pragma unroll
-  for (int m = 1; m < 64; m *= 2) {
-    live += __shfl_xor(live, m);
-    always += __shfl_xor(always, m);
-    any |= __shfl_xor(any, m);
-    all &= __shfl_xor(all, m);
+  wave_bits(any, all);
+  if (!HELD) {  // (the lanes of a sweep's end have not seen it)
+    live = __builtin_amdgcn_readfirstlane(live);
+    always = __builtin_amdgcn_readfirstlane(always);
   }
   if (lane == 0) {
     sh.first[wave] = live;
@@ -562,7 +619,7 @@ __device__ void pick(const BlockSelectArgs &a, const uint64_t *key, int n, int *
     sh.any[wave] = any;
     sh.all[wave] = all;
   }
-  if (tid < 256) sh.bins[tid] = 0;
+  for (int i = tid; i < PickShared<NT>::kBins; i += NT) sh.bins[i] = 0;
   if (tid == 0) sh.found = 0;
   __syncthreads();
   live = always = 0;
@@ -609,9 +666,9 @@ hipError_t launch_select_width(const BlockSelectArgs &a, uint64_t *keys, int num
   constexpr int kRows = 64 / (D / 8) * kScoreWaves;  // blocks of a workgroup at once
   const int64_t rows = (int64_t)a.c.sequences * a.c.nkv, table_blocks = ((int64_t)a.c.width << a.c.page_shift) >> a.b.shift;
   // four workgroups a CU where there are as many blocks (24 contexts up to 32768
-  // in blocks of 64, 8 KV heads of 128, groups of 4: 12.0 us, eight 14.6, sixteen
-  // 17.4; two of 262144 in blocks of 32, 4 KV heads: 14.4, 15.4, 17.0; two heads at
-  // a time in place of four 14.9 and 16.4, one 21.4 and 20.0)
+  // in blocks of 64, 8 KV heads of 128, groups of 4: 11.2 us, eight 14, two 15; two
+  // of 262144 in blocks of 32, 4 KV heads: 14.1, 16, 13.0; two heads at a time in
+  // place of four cost 0.5 to 1 us more, one 6)
   int64_t per = (rows * table_blocks + 4 * num_cus - 1) / (4 * num_cus);
   per = (per + kRows - 1) / kRows * kRows;
   per = per < kRows ? kRows : per > 64 * kRows ? 64 * kRows : per;

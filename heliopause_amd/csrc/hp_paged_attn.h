@@ -179,20 +179,6 @@ __device__ __forceinline__ float row_scale(float m, float l, float value_scale) 
   return m == kNegInf && l == 0.0f ? 0.0f : l == 0.0f ? __builtin_nanf("") : value_scale / l;
 }
 
-// Sum of v over the lanes up to this one.
-template <int CTRL, int ROWS>
-__device__ __forceinline__ uint32_t dpp_add(uint32_t v) {
-  return v + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
-}
-__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
-  v = dpp_add<0x111, 0xf>(v);         // row_shr 1, 2, 4, 8: within the 16 lanes
-  v = dpp_add<0x112, 0xf>(v);
-  v = dpp_add<0x114, 0xf>(v);
-  v = dpp_add<0x118, 0xf>(v);
-  v = dpp_add<0x142, 0xa>(v);         // lane 15's into rows 1 and 3
-  return dpp_add<0x143, 0xc>(v);      // lane 31's into rows 2 and 3
-}
-
 // A lane's elements of a key row of each tile (D / 32 operand fragments) and of
 // the four value rows of each (D / 16 elements each), as loaded.
 template <int D, int CT>

@@ -77,6 +77,20 @@ __device__ __forceinline__ float wave_max_f32(float v) {
   return fmaxf(fmaxf(readlane_f32(v, 0), readlane_f32(v, 16)), fmaxf(readlane_f32(v, 32), readlane_f32(v, 48)));
 }
 
+// Sum of v over the lanes up to this one.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_add(uint32_t v) {
+  return v + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+  v = dpp_add<0x111, 0xf>(v);         // row_shr 1, 2, 4, 8: within the 16 lanes
+  v = dpp_add<0x112, 0xf>(v);
+  v = dpp_add<0x114, 0xf>(v);
+  v = dpp_add<0x118, 0xf>(v);
+  v = dpp_add<0x142, 0xa>(v);         // lane 15's into rows 1 and 3
+  return dpp_add<0x143, 0xc>(v);      // lane 31's into rows 2 and 3
+}
+
 // Sum over the 8 lanes 8k .. 8k + 7 (every lane of the group gets it).
 __device__ __forceinline__ float oct_sum_f32(float v) {
   v += dpp_f32<kDppXor1>(v);
