@@ -21,7 +21,10 @@
 //
 // The frequencies are formed in 64 bits, as the turns of an angle are; what is
 // left of a turn, at most half of one, is 2^-25 off in f32, and its sine and
-// cosine are f32's.
+// cosine are series in f32 after the quarter turns are taken off.  A key's angles
+// are its lanes' own, four each; a token's query rows share theirs through LDS
+// (with every row's lanes forming them the vector unit was the bound: 16000 tokens
+// of 32 + 16 head rows of 128, 622 MB in and out, 126 us; now ... us).
 #include "hp_serving.h"
 #include "hp_wave.h"
 
@@ -107,35 +110,61 @@ __device__ __forceinline__ Lane lane_of(int l, int rope_dims) {
   return Lane{u0, at0, paired ? u0 + half : at0 + 4, paired};
 }
 
-// Norm (weighted where w is given) of a row of which the lane has x and y.
+// The lane's weights of a norm; none: ones.
+struct Weights {
+  float x[4], y[4];
+  __device__ __forceinline__ Weights(const float *w, const Lane &at) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      x[j] = w ? w[at.at0 + j] : 1.0f;
+      y[j] = w ? w[at.at1 + j] : 1.0f;
+    }
+  }
+};
+
+// Norm of a row of which the lane has x and y.
 template <int D>
-__device__ __forceinline__ void norm_row(float (&x)[4], float (&y)[4], const float *w, const Lane &at, float eps) {
+__device__ __forceinline__ void norm_row(float (&x)[4], float (&y)[4], const Weights &w, float eps) {
   float s = 0.0f;
 #pragma unroll
   for (int j = 0; j < 4; j++) s += x[j] * x[j] + y[j] * y[j];
   const float scale = 1.0f / sqrtf(row_sum<D / 8>(s) / (float)D + eps);
 #pragma unroll
   for (int j = 0; j < 4; j++) {
-    x[j] = x[j] * scale * (w ? w[at.at0 + j] : 1.0f);
-    y[j] = y[j] * scale * (w ? w[at.at1 + j] : 1.0f);
+    x[j] = x[j] * scale * w.x[j];
+    y[j] = y[j] * scale * w.y[j];
   }
 }
 
-// Cosine and sine of the lane's four pairs at a position; sh_turns: turns a
-// position.
-__device__ __forceinline__ void angles_at(const double *sh_turns, const Lane &at, int position, float (&c)[4], float (&s)[4]) {
-#pragma unroll
-  for (int j = 0; j < 4; j++) {
-    const double turns = (double)position * sh_turns[at.u0 + j];
-    sincospif(2.0f * (float)(turns - rint(turns)), &s[j], &c[j]);
-  }
+// Cosine and sine of a part of a turn, -1/2 .. 1/2: the quarter turns, then the
+// series at x = -pi/4 .. pi/4, whose first terms left out are x^11 / 11! < 2^-28
+// and x^12 / 12!.
+__device__ __forceinline__ float2 cos_sin(float part) {
+  const float quarters = part * 4.0f, k = rintf(quarters);
+  const float x = (quarters - k) * 1.57079632679489662f, z = x * x;
+  float s = fmaf(z, 1.0f / 362880.0f, -1.0f / 5040.0f);
+  s = fmaf(z, s, 1.0f / 120.0f);
+  s = fmaf(z, s, -1.0f / 6.0f);
+  s = fmaf(x * z, s, x);
+  float c = fmaf(z, -1.0f / 3628800.0f, 1.0f / 40320.0f);
+  c = fmaf(z, c, -1.0f / 720.0f);
+  c = fmaf(z, c, 1.0f / 24.0f);
+  c = fmaf(z, c, -0.5f);
+  c = fmaf(z, c, 1.0f);
+  const int q = (int)k;
+  const float cosine = q & 1 ? s : c, sine = q & 1 ? c : s;
+  return make_float2(q + 1 & 2 ? -cosine : cosine, q & 2 ? -sine : sine);
 }
-__device__ __forceinline__ void rotate_row(float (&x)[4], float (&y)[4], const float (&c)[4], const float (&s)[4]) {
+__device__ __forceinline__ float2 angle_at(double turns_each, int position) {
+  const double turns = (double)position * turns_each;
+  return cos_sin((float)(turns - rint(turns)));
+}
+__device__ __forceinline__ void rotate_row(float (&x)[4], float (&y)[4], const float2 (&a)[4]) {
 #pragma unroll
   for (int j = 0; j < 4; j++) {
     const float p = x[j], q = y[j];
-    x[j] = p * c[j] - q * s[j];
-    y[j] = p * s[j] + q * c[j];
+    x[j] = p * a[j].x - q * a[j].y;
+    y[j] = p * a[j].y + q * a[j].x;
   }
 }
 
@@ -145,50 +174,85 @@ __device__ __forceinline__ void load_row(const float *row, const Lane &at, float
   y[0] = b.x, y[1] = b.y, y[2] = b.z, y[3] = b.w;
 }
 
+// Tokens whose query rows a workgroup has: a thread an angle.
+template <int D, int NT>
+constexpr int query_tokens() {
+  return NT / (D / 2) > 1 ? NT / (D / 2) : 1;
+}
+
 // NP: passes of a block's rows.  Workgroups 0 .. kv_units - 1 have keys and
 // values, (block slot, KV head, key or value), the others tokens' query rows,
-// (token, part).
+// (tokens, part).
 template <int D, int CT, int NT, int NP>
 __global__ __launch_bounds__(NT) void block_append_kernel(const PagedAppendArgs a, const CacheBlocks b, int kv_units,
                                                           int q_parts) {
   constexpr int kLanes = D / 8, kRows = NT / kLanes;  // of a row, rows at once
-  __shared__ double sh_turns[D / 2];
+  constexpr int kTokens = query_tokens<D, NT>();
+  __shared__ float2 sh_angle[kTokens][D / 2];  // a key's workgroup has its turns there
+  __shared__ int sh_pos[kTokens];
   __shared__ float sh_most[NT / 64], sh_old;
   const int tid = threadIdx.x, sub = tid / kLanes;
   const Lane at = lane_of<D>(tid % kLanes, a.rope_dims);
   const int half = a.rope_dims >> 1;
   const int64_t table_keys = (int64_t)a.c.width << a.c.page_shift;
-  auto fill_turns = [&] {
-    for (int u = tid; u < half; u += NT) {
-      double turns = exp2(a.log2_base * (-2.0 * u / a.rope_dims)) * kInvTwoPi;
-      if (a.freq_factors) turns /= (double)a.freq_factors[u];
-      sh_turns[u] = turns;
-    }
-    __syncthreads();
+  auto turns_of = [&](int u) {
+    const double turns = exp2(a.log2_base * (-2.0 * u / a.rope_dims)) * kInvTwoPi;
+    return a.freq_factors ? turns / (double)a.freq_factors[u] : turns;
   };
 
   if ((int)blockIdx.x >= kv_units) {  // query rows
-    const int unit = blockIdx.x - kv_units, t = unit / q_parts;
-    int seq = t, pos = -1;
-    if (a.offsets) {
-      seq = packed_sequence_of(a.offsets, a.c.sequences, t);
-      if (seq < a.c.sequences) {
-        const int begin = a.offsets[seq], end = a.offsets[seq + 1];
-        if (t >= begin && t < end) pos = append_position(a.c.lengths[seq], (int64_t)end - t, a.c.page_shift, a.c.width);
+    const int unit = blockIdx.x - kv_units, t0 = unit / q_parts * kTokens, part = unit % q_parts;
+    const int tokens = min(kTokens, a.tokens - t0);
+    // row (t, h) of the thread, `step` rows on from one to the next; the first are on
+    // their way before the positions are known
+    const int step = q_parts * kRows, step_t = step / a.nq, step_h = step - step_t * a.nq;
+    int t = (part * kRows + sub) / a.nq, h = part * kRows + sub - t * a.nq;
+    float x[4], y[4], next_x[4], next_y[4];
+    auto load = [&] {  // (behind the last row: another of the last token's)
+      load_row(a.q + (t0 + min(t, tokens - 1)) * a.q_stride + (int64_t)h * D, at, next_x, next_y);
+    };
+    load();
+    const Weights weights(a.q_norm, at);
+    for (int i = tid >> 6; i < tokens; i += NT / 64) {  // a wave a token
+      const int t = t0 + i;
+      int seq = t, pos = -1;
+      if (a.offsets) {
+        seq = packed_sequence_of(a.offsets, a.c.sequences, t);
+        if (seq < a.c.sequences) {
+          const int begin = a.offsets[seq], end = a.offsets[seq + 1];
+          if (t >= begin && t < end) pos = append_position(a.c.lengths[seq], (int64_t)end - t, a.c.page_shift, a.c.width);
+        }
+      } else {
+        pos = append_position(a.c.lengths[seq], 1, a.c.page_shift, a.c.width);
       }
-    } else {
-      pos = append_position(a.c.lengths[seq], 1, a.c.page_shift, a.c.width);
+      if ((tid & 63) == 0) sh_pos[i] = pos;
     }
-    if (pos < 0) return;  // (the same for the workgroup)
-    fill_turns();
-    float c[4], s[4];
-    if (at.paired) angles_at(sh_turns, at, pos, c, s);
-    for (int r = unit % q_parts * kRows + sub; r < a.nq; r += q_parts * kRows) {  // (the same for the lanes of a row)
-      float x[4], y[4];
-      load_row(a.q + t * a.q_stride + (int64_t)r * D, at, x, y);
-      if (a.q_norm) norm_row<D>(x, y, a.q_norm, at, a.eps);
-      if (at.paired) rotate_row(x, y, c, s);
-      const int64_t o = ((int64_t)t * a.nq + r) * D;
+    __syncthreads();
+    if (half > 0) {
+      for (int i = tid; i < tokens * (D / 2); i += NT) {
+        const int t = i / (D / 2), u = i - t * (D / 2);
+        if (u < half) sh_angle[t][u] = angle_at(turns_of(u), sh_pos[t]);
+      }
+      __syncthreads();
+    }
+    while (t < tokens) {  // (the same for the lanes of a row)
+#pragma unroll
+      for (int j = 0; j < 4; j++) x[j] = next_x[j], y[j] = next_y[j];
+      const int i = t;
+      const int64_t o = ((int64_t)(t0 + t) * a.nq + h) * D;
+      t += step_t;
+      h += step_h;
+      if (h >= a.nq) {
+        t++;
+        h -= a.nq;
+      }
+      load();
+      if (sh_pos[i] < 0) continue;
+      if (a.q_norm) norm_row<D>(x, y, weights, a.eps);
+      if (at.paired) {
+        const float2 angle[4] = {sh_angle[i][at.u0], sh_angle[i][at.u0 + 1], sh_angle[i][at.u0 + 2], sh_angle[i][at.u0 + 3]};
+        rotate_row(x, y, angle);
+      }
       store4(a.q_out, o + at.at0, a.out_type, x);
       store4(a.q_out, o + at.at1, a.out_type, y);
     }
@@ -230,19 +294,25 @@ __global__ __launch_bounds__(NT) void block_append_kernel(const PagedAppendArgs 
   float *scales = is_key ? b.key_scales : b.value_scales;
   float old = 0.0f;  // (read by the thread that writes it in the end)
   if (tid == 0) old = scales[scale_at];
-  if (is_key && half > 0) fill_turns();
+  double *sh_turns = reinterpret_cast<double *>(&sh_angle[0][0]);
+  if (is_key && half > 0) {
+    for (int u = tid; u < half; u += NT) sh_turns[u] = turns_of(u);
+    __syncthreads();
+  }
 
-  const float *w = is_key ? a.k_norm : nullptr;
+  const bool norm = is_key ? a.k_norm != nullptr : a.norm_values != 0;
+  const Weights weights(is_key ? a.k_norm : nullptr, at);
   void *out = is_key ? a.k_out : a.v_out;
   float most = 0.0f;
 #pragma unroll
   for (int i = 0; i < NP; i++) {
     const int64_t t = row0 + i * kRows + sub;
-    if (w || (!is_key && a.norm_values)) norm_row<D>(x[i], y[i], w, at, a.eps);
+    if (norm) norm_row<D>(x[i], y[i], weights, a.eps);
     if (is_key && at.paired) {
-      float c[4], s[4];
-      angles_at(sh_turns, at, n.first + i * kRows + sub, c, s);
-      rotate_row(x[i], y[i], c, s);
+      float2 angle[4];
+#pragma unroll
+      for (int j = 0; j < 4; j++) angle[j] = angle_at(sh_turns[at.u0 + j], n.first + i * kRows + sub);
+      rotate_row(x[i], y[i], angle);
     }
     if (i * kRows + sub < rows && t >= 0 && t < a.tokens) {
       if (out) {
@@ -312,10 +382,12 @@ hipError_t launch(const PagedAppendArgs &a, const CacheBlocks &b, int num_cus, h
   constexpr int kRows = NT / (D / 8);
   const int64_t slots = a.offsets ? touched_blocks(a.tokens, a.c.sequences, 1 << b.shift) : a.c.sequences;
   const int64_t kv_units = 2 * slots * a.c.nkv;
-  int q_parts = (a.nq + kRows - 1) / kRows;
-  const int most = (4 * num_cus * 256 / NT + a.tokens - 1) / a.tokens;  // sixteen waves a CU
+  constexpr int kTokens = query_tokens<D, NT>();
+  const int q_groups = (a.tokens + kTokens - 1) / kTokens;
+  int q_parts = (kTokens * a.nq + kRows - 1) / kRows;
+  const int most = (4 * num_cus * 256 / NT + q_groups - 1) / q_groups;  // sixteen waves a CU
   q_parts = q_parts < 1 ? 1 : q_parts > most ? most : q_parts;
-  const int64_t grid = kv_units + (a.nq > 0 ? (int64_t)a.tokens * q_parts : 0);
+  const int64_t grid = kv_units + (a.nq > 0 ? (int64_t)q_groups * q_parts : 0);
   if (grid >> 31) return hipErrorInvalidValue;
   hipLaunchKernelGGL((block_append_kernel<D, CT, NT, NP>), dim3((unsigned)grid), dim3(NT), 0, s, a, b, (int)kv_units,
                      q_parts);
