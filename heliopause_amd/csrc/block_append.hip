@@ -23,8 +23,8 @@
 // left of a turn, at most half of one, is 2^-25 off in f32, and its sine and
 // cosine are series in f32 after the quarter turns are taken off.  A key's angles
 // are its lanes' own, four each; a token's query rows share theirs through LDS
-// (with every row's lanes forming them the vector unit was the bound: 16000 tokens
-// of 32 + 16 head rows of 128, 622 MB in and out, 126 us; now ... us).
+// (a quarter of the vector unit's work with every row's lanes forming them).
+// 16000 tokens of 32 + 16 head rows of 128, 622 MB in and out: 124 us, 5.0 TB/s.
 #include "hp_serving.h"
 #include "hp_wave.h"
 

@@ -253,21 +253,25 @@ __global__ __launch_bounds__(kThreads) void plan_deal_kernel(const PagePlanArgs 
 
 constexpr int kOneThreads = 1024, kOneWaves = kOneThreads / 64, kOneAtOnce = 4;
 
-// Sum over the threads before, and over all.
-__device__ __forceinline__ uint64_t block_scan(uint64_t v, uint64_t *sh, uint64_t *all) {
+// Two sums over the threads before, and over all.
+__device__ __forceinline__ void block_scan(uint64_t x, uint64_t y, uint64_t (*sh)[2], uint64_t (&before)[2], uint64_t (&all)[2]) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const uint64_t to = wave_scan(v);
-  __syncthreads();
-  if (lane == 63) sh[wave] = to;
-  __syncthreads();
-  uint64_t before = to - v, sum = 0;
-#pragma unroll
-  for (int w = 0; w < kOneWaves; w++) {
-    before += w < wave ? sh[w] : 0;
-    sum += sh[w];
+  const uint64_t x_to = wave_scan(x), y_to = wave_scan(y);
+  if (lane == 63) {
+    sh[wave][0] = x_to;
+    sh[wave][1] = y_to;
   }
-  *all = sum;
-  return before;
+  __syncthreads();
+  before[0] = x_to - x;
+  before[1] = y_to - y;
+  all[0] = all[1] = 0;
+#pragma unroll
+  for (int w = 0; w < kOneWaves; w++)
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      before[i] += w < wave ? sh[w][i] : 0;
+      all[i] += sh[w][i];
+    }
 }
 
 // The largest s in 0 .. n - 1 with at[s] <= i (at[0] = 0; n <= 1024).
@@ -282,7 +286,7 @@ __device__ __forceinline__ int find(const int *at, int n, int i) {
 // The entries of all sequences' ranges lie end to end, thread after thread, so
 // that one count over them ranks them all.
 __global__ __launch_bounds__(kOneThreads) void plan_one_kernel(const PagePlanArgs a) {
-  __shared__ uint64_t sh_scan[kOneWaves];
+  __shared__ uint64_t sh_scan[kOneWaves][2];
   __shared__ int sh_old[kOneThreads], sh_first[kOneThreads], sh_back[kOneThreads], sh_want[kOneThreads],
       sh_rows[kOneThreads + 1], sh_missing[kOneThreads];
   __shared__ int sh_counts[kOneAtOnce][kOneWaves];
@@ -290,10 +294,10 @@ __global__ __launch_bounds__(kOneThreads) void plan_one_kernel(const PagePlanArg
   PlanSpan p = {0, 0, 0, 0, 0};
   if (tid < S) p = span_of(a, tid);
   int top = min(max(*a.free_count, 0), a.page_count);
-  uint64_t ranges = 0, tokens = 0;
   const int fresh = (int)(p.fresh > 0x7fffffff ? 0x7fffffff : p.fresh);
-  const uint64_t range_at = block_scan((uint64_t)(uint32_t)p.back << 32 | (uint32_t)(p.last - p.first), sh_scan, &ranges);
-  const uint64_t row_at = block_scan((uint32_t)fresh, sh_scan, &tokens);
+  uint64_t before[2], all[2];
+  block_scan((uint64_t)(uint32_t)p.back << 32 | (uint32_t)(p.last - p.first), (uint32_t)fresh, sh_scan, before, all);
+  const uint64_t range_at = before[0], row_at = before[1], ranges = all[0], tokens = all[1];
   sh_old[tid] = p.old;
   sh_first[tid] = p.first;
   sh_back[tid] = (int)(range_at >> 32);
