@@ -3257,15 +3257,15 @@ int32_t hp_hip_page_plan_device(const hp_hip_page_plan_t *plan, void *stream) {
       [&](State &s, hipStream_t strm) -> int32_t {
         if (a.sequences == 0) return HP_OK;
         void *scratch = nullptr;
-        const bool small = page_plan_is_small(a);
-        if (!small) {
+        const int launches = page_plan_launches(a);
+        if (launches > 1) {
           int32_t rc = stream_scratch(strm, kScratchPlan, page_plan_scratch_bytes(a), &scratch);
           if (rc != HP_OK) return rc;
         }
         hipEvent_t e = prof_begin(strm);
         HP_HIP_TRY(launch_page_plan(a, scratch, strm));
         prof_end(HP_KERNEL_ATTENTION, e, strm);
-        s.launches += small ? 1 : 3 + (a.keep_from != nullptr);
+        s.launches += launches;
         return HP_OK;
       });
 }

@@ -106,7 +106,7 @@ struct PagePlanArgs {
   int64_t *slots;
   int sequences, width, page_shift, page_count, rows;
 };
-bool page_plan_is_small(const PagePlanArgs &a);  // one launch, no scratch
+int page_plan_launches(const PagePlanArgs &a);  // one: no scratch
 size_t page_plan_scratch_bytes(const PagePlanArgs &a);
 hipError_t launch_page_plan(const PagePlanArgs &a, void *scratch, hipStream_t s);
 

@@ -17,22 +17,30 @@ namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr int kScanThreads = 1024;
+constexpr int kAtOnce = 8;  // entries that a lane has on their way
 
 // Scratch: what one launch leaves for the next.
 struct PlanState {
-  int free_before, free_with;  // entries of the stack, before and with those given back
+  int free_with, free_after;  // entries of the stack, with those given back and in the end
   int pad[2];
 };
 struct PlanRow {
-  int old, fresh, back_at, want_at;  // (counts until they are summed up)
+  int old, fresh, back, want;  // pages that go back, that are wanted
+};
+struct PlanAt {
+  int back, want;  // the same of the sequences before
 };
 // In `old` and `fresh`, which are not negative: some of the new pages' entries want
 // a page and some have one; all have one.
 constexpr int kGaps = 1 << 31, kNamed = 1 << 31;
 __device__ __forceinline__ PlanRow *rows_of(PlanState *s) { return reinterpret_cast<PlanRow *>(s + 1); }
-__device__ __forceinline__ int *offsets_of(PlanState *s, int sequences) {
-  return reinterpret_cast<int *>(rows_of(s) + sequences);
+__device__ __forceinline__ PlanAt *places_of(PlanState *s, int sequences) {
+  return reinterpret_cast<PlanAt *>(rows_of(s) + sequences);
 }
+__device__ __forceinline__ int *offsets_of(PlanState *s, int sequences) {
+  return reinterpret_cast<int *>(places_of(s, sequences) + sequences);
+}
+__device__ __forceinline__ int free_before(const PagePlanArgs &a) { return min(max(*a.free_count, 0), a.page_count); }
 
 __device__ __forceinline__ PlanSpan span_of(const PagePlanArgs &a, int s) {
   const int length = a.lengths[s], keep = a.keep_from ? a.keep_from[s] : 0;
@@ -56,8 +64,20 @@ __device__ __forceinline__ void count_sequence(const PagePlanArgs &a, PlanState 
   const PlanSpan p = span_of(a, s);
   const int *table = a.pages + (int64_t)s * a.width;
   int back = 0, want = 0;
-  for (int i = lane; i < p.back; i += 64) back += page_or_none(table[i], a.page_count) >= 0;
-  for (int i = p.first + lane; i < p.last; i += 64) want += i < p.back || page_or_none(table[i], a.page_count) < 0;
+  for (int i0 = lane; i0 < p.back; i0 += 64 * kAtOnce) {
+#pragma unroll
+    for (int j = 0; j < kAtOnce; j++) {
+      const int i = i0 + 64 * j, entry = table[min(i, p.back - 1)];
+      back += i < p.back && page_or_none(entry, a.page_count) >= 0;
+    }
+  }
+  for (int i0 = p.first + lane; i0 < p.last; i0 += 64 * kAtOnce) {
+#pragma unroll
+    for (int j = 0; j < kAtOnce; j++) {
+      const int i = i0 + 64 * j, entry = table[min(i, p.last - 1)];
+      want += i < p.last && (i < p.back || page_or_none(entry, a.page_count) < 0);
+    }
+  }
   const uint64_t both = wave_scan((uint64_t)(uint32_t)back << 32 | (uint32_t)want);
   if (lane == 63) {
     want = (int)(uint32_t)both;
@@ -71,13 +91,14 @@ __device__ __forceinline__ void count_sequence(const PagePlanArgs &a, PlanState 
 template <int THREADS>
 __device__ void scan_sequences(const PagePlanArgs &a, PlanState *st) {
   __shared__ uint64_t sh_pages[THREADS / 64], sh_tokens[THREADS / 64];
-  PlanRow *rows = rows_of(st);
+  const PlanRow *rows = rows_of(st);
+  PlanAt *places = places_of(st, a.sequences);
   int *offsets = offsets_of(st, a.sequences);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int run = (a.sequences + THREADS - 1) / THREADS, begin = min(tid * run, a.sequences), end = min(begin + run, a.sequences);
   uint64_t pages = 0, tokens = 0;  // (given back, wanted) of 2^31 at most each
   for (int s = begin; s < end; s++) {
-    pages += (uint64_t)(uint32_t)rows[s].back_at << 32 | (uint32_t)rows[s].want_at;
+    pages += (uint64_t)(uint32_t)rows[s].back << 32 | (uint32_t)rows[s].want;
     tokens += (uint32_t)(rows[s].fresh & ~kNamed);
   }
   const uint64_t pages_to = wave_scan(pages), tokens_to = wave_scan(tokens);
@@ -95,27 +116,24 @@ __device__ void scan_sequences(const PagePlanArgs &a, PlanState *st) {
   }
   for (int s = begin; s < end; s++) {
     const PlanRow r = rows[s];
-    rows[s].back_at = (int)(p >> 32);
-    rows[s].want_at = (int)(uint32_t)p;
+    places[s] = PlanAt{(int)(p >> 32), (int)(uint32_t)p};
     const int at = (int)(t < 0x7fffffff ? t : 0x7fffffff);
     offsets[s] = at;
     if (a.offsets) a.offsets[s] = at;
     const int fresh = r.fresh & ~kNamed;
     const int64_t length = (int64_t)(r.old & ~kGaps) + fresh;
     a.lengths_out[s] = (int)(length < 0x7fffffff ? length : 0x7fffffff);
-    p += (uint64_t)(uint32_t)r.back_at << 32 | (uint32_t)r.want_at;
+    p += (uint64_t)(uint32_t)r.back << 32 | (uint32_t)r.want;
     t += (uint32_t)fresh;
   }
   if (tid == 0) {
     const int at = (int)(rows_all < 0x7fffffff ? rows_all : 0x7fffffff);
     offsets[a.sequences] = at;
     if (a.offsets) a.offsets[a.sequences] = at;
-    const int before = min(max(*a.free_count, 0), a.page_count);
-    const int64_t with = (int64_t)before + (int64_t)(all >> 32), want = (int64_t)(uint32_t)all;
+    const int64_t with = free_before(a) + (int64_t)(all >> 32), want = (int64_t)(uint32_t)all;
     const int top = (int)(with < a.page_count ? with : a.page_count);
-    st->free_before = before;
     st->free_with = top;
-    *a.free_count = want < top ? top - (int)want : 0;
+    st->free_after = want < top ? top - (int)want : 0;
   }
 }
 
@@ -128,26 +146,53 @@ __global__ __launch_bounds__(kScanThreads) void plan_scan_kernel(const PagePlanA
   scan_sequences<kScanThreads>(a, st);
 }
 
-// One sequence's pages onto the stack, by a wave.
-__device__ __forceinline__ void give_back(const PagePlanArgs &a, const PlanState *st, const PlanRow &r, int s) {
+// One sequence's pages onto the stack behind `at` others, by a wave.
+__device__ __forceinline__ void give_back(const PagePlanArgs &a, int64_t at, int s) {
   const int lane = threadIdx.x & 63;
   const int keep = a.keep_from[s], back = plan_span(0, 0, keep, a.page_shift, a.width).back;
   int *table = a.pages + (int64_t)s * a.width;
-  int64_t at = (int64_t)st->free_before + r.back_at;
-  for (int i0 = 0; i0 < back; i0 += 64) {
-    const int i = i0 + lane;
-    const int entry = i < back ? table[i] : -1, page = page_or_none(entry, a.page_count);
-    const uint64_t named = __ballot(page >= 0);
-    const int64_t to = at + __popcll(named & ((1ull << lane) - 1));
-    if (page >= 0 && to < a.page_count) a.free[to] = page;
-    if (i < back && entry != -1) table[i] = -1;
-    at += __popcll(named);
+  at += free_before(a);
+  for (int i0 = lane; i0 - lane < back; i0 += 64 * kAtOnce) {
+    int entry[kAtOnce];
+#pragma unroll
+    for (int j = 0; j < kAtOnce; j++) entry[j] = table[min(i0 + 64 * j, back - 1)];
+#pragma unroll
+    for (int j = 0; j < kAtOnce; j++) {
+      const bool in = i0 + 64 * j < back;
+      const int page = in ? page_or_none(entry[j], a.page_count) : -1;
+      const uint64_t named = __ballot(page >= 0);
+      const int64_t to = at + __popcll(named & ((1ull << lane) - 1));
+      if (page >= 0 && to < a.page_count) a.free[to] = page;
+      if (in && entry[j] != -1) table[i0 + 64 * j] = -1;
+      at += __popcll(named);
+    }
   }
 }
 
+// SUM: the sums are not there yet; each workgroup adds up what the sequences
+// before its own give back, and one more has the scan for the next launch.
+template <bool SUM>
 __global__ __launch_bounds__(kThreads) void plan_back_kernel(const PagePlanArgs a, PlanState *__restrict__ st) {
-  const int s = blockIdx.x * kWaves + (threadIdx.x >> 6);
-  if (s < a.sequences) give_back(a, st, rows_of(st)[s], s);
+  const int s0 = blockIdx.x * kWaves, s = s0 + (threadIdx.x >> 6);
+  if (!SUM) {
+    if (s < a.sequences) give_back(a, places_of(st, a.sequences)[s].back, s);
+    return;
+  }
+  if (blockIdx.x == gridDim.x - 1) {
+    scan_sequences<kThreads>(a, st);
+    return;
+  }
+  __shared__ uint64_t sh_sum[kWaves];
+  const PlanRow *rows = rows_of(st);
+  uint64_t before = 0;
+  for (int i = threadIdx.x; i < s0; i += kThreads) before += (uint32_t)rows[i].back;
+  before = wave_scan(before);
+  if ((threadIdx.x & 63) == 63) sh_sum[threadIdx.x >> 6] = before;
+  __syncthreads();
+  before = 0;
+  for (int w = 0; w < kWaves; w++) before += sh_sum[w];
+  for (int i = s0; i < s && i < a.sequences; i++) before += (uint32_t)rows[i].back;
+  if (s < a.sequences) give_back(a, (int64_t)before, s);
 }
 
 // A row's place: position p of sequence s (-1: none) on `page`.
@@ -164,7 +209,7 @@ __device__ __forceinline__ int page_at(const PagePlanArgs &a, int s, int64_t p) 
 
 // One sequence's new pages off the stack, by a wave; where some entries have
 // theirs already, its rows too.
-__device__ __forceinline__ void deal(const PagePlanArgs &a, const PlanState *st, const int *offsets, PlanRow r, int s) {
+__device__ __forceinline__ void deal(const PagePlanArgs &a, const PlanState *st, const int *offsets, PlanRow r, int want_at, int s) {
   const int lane = threadIdx.x & 63;
   const bool gaps = (r.old & kGaps) != 0, named = (r.fresh & kNamed) != 0;
   if (named) {
@@ -174,19 +219,27 @@ __device__ __forceinline__ void deal(const PagePlanArgs &a, const PlanState *st,
   r.old &= ~kGaps;
   const PlanSpan p = plan_span(r.old, r.fresh, 0, a.page_shift, a.width);
   int *table = a.pages + (int64_t)s * a.width;
-  int64_t at = (int64_t)st->free_with - 1 - (uint32_t)r.want_at;
+  int64_t at = (int64_t)st->free_with - 1 - (uint32_t)want_at;
   int missing = 0;
-  for (int i0 = p.first; i0 < p.last; i0 += 64) {
-    const int i = i0 + lane;
-    const bool want = i < p.last && (!gaps || page_or_none(table[i], a.page_count) < 0);
-    const uint64_t wanted = __ballot(want);
-    const int64_t from = at - __popcll(wanted & ((1ull << lane) - 1));
-    if (want) {
-      const int page = from >= 0 ? page_or_none(a.free[from], a.page_count) : -1;
-      table[i] = page;
-      missing += page < 0;
+  for (int i0 = p.first + lane; i0 - lane < p.last; i0 += 64 * kAtOnce) {
+    int entry[kAtOnce], page[kAtOnce];
+    bool want[kAtOnce];
+#pragma unroll
+    for (int j = 0; j < kAtOnce; j++) entry[j] = gaps ? table[min(i0 + 64 * j, p.last - 1)] : -1;
+#pragma unroll
+    for (int j = 0; j < kAtOnce; j++) {
+      want[j] = i0 + 64 * j < p.last && page_or_none(entry[j], a.page_count) < 0;
+      const uint64_t wanted = __ballot(want[j]);
+      const int64_t from = at - __popcll(wanted & ((1ull << lane) - 1));
+      page[j] = want[j] && from >= 0 ? a.free[from] : -1;
+      at -= __popcll(wanted);
     }
-    at -= __popcll(wanted);
+#pragma unroll
+    for (int j = 0; j < kAtOnce; j++) {
+      page[j] = page_or_none(page[j], a.page_count);
+      if (want[j]) table[i0 + 64 * j] = page[j];
+      missing += want[j] && page[j] < 0;
+    }
   }
   const uint64_t all = wave_scan((uint64_t)(uint32_t)missing);
   if (lane == 63 && a.missing) a.missing[s] = (int)all;
@@ -197,11 +250,11 @@ __device__ __forceinline__ void deal(const PagePlanArgs &a, const PlanState *st,
     put_row(a, (int)(row0 + i), s, r.old + i, page_at(a, s, r.old + i));
 }
 
-// The row's sequence: 64 rows of a wave mostly have one.
-__device__ __forceinline__ int sequence_of(const PagePlanArgs &a, const int *offsets, int t0, int t) {
-  if (!a.fresh) return t;
-  int lo = packed_sequence_of(offsets, a.sequences, t0);
-  if (__any(lo < a.sequences && offsets[min(lo, a.sequences - 1) + 1] <= t)) {
+// Row t's sequence, from that of a row before it: mostly the same, or the next.
+__device__ __forceinline__ int sequence_from(const PagePlanArgs &a, const int *offsets, int lo, int t) {
+  for (int step = 0; lo < a.sequences && offsets[lo + 1] <= t; step++) {
+    lo++;
+    if (step < 2) continue;
     int n = a.sequences;  // lo .. n: the first whose end is past the row
     while (lo < n) {
       const int mid = (lo + n) >> 1;
@@ -210,9 +263,12 @@ __device__ __forceinline__ int sequence_of(const PagePlanArgs &a, const int *off
       else
         n = mid;
     }
+    break;
   }
   return lo;
 }
+
+constexpr int kRowsEach = 4;
 
 // The first workgroups deal, a wave a sequence; the others have the rows.  Where
 // all of a sequence's new pages come off the stack the i-th is known without the
@@ -221,32 +277,44 @@ __global__ __launch_bounds__(kThreads) void plan_deal_kernel(const PagePlanArgs 
                                                              int deals) {
   PlanState *st = const_cast<PlanState *>(st_in);
   const int *offsets = offsets_of(st, a.sequences);
+  const PlanAt *places = places_of(st, a.sequences);
   if ((int)blockIdx.x < deals) {
     const int s = blockIdx.x * kWaves + (threadIdx.x >> 6);
-    if (s < a.sequences) deal(a, st, offsets, rows_of(st)[s], s);
+    if (s < a.sequences) deal(a, st, offsets, rows_of(st)[s], places[s].want, s);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *a.free_count = st->free_after;
     return;
   }
-  const int t = (blockIdx.x - deals) * kThreads + threadIdx.x, t0 = t & ~63;
+  // a wave has 64 * kRowsEach rows
+  const int t0 = ((blockIdx.x - deals) * kWaves + (threadIdx.x >> 6)) * 64 * kRowsEach, lane = threadIdx.x & 63;
   if (t0 >= a.rows) return;
-  const int s = sequence_of(a, offsets, t0, t);
-  if (t >= a.rows) return;
-  const PlanRow r = rows_of(st)[min(s, a.sequences - 1)];
-  const bool named = (r.fresh & kNamed) != 0;
-  if (s >= a.sequences || (r.fresh & ~kNamed) == 0) {
-    put_row(a, t, -1, 0, -1);
-    return;
+  int at = a.fresh ? packed_sequence_of(offsets, a.sequences, t0) : 0;
+#pragma unroll
+  for (int j = 0; j < kRowsEach; j++) {
+    const int t = t0 + 64 * j + lane;
+    if (t >= a.rows) continue;
+    int s = t;
+    if (a.fresh) {
+      at = sequence_from(a, offsets, at, t);
+      s = at;
+    }
+    const PlanRow r = rows_of(st)[min(s, a.sequences - 1)];
+    const bool named = (r.fresh & kNamed) != 0;
+    if (s >= a.sequences || (r.fresh & ~kNamed) == 0) {
+      put_row(a, t, -1, 0, -1);
+      continue;
+    }
+    if (r.old & kGaps) continue;  // (the dealing wave's)
+    const int64_t p = (int64_t)r.old + (a.fresh ? t - offsets[s] : 0), i = p >> a.page_shift;
+    const int first = plan_span(r.old, 0, 0, a.page_shift, a.width).first;
+    int page = -1;
+    if (named || i < first) {
+      page = page_at(a, s, p);
+    } else if (i < a.width) {
+      const int64_t from = (int64_t)st->free_with - 1 - (uint32_t)places[s].want - (i - first);
+      page = from >= 0 ? page_or_none(a.free[from], a.page_count) : -1;
+    }
+    put_row(a, t, s, p, page);
   }
-  if (r.old & kGaps) return;  // (the dealing wave's)
-  const int64_t p = (int64_t)r.old + (a.fresh ? t - offsets[s] : 0), i = p >> a.page_shift;
-  const int first = plan_span(r.old, 0, 0, a.page_shift, a.width).first;
-  int page = -1;
-  if (named || i < first) {
-    page = page_at(a, s, p);
-  } else if (i < a.width) {
-    const int64_t from = (int64_t)st->free_with - 1 - (uint32_t)r.want_at - (i - first);
-    page = from >= 0 ? page_or_none(a.free[from], a.page_count) : -1;
-  }
-  put_row(a, t, s, p, page);
 }
 
 // ---- small batches: everything in one workgroup ----------------------------------
@@ -396,28 +464,36 @@ __global__ __launch_bounds__(kOneThreads) void plan_one_kernel(const PagePlanArg
 
 }  // namespace
 
-bool page_plan_is_small(const PagePlanArgs &a) {
-  return a.sequences <= kOneThreads && (int64_t)a.sequences * a.width <= 1 << 16 && a.rows <= 1 << 13;
+int page_plan_launches(const PagePlanArgs &a) {
+  if (a.sequences <= kOneThreads && (int64_t)a.sequences * a.width <= 1 << 16 && a.rows <= 1 << 13) return 1;
+  return a.keep_from && a.sequences > 4096 ? 4 : 3;
 }
 
 size_t page_plan_scratch_bytes(const PagePlanArgs &a) {
-  return sizeof(PlanState) + (size_t)a.sequences * sizeof(PlanRow) + ((size_t)a.sequences + 1) * sizeof(int);
+  return sizeof(PlanState) + (size_t)a.sequences * (sizeof(PlanRow) + sizeof(PlanAt)) + ((size_t)a.sequences + 1) * sizeof(int);
 }
 
 hipError_t launch_page_plan(const PagePlanArgs &a, void *scratch, hipStream_t s) {
-  if (a.sequences < 1 || a.width < 1 || a.page_count < 1 || (!scratch && !page_plan_is_small(a)) || (!a.fresh && a.rows > a.sequences))
+  if (a.sequences < 1 || a.width < 1 || a.page_count < 1 || (!scratch && page_plan_launches(a) > 1) || (!a.fresh && a.rows > a.sequences))
     return hipErrorInvalidValue;
   // one launch where one workgroup has a few turns of work (201 sequences, some 45
   // entries of each to look through: 9.3 us a call, 18.6 in several launches)
-  if (page_plan_is_small(a)) {
+  if (page_plan_launches(a) == 1) {
     hipLaunchKernelGGL(plan_one_kernel, dim3(1), dim3(kOneThreads), 0, s, a);
     return hipGetLastError();
   }
   PlanState *st = static_cast<PlanState *>(scratch);
-  const int by_sequence = (a.sequences + kWaves - 1) / kWaves, by_row = (a.rows + kThreads - 1) / kThreads;
+  const int by_sequence = (a.sequences + kWaves - 1) / kWaves,
+            by_row = (int)(((int64_t)a.rows + kThreads * kRowsEach - 1) / (kThreads * kRowsEach));
   hipLaunchKernelGGL(plan_count_kernel, dim3(by_sequence), dim3(kThreads), 0, s, a, st);
-  hipLaunchKernelGGL(plan_scan_kernel, dim3(1), dim3(kScanThreads), 0, s, a, st);
-  if (a.keep_from) hipLaunchKernelGGL(plan_back_kernel, dim3(by_sequence), dim3(kThreads), 0, s, a, st);
+  // (to 4096 sequences the sums are a launch's overhead: 4 us of the 18 of 256
+  // sequences and 700001 rows)
+  if (page_plan_launches(a) == 3 && a.keep_from) {
+    hipLaunchKernelGGL(plan_back_kernel<true>, dim3(by_sequence + 1), dim3(kThreads), 0, s, a, st);
+  } else {
+    hipLaunchKernelGGL(plan_scan_kernel, dim3(1), dim3(kScanThreads), 0, s, a, st);
+    if (a.keep_from) hipLaunchKernelGGL(plan_back_kernel<false>, dim3(by_sequence), dim3(kThreads), 0, s, a, st);
+  }
   hipLaunchKernelGGL(plan_deal_kernel, dim3(by_sequence + by_row), dim3(kThreads), 0, s, a, st, by_sequence);
   return hipGetLastError();
 }

@@ -208,6 +208,23 @@ def test_plans_of_many_sequences(hip, L, S):
     run_plan(L, pages, lengths, None, keep, free, S // 2, 16, count, S)
 
 
+@pytest.mark.parametrize("S,rows", [(40, 9000), (700, 20000), (5000, 30000)])
+@pytest.mark.parametrize("back", [False, True])
+def test_large_plans(hip, L, S, rows, back):
+    """More rows than one workgroup takes, long rows of the table, sequences without new tokens, with gaps in their tables,
+    and with all their pages there; few free pages in the end."""
+    rng = np.random.default_rng(S)
+    lengths = rng.integers(0, 3000, S)
+    pages, free, count = table(rng, lengths, 16, 260, rows // 16)
+    weight = rng.random(S) * (rng.random(S) < 0.6)
+    new = rng.multinomial(rows, weight / weight.sum())
+    keep = np.where(rng.random(S) < 0.3, -1, rng.integers(0, 2000, S)) if back else None
+    first = run_plan(L, pages, lengths, new, keep, free, rows // 16, 16, count, rows + 100)
+    again = first["pages"].copy()
+    again[rng.random(again.shape) < 0.02] = -1  # some gaps
+    run_plan(L, again, lengths, new, keep, first["free"], int(first["free_count"]), 16, count, rows + 100)
+
+
 def test_plans_with_bad_entries(hip, L):
     """Entries and free pages that name no page, gaps, tokens past the table's end, a stack that overflows or has a bad
     count; nothing outside the arrays is touched."""
