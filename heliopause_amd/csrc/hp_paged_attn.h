@@ -430,6 +430,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(const PagedAttn
       if (q4 == 0) sh_most[wave][c16] = most;
     }
     __syncthreads();
+    bool lifted;
     float factor, lift;  // of a score, to base 2: their product
     {
       float most = sh_most[0][c16];
@@ -449,6 +450,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(const PagedAttn
       const bool far = whole >= 0x1p126;
       factor = (float)(far ? whole * 0x1p-126 : whole);
       lift = far ? 0x1p126f : 1.0f;
+      lifted = __any(far);
       const bool rest = c16 >= kHeads;
 #pragma unroll
       for (int i = 0; i < kMine; i++) {
@@ -522,7 +524,8 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(const PagedAttn
       for (int j = 0; j < kKeys; j++) {
         const float v = s[j >> 2][j & 3];
         const float all = v + dpp_f32<kDppRor8>(v);
-        x[j] = (kScales ? all * key_scale[j >> 2] : all) * factor * lift;
+        x[j] = (kScales ? all * key_scale[j >> 2] : all) * factor;
+        if (MODE == kWhole || lifted) x[j] *= lift;
       }
       has_key = has_key || !edge;
       if (edge) {  // the same for the wave
@@ -536,25 +539,27 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(const PagedAttn
           for (int w = 0; w < T::kValueWords; w++) t.v[j][w] = off ? 0u : t.v[j][w];
         }
       }
-      // a value scale f 2^e, f in [1, 2): the maximum is that of x + e, so that the
-      // weights f 2^(x + e - m) of the stored values are within range whatever the
-      // blocks' scales are; the normaliser's 2^(x - m) are at most 2^100
-      float part[kTiles], e[kTiles];
+      // a value scale s >= 2^e: the maximum is that of x + e, so that the weights
+      // s 2^(x - m) of the stored values are within range whatever the blocks' scales
+      // are.  2^(x - m) itself is at most 2^100, and below f32 only where the weight
+      // is less than 2^-26 of the largest, bias and all
+      float most = kNegInf;
+      if (kScales) {
 #pragma unroll
-      for (int h = 0; h < kTiles; h++) {
-        part[h] = 1.0f;
-        e[h] = 0.0f;
-        if (!kScales || page[h] < 0) continue;
-        const uint32_t bits = __builtin_bit_cast(uint32_t, value_scale[h]);
-        const int exponent = (int)(bits >> 23 & 255) - 127;
-        part[h] = exponent == 128 ? value_scale[h]  // (an infinity or NaN)
-                  : exponent < -100 ? 0.0f
-                                    : __builtin_bit_cast(float, (bits & 0x807fffffu) | 0x3f800000u);
-        e[h] = exponent == 128 ? 0.0f : (float)max(exponent, -100);
+        for (int h = 0; h < kTiles; h++) {
+          const int exponent = (int)(__builtin_bit_cast(uint32_t, value_scale[h]) >> 23 & 255) - 127;
+          const float e = exponent == 128 ? 0.0f : (float)max(exponent, -100);  // (an infinity or NaN)
+          float of_tile = x[4 * h];
+#pragma unroll
+          for (int j = 1; j < 4; j++) of_tile = fmaxf(of_tile, x[4 * h + j]);
+          most = fmaxf(most, of_tile + e);
+          if (page[h] < 0) value_scale[h] = 0.0f;  // (whatever is there)
+        }
+      } else {
+        most = x[0];
+#pragma unroll
+        for (int j = 1; j < kKeys; j++) most = fmaxf(most, x[j]);
       }
-      float most = kScales ? x[0] + e[0] : x[0];
-#pragma unroll
-      for (int j = 1; j < kKeys; j++) most = fmaxf(most, kScales ? x[j] + e[j >> 2] : x[j]);
       most = column_max(most);
       if (__any(most > m_run)) {
         const float m_new = fmaxf(m_run, most);
@@ -575,8 +580,12 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(const PagedAttn
 #pragma unroll
       for (int j = 0; j < kKeys; j++) {
         float p = __builtin_amdgcn_exp2f(x[j] - m_use);
-        l_part += kScales ? p * kUnbias : p;
-        if (kScales) p = part[j >> 2] * __builtin_amdgcn_exp2f((x[j] - m_use) + e[j >> 2]);
+        if (kScales) {
+          l_part = fmaf(p, kUnbias, l_part);
+          p *= value_scale[j >> 2];
+        } else {
+          l_part += p;
+        }
         const uint32_t hi = part_bits<CT>(p), lo = part_bits<CT>(p - part_value<CT>(hi));
         pb[j] = rest ? lo : hi;
       }
