@@ -352,16 +352,131 @@ __device__ __forceinline__ int find(const int *at, int n, int i) {
 }
 
 // The entries of all sequences' ranges lie end to end, thread after thread, so
-// that one count over them ranks them all.
+// that one count over them ranks them all: f(j, index) says whether one counts,
+// g(j, whether, rank) has what becomes of it.
+struct RankShared {
+  int counts[kOneAtOnce][kOneWaves];
+};
+template <class F, class G>
+__device__ __forceinline__ int ranked(RankShared &sh, int n, F f, G g) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  int total = 0;
+  for (int i0 = 0; i0 < n; i0 += kOneThreads * kOneAtOnce) {
+    uint64_t mask[kOneAtOnce];
+#pragma unroll
+    for (int j = 0; j < kOneAtOnce; j++) mask[j] = __ballot(i0 + j * kOneThreads + tid < n && f(j, i0 + j * kOneThreads + tid));
+    __syncthreads();
+    if (lane == 0) {
+#pragma unroll
+      for (int j = 0; j < kOneAtOnce; j++) sh.counts[j][wave] = __popcll(mask[j]);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kOneAtOnce; j++) {
+      int rank = total + __popcll(mask[j] & ((1ull << lane) - 1));
+#pragma unroll
+      for (int w = 0; w < kOneWaves; w++) {
+        rank += w < wave ? sh.counts[j][w] : 0;
+        total += sh.counts[j][w];
+      }
+      if (i0 + j * kOneThreads + tid < n) g(j, (mask[j] >> lane & 1) != 0, rank);
+    }
+  }
+  return total;
+}
+
+// All sequences' pages onto the stack of `before`; sh_back: where their ranges
+// begin among `back` entries.  The entries of the stack with them.
+__device__ __forceinline__ int give_all_back(const PagePlanArgs &a, RankShared &sh, const int *sh_back, int back, int before) {
+  if (back == 0) return before;
+  int *at[kOneAtOnce];
+  int entry[kOneAtOnce];
+  const int n = ranked(
+      sh, back,
+      [&](int j, int i) {
+        const int s = find(sh_back, a.sequences, i);
+        at[j] = a.pages + (int64_t)s * a.width + (i - sh_back[s]);
+        entry[j] = *at[j];
+        return page_or_none(entry[j], a.page_count) >= 0;
+      },
+      [&](int j, bool named, int rank) {
+        if (named && rank < a.page_count - before) a.free[before + rank] = entry[j];
+        if (entry[j] != -1) *at[j] = -1;
+      });
+  __syncthreads();  // (the stack and the table are read next)
+  return min(n, a.page_count - before) + before;
+}
+
+// One token each: a sequence's thread has its position, its page and its row.
+__global__ __launch_bounds__(kOneThreads) void plan_step_kernel(const PagePlanArgs a) {
+  __shared__ RankShared sh;
+  __shared__ int sh_back[kOneThreads], sh_sum[kOneWaves], sh_more[kOneWaves];
+  __shared__ int sh_free;  // (read by the thread that writes it in the end)
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const uint64_t below = (1ull << lane) - 1;
+  PlanSpan p = {0, 0, 0, 0, 0};
+  if (tid < a.sequences) p = span_of(a, tid);
+  // the position's entry, read ahead of what goes back
+  const int i = p.old >> a.page_shift;
+  int *entry = a.pages + (int64_t)tid * a.width + i;
+  const bool has = p.fresh > 0 && i < a.width;
+  int page = has ? page_or_none(*entry, a.page_count) : -1;
+  page = i < p.back ? -1 : page;
+  const uint32_t back_to = wave_scan((uint32_t)p.back);
+  const uint64_t rows = __ballot(p.fresh > 0);
+  if (tid == 0) sh_free = free_before(a);
+  if (lane == 63) sh_sum[wave] = (int)back_to;
+  if (lane == 0) sh_more[wave] = __popcll(rows);
+  __syncthreads();
+  int back_at = (int)back_to - p.back, back = 0, row_at = __popcll(rows & below), row_all = 0;
+#pragma unroll
+  for (int w = 0; w < kOneWaves; w++) {
+    back_at += w < wave ? sh_sum[w] : 0;
+    back += sh_sum[w];
+    row_at += w < wave ? sh_more[w] : 0;
+    row_all += sh_more[w];
+  }
+  sh_back[tid] = back_at;
+  __syncthreads();
+  const int top = give_all_back(a, sh, sh_back, back, sh_free);
+
+  const bool want = has && p.first < p.last && page < 0;
+  const uint64_t wants = __ballot(want);
+  if (lane == 0) sh_sum[wave] = __popcll(wants);
+  __syncthreads();
+  int rank = __popcll(wants & below), wanted = 0;
+#pragma unroll
+  for (int w = 0; w < kOneWaves; w++) {
+    rank += w < wave ? sh_sum[w] : 0;
+    wanted += sh_sum[w];
+  }
+  if (want) {
+    page = rank < top ? page_or_none(a.free[top - 1 - rank], a.page_count) : -1;
+    *entry = page;
+  }
+  if (tid < a.sequences) {
+    const int64_t length = (int64_t)p.old + p.fresh;
+    a.lengths_out[tid] = (int)(length < 0x7fffffff ? length : 0x7fffffff);
+    if (a.missing) a.missing[tid] = want && page < 0;
+    if (a.offsets) a.offsets[tid] = row_at;
+  }
+  if (tid < a.rows) put_row(a, tid, p.fresh > 0 ? tid : -1, p.old, page);
+  if (tid == 0) {
+    if (a.offsets) a.offsets[a.sequences] = row_all;
+    *a.free_count = wanted < top ? top - wanted : 0;
+  }
+}
+
+// Any number of tokens each.
 __global__ __launch_bounds__(kOneThreads) void plan_one_kernel(const PagePlanArgs a) {
   __shared__ uint64_t sh_scan[kOneWaves][2];
   __shared__ int sh_old[kOneThreads], sh_first[kOneThreads], sh_back[kOneThreads], sh_want[kOneThreads],
       sh_rows[kOneThreads + 1], sh_missing[kOneThreads];
-  __shared__ int sh_counts[kOneAtOnce][kOneWaves];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, S = a.sequences;
+  __shared__ RankShared sh;
+  __shared__ int sh_free;
+  const int tid = threadIdx.x, S = a.sequences;
   PlanSpan p = {0, 0, 0, 0, 0};
   if (tid < S) p = span_of(a, tid);
-  int top = min(max(*a.free_count, 0), a.page_count);
   const int fresh = (int)(p.fresh > 0x7fffffff ? 0x7fffffff : p.fresh);
   uint64_t before[2], all[2];
   block_scan((uint64_t)(uint32_t)p.back << 32 | (uint32_t)(p.last - p.first), (uint32_t)fresh, sh_scan, before, all);
@@ -373,62 +488,16 @@ __global__ __launch_bounds__(kOneThreads) void plan_one_kernel(const PagePlanArg
   sh_rows[tid] = (int)(row_at < 0x7fffffff ? row_at : 0x7fffffff);
   if (tid == 0) sh_rows[S] = (int)(tokens < 0x7fffffff ? tokens : 0x7fffffff);
   sh_missing[tid] = 0;
+  if (tid == 0) sh_free = free_before(a);
   __syncthreads();
 
-  // Ranks of the entries of one kind: f(index) says whether one counts, g(index,
-  // rank) has what becomes of it.
-  auto ranked = [&](int n, auto f, auto g) {
-    int total = 0;
-    for (int i0 = 0; i0 < n; i0 += kOneThreads * kOneAtOnce) {
-      uint64_t mask[kOneAtOnce];
-#pragma unroll
-      for (int j = 0; j < kOneAtOnce; j++) mask[j] = __ballot(i0 + j * kOneThreads + tid < n && f(j, i0 + j * kOneThreads + tid));
-      __syncthreads();
-      if (lane == 0) {
-#pragma unroll
-        for (int j = 0; j < kOneAtOnce; j++) sh_counts[j][wave] = __popcll(mask[j]);
-      }
-      __syncthreads();
-#pragma unroll
-      for (int j = 0; j < kOneAtOnce; j++) {
-        int rank = total + __popcll(mask[j] & ((1ull << lane) - 1));
-#pragma unroll
-        for (int w = 0; w < kOneWaves; w++) {
-          rank += w < wave ? sh_counts[j][w] : 0;
-          total += sh_counts[j][w];
-        }
-        if (i0 + j * kOneThreads + tid < n) g(j, (mask[j] >> lane & 1) != 0, rank);
-      }
-    }
-    return total;
-  };
-
-  const int back = (int)(ranges >> 32), want = (int)(uint32_t)ranges;
-  if (back > 0) {
-    int *at[kOneAtOnce];
-    int entry[kOneAtOnce];
-    const int before = top;
-    const int n = ranked(
-        back,
-        [&](int j, int i) {
-          const int s = find(sh_back, S, i);
-          at[j] = a.pages + (int64_t)s * a.width + (i - sh_back[s]);
-          entry[j] = *at[j];
-          return page_or_none(entry[j], a.page_count) >= 0;
-        },
-        [&](int j, bool named, int rank) {
-          if (named && rank < a.page_count - before) a.free[before + rank] = entry[j];
-          if (entry[j] != -1) *at[j] = -1;
-        });
-    top = min(n, a.page_count - before) + before;
-    __syncthreads();  // (the stack and the table are read next)
-  }
+  const int want = (int)(uint32_t)ranges, top = give_all_back(a, sh, sh_back, (int)(ranges >> 32), sh_free);
   int wanted = 0;
   if (want > 0) {
     int *at[kOneAtOnce];
     int seq[kOneAtOnce];
     wanted = ranked(
-        want,
+        sh, want,
         [&](int j, int i) {
           const int s = find(sh_want, S, i);
           seq[j] = s;
@@ -454,10 +523,9 @@ __global__ __launch_bounds__(kOneThreads) void plan_one_kernel(const PagePlanArg
     if (a.offsets) a.offsets[S] = sh_rows[S];
   }
   for (int t = tid; t < a.rows; t += kOneThreads) {
-    int s = t;
-    if (a.fresh) s = t < sh_rows[S] ? find(sh_rows, S, t) : S;
-    const bool is = s < S && (a.fresh || sh_rows[s + 1] > sh_rows[s]);
-    const int64_t p = is ? (int64_t)sh_old[s] + (a.fresh ? t - sh_rows[s] : 0) : 0;
+    const int s = t < sh_rows[S] ? find(sh_rows, S, t) : S;
+    const bool is = s < S;
+    const int64_t p = is ? (int64_t)sh_old[s] + t - sh_rows[s] : 0;
     put_row(a, t, is ? s : -1, p, is ? page_at(a, s, p) : -1);
   }
 }
@@ -476,10 +544,14 @@ size_t page_plan_scratch_bytes(const PagePlanArgs &a) {
 hipError_t launch_page_plan(const PagePlanArgs &a, void *scratch, hipStream_t s) {
   if (a.sequences < 1 || a.width < 1 || a.page_count < 1 || (!scratch && page_plan_launches(a) > 1) || (!a.fresh && a.rows > a.sequences))
     return hipErrorInvalidValue;
-  // one launch where one workgroup has a few turns of work (201 sequences, some 45
-  // entries of each to look through: 9.3 us a call, 18.6 in several launches)
+  // one launch where one workgroup has a few turns of work (a token each of 201
+  // sequences, 2700 entries to look through: 6.3 us a call, in several launches 18.6;
+  // as one of several tokens 8.9)
   if (page_plan_launches(a) == 1) {
-    hipLaunchKernelGGL(plan_one_kernel, dim3(1), dim3(kOneThreads), 0, s, a);
+    if (a.fresh)
+      hipLaunchKernelGGL(plan_one_kernel, dim3(1), dim3(kOneThreads), 0, s, a);
+    else
+      hipLaunchKernelGGL(plan_step_kernel, dim3(1), dim3(kOneThreads), 0, s, a);
     return hipGetLastError();
   }
   PlanState *st = static_cast<PlanState *>(scratch);

@@ -704,7 +704,7 @@ int32_t hp_hip_logit_rules_device(const hp_hip_logit_rules_t *rules, void *strea
 typedef struct hp_hip_page_plan {
   int32_t *d_pages;              /* [sequence_count][pages_per_sequence] */
   const int32_t *d_lengths;      /* [sequence_count]; below 1: empty */
-  const int32_t *d_new_tokens;   /* [sequence_count]; NULL: one for each sequence that has tokens, as row s */
+  const int32_t *d_new_tokens;   /* [sequence_count]; NULL: one for each sequence that has tokens and is not over, as row s */
   const int32_t *d_keep_from;    /* [sequence_count]; NULL: no page goes back */
   int32_t *d_lengths_out;        /* [sequence_count] */
   int32_t *d_free, *d_free_count; /* [page_count], [1] */
@@ -783,7 +783,8 @@ int32_t hp_hip_block_select_device(const hp_hip_paged_cache_t *cache, const hp_h
  * which the first d_counts count (NULL: all; others than the sequence's blocks
  * are left out); a block named twice counts twice.  sliding_window is 0 with it.
  * Bounds are not used here.  Products are exact to some 2^-22 of the largest
- * (bf16 pages 2^-16); a NaN scale makes NaN what its block has weight in. */
+ * (bf16 pages 2^-16); the outputs of every head that attends to a block of a NaN
+ * scale are NaN. */
 int32_t hp_hip_block_attention_device(const hp_hip_paged_cache_t *cache, const hp_hip_cache_blocks_t *blocks,
                                       const hp_hip_paged_attention_t *attention, const int32_t *d_selected,
                                       const int32_t *d_counts, int32_t budget, void *stream);
