@@ -288,7 +288,25 @@ __global__ __launch_bounds__(kThreads) void plan_deal_kernel(const PagePlanArgs 
   const int t0 = ((blockIdx.x - deals) * kWaves + (threadIdx.x >> 6)) * 64 * kRowsEach, lane = threadIdx.x & 63;
   if (t0 >= a.rows) return;
   int at = a.fresh ? packed_sequence_of(offsets, a.sequences, t0) : 0;
+  // the place of row t of sequence s
+  auto put = [&](int t, int s, const PlanRow &r, int want_at, int offset) {
+    const int fresh = r.fresh & ~kNamed;
+    const int64_t p = (int64_t)(r.old & ~kGaps) + (a.fresh ? t - offset : 0), i = p >> a.page_shift;
+    const int first = plan_span(r.old & ~kGaps, 0, 0, a.page_shift, a.width).first;
+    // (one load, of the table or of the stack)
+    const int64_t from = (int64_t)st->free_with - 1 - (uint32_t)want_at - (i - first);
+    const bool in_table = (r.fresh & kNamed) != 0 || i < first, there = i < a.width && (in_table || from >= 0);
+    const int *entry = in_table ? a.pages + (int64_t)s * a.width + i : a.free + from;
+    const int page = there && fresh > 0 ? page_or_none(*entry, a.page_count) : -1;
+    if (!(r.old & kGaps) && t < a.rows) put_row(a, t, fresh > 0 ? s : -1, p, page);  // (gaps: the dealing wave's)
+  };
+  if (a.fresh && at < a.sequences && offsets[at + 1] >= min(t0 + 64 * kRowsEach, a.rows)) {  // mostly: one sequence's
+    const PlanRow r = rows_of(st)[at];
+    const int want_at = places[at].want, offset = offsets[at];
 #pragma unroll
+    for (int j = 0; j < kRowsEach; j++) put(t0 + 64 * j + lane, at, r, want_at, offset);
+    return;
+  }
   for (int j = 0; j < kRowsEach; j++) {
     const int t = t0 + 64 * j + lane;
     if (t >= a.rows) continue;
@@ -297,23 +315,10 @@ __global__ __launch_bounds__(kThreads) void plan_deal_kernel(const PagePlanArgs 
       at = sequence_from(a, offsets, at, t);
       s = at;
     }
-    const PlanRow r = rows_of(st)[min(s, a.sequences - 1)];
-    const bool named = (r.fresh & kNamed) != 0;
-    if (s >= a.sequences || (r.fresh & ~kNamed) == 0) {
+    if (s < a.sequences)
+      put(t, s, rows_of(st)[s], places[s].want, offsets[s]);
+    else
       put_row(a, t, -1, 0, -1);
-      continue;
-    }
-    if (r.old & kGaps) continue;  // (the dealing wave's)
-    const int64_t p = (int64_t)r.old + (a.fresh ? t - offsets[s] : 0), i = p >> a.page_shift;
-    const int first = plan_span(r.old, 0, 0, a.page_shift, a.width).first;
-    int page = -1;
-    if (named || i < first) {
-      page = page_at(a, s, p);
-    } else if (i < a.width) {
-      const int64_t from = (int64_t)st->free_with - 1 - (uint32_t)places[s].want - (i - first);
-      page = from >= 0 ? page_or_none(a.free[from], a.page_count) : -1;
-    }
-    put_row(a, t, s, p, page);
   }
 }
 
