@@ -105,4 +105,19 @@ HP_PAGES_FN PlanSpan plan_span(int length, int64_t fresh, int keep_from, int pag
   return p;
 }
 
+// The other pages that the new tokens lie in: entry `begun` of the table (-1:
+// none), whose first positions are older, and `beyond` that are past its end.
+struct PlanRest {
+  int begun, beyond;
+};
+HP_PAGES_FN PlanRest plan_rest(int old, int64_t fresh, int page_shift, int width) {
+  PlanRest r = {-1, 0};
+  if (fresh <= 0) return r;
+  const int64_t page = (int64_t)1 << page_shift, end = ((int64_t)old + fresh + page - 1) >> page_shift;
+  const int first = old >> page_shift;
+  if ((old & (page - 1)) != 0 && first < width) r.begun = first;
+  if (end > width) r.beyond = (int)(end - (first > width ? first : width));
+  return r;
+}
+
 }  // namespace hp

@@ -7,6 +7,9 @@
 // each sequence, their sums over the sequences before it, and copies:
 //   stack = free[0 .. f) ++ (named entries given back),  T = its size
 //   entry of rank r among those wanted: stack[T - 1 - r], -1 from r = T on
+// A page that was begun without one gets none, since its first positions are not
+// in the cache; it is among those missing as long as new tokens lie in it, as what
+// lies past the table's end is.
 // and the outcome does not depend on which workgroup comes first.
 #include "hp_serving.h"
 #include "hp_wave.h"
@@ -207,16 +210,25 @@ __device__ __forceinline__ int page_at(const PagePlanArgs &a, int s, int64_t p) 
   return i < a.width ? page_or_none(a.pages[(int64_t)s * a.width + i], a.page_count) : -1;
 }
 
+// Pages that a sequence's new tokens lie in and lack, other than the new ones.
+__device__ __forceinline__ int missing_of(const PagePlanArgs &a, int s, int old, int64_t fresh) {
+  const PlanRest r = plan_rest(old, fresh, a.page_shift, a.width);
+  const bool begun = r.begun >= 0 && page_or_none(a.pages[(int64_t)s * a.width + r.begun], a.page_count) < 0;
+  return r.beyond + begun;
+}
+
 // One sequence's new pages off the stack, by a wave; where some entries have
 // theirs already, its rows too.
 __device__ __forceinline__ void deal(const PagePlanArgs &a, const PlanState *st, const int *offsets, PlanRow r, int want_at, int s) {
   const int lane = threadIdx.x & 63;
   const bool gaps = (r.old & kGaps) != 0, named = (r.fresh & kNamed) != 0;
+  r.old &= ~kGaps;
+  r.fresh &= ~kNamed;
+  const int rest = lane == 63 && a.missing ? missing_of(a, s, r.old, r.fresh) : 0;
   if (named) {
-    if (lane == 63 && a.missing) a.missing[s] = 0;
+    if (lane == 63 && a.missing) a.missing[s] = rest;
     return;
   }
-  r.old &= ~kGaps;
   const PlanSpan p = plan_span(r.old, r.fresh, 0, a.page_shift, a.width);
   int *table = a.pages + (int64_t)s * a.width;
   int64_t at = (int64_t)st->free_with - 1 - (uint32_t)want_at;
@@ -242,7 +254,7 @@ __device__ __forceinline__ void deal(const PagePlanArgs &a, const PlanState *st,
     }
   }
   const uint64_t all = wave_scan((uint64_t)(uint32_t)missing);
-  if (lane == 63 && a.missing) a.missing[s] = (int)all;
+  if (lane == 63 && a.missing) a.missing[s] = (int)all + rest;
   if (!gaps || a.rows == 0) return;
   __threadfence_block();  // (the wave's own entries)
   const int row0 = a.fresh ? offsets[s] : s;
@@ -462,7 +474,7 @@ __global__ __launch_bounds__(kOneThreads) void plan_step_kernel(const PagePlanAr
   if (tid < a.sequences) {
     const int64_t length = (int64_t)p.old + p.fresh;
     a.lengths_out[tid] = (int)(length < 0x7fffffff ? length : 0x7fffffff);
-    if (a.missing) a.missing[tid] = want && page < 0;
+    if (a.missing) a.missing[tid] = p.fresh > 0 && page < 0;
     if (a.offsets) a.offsets[tid] = row_at;
   }
   if (tid < a.rows) put_row(a, tid, p.fresh > 0 ? tid : -1, p.old, page);
@@ -520,7 +532,7 @@ __global__ __launch_bounds__(kOneThreads) void plan_one_kernel(const PagePlanArg
   if (tid < S) {
     const int64_t length = (int64_t)p.old + fresh;
     a.lengths_out[tid] = (int)(length < 0x7fffffff ? length : 0x7fffffff);
-    if (a.missing) a.missing[tid] = sh_missing[tid];
+    if (a.missing) a.missing[tid] = sh_missing[tid] + missing_of(a, tid, p.old, fresh);
     if (a.offsets) a.offsets[tid] = sh_rows[tid];
   }
   if (tid == 0) {

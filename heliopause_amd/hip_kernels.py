@@ -865,7 +865,7 @@ def page_plan_device(sequence_count: int, pages_per_sequence: int, page_size: in
                      d_sequences: int = 0, d_positions: int = 0, d_slots: int = 0, stream: int = 0) -> None:
     """A step's page tables, lengths, row offsets and slot maps from the requests' lengths (d_new_tokens 0: one token
     for each sequence that has tokens): pages that are no longer needed go back on the stack of free ones, new ones come
-    off it."""
+    off it.  d_missing: the pages that a sequence's new tokens lie in and lack."""
     p = HipPagePlan(d_pages, d_lengths, d_new_tokens, d_keep_from, d_lengths_out, d_free, d_free_count, d_offsets,
                     d_missing, d_sequences, d_positions, d_slots, token_count, sequence_count, pages_per_sequence,
                     page_size, page_count)

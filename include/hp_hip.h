@@ -690,17 +690,25 @@ int32_t hp_hip_logit_rules_device(const hp_hip_logit_rules_t *rules, void *strea
  *   - the new tokens' pages, those all of whose positions are new and whose entry
  *     names no page, are dealt, in order of sequence and position.  When there
  *     is none left they stay -1: rows appended there are dropped and their
- *     positions left out of the attention; d_missing[s] counts them;
+ *     positions left out of the attention.  A page that was begun before gets
+ *     none, since its first positions would not be in it;
+ *   - d_missing[s] is the number of pages that the sequence's new tokens lie in
+ *     and lack, begun ones and those past the table's end among them: 0 where
+ *     each of these tokens has its slot.  It is each step's own: it says nothing
+ *     of rows that were dropped in the steps before;
  *   - d_lengths_out[s] (may be d_lengths) is the length with the new tokens,
  *     d_offsets the sums of the new tokens (the packed rows of
  *     hp_hip_paged_append_device), and row t of the maps is the t-th new token:
  *     its sequence, position, and slot page * page_size + position % page_size.
  *     Rows behind the last are -1, a slot without a page too.
  * A step that lacks pages can be taken again once some are free: with the
- * lengths as they were, pages dealt before are found in the table.  A page that
- * two rows of the table name must not go back through both; the stack holds
- * d_free's page_count entries at most, what goes back beyond is lost.  Up to four
- * launches, over scratch of the stream's; one where it is small. */
+ * lengths as they were, pages dealt before are found in the table.  Steps on
+ * from it cannot mend it: the sequence goes back to where the page begins (a
+ * length that is a multiple of page_size), with the tokens from there on as new
+ * ones.  A page that two rows of the table name must not go back through both;
+ * the stack holds d_free's page_count entries at most, what goes back beyond is
+ * lost.  Up to four launches, over scratch of the stream's; one where it is
+ * small. */
 typedef struct hp_hip_page_plan {
   int32_t *d_pages;              /* [sequence_count][pages_per_sequence] */
   const int32_t *d_lengths;      /* [sequence_count]; below 1: empty */

@@ -40,7 +40,8 @@ def plan(pages, lengths, new, keep, free, free_count, page_size, page_count, row
             if not named(pages[s, i]):
                 entry = stack.pop() if stack else -1
                 pages[s, i] = entry if named(entry) else -1
-                missing[s] += pages[s, i] < 0
+        if fresh[s]:  # the pages that the new tokens lie in
+            missing[s] = sum(i >= W or not named(pages[s, i]) for i in range(old[s] // page_size, -(-int(after[s]) // page_size)))
     free[:len(full)] = full
     maps = np.full((3, rows), -1, np.int64)
     for s in range(S):
