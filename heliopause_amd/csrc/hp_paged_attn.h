@@ -179,6 +179,20 @@ __device__ __forceinline__ float row_scale(float m, float l, float value_scale) 
   return m == kNegInf && l == 0.0f ? 0.0f : l == 0.0f ? __builtin_nanf("") : value_scale / l;
 }
 
+// 2^d, for a part's sums whose maximum is 2^d of the others'.  Under scales the
+// sum l of a row's weights lies within 2^-100 and 2^100 n of its maximum's, whose
+// scale counts there, and one maximum may be 2^200 above the next: 2^d by itself is
+// 0 then, where its product with l is not, and l takes its root twice.
+template <int MODE>
+struct Exp2 {
+  float root, all;
+  __device__ __forceinline__ explicit Exp2(float d) {
+    root = (MODE & kScaled) ? __builtin_amdgcn_exp2f(0.5f * d) : 0.0f;
+    all = (MODE & kScaled) ? root * root : __builtin_amdgcn_exp2f(d);
+  }
+  __device__ __forceinline__ float of_sum(float l) const { return (MODE & kScaled) ? l * root * root : l * all; }
+};
+
 // A lane's elements of a key row of each tile (D / 32 operand fragments) and of
 // the four value rows of each (D / 16 elements each), as loaded.
 template <int D, int CT>
@@ -563,11 +577,11 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(const PagedAttn
       most = column_max(most);
       if (__any(most > m_run)) {
         const float m_new = fmaxf(m_run, most);
-        const float alpha = m_new == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_new);
+        const Exp2<MODE> alpha(m_new == kNegInf ? 0.0f : m_run - m_new);
         m_run = m_new;
-        l_part *= alpha;
+        l_part = alpha.of_sum(l_part);
 #pragma unroll
-        for (int i = 0; i < kT; i++) acc[i] *= alpha;
+        for (int i = 0; i < kT; i++) acc[i] *= alpha.all;
       }
       // a row without a key so far: exp2(-inf - 0) = 0.  From 2^27 on f32's steps
       // are as large as the bias, and what is left of it could be more: 2^16 is
@@ -662,9 +676,11 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(const PagedAttn
       float l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int w = 0; w < kWaves; w++) {
-        const float mw = sh_m[w][h], f = mw == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(mw - m);
+        const float mw = sh_m[w][h];
+        const Exp2<MODE> e(mw == kNegInf ? kNegInf : mw - m);
+        const float f = e.all;
         const float4 v = sh_o[w][h][d];
-        l += f * sh_l[w][h];
+        l += e.of_sum(sh_l[w][h]);
         o[0] += f * v.x;
         o[1] += f * v.y;
         o[2] += f * v.z;
@@ -732,15 +748,16 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(const PagedAttnAr
       if (c0 + i * kAtOnce > r.last) mc[i] = kNegInf;
       m_new = fmaxf(m_new, mc[i]);
     }
-    const float f = m == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(m - m_new);
-    l *= f;
+    const Exp2<MODE> f(m == kNegInf ? kNegInf : m - m_new);
+    l = f.of_sum(l);
 #pragma unroll
-    for (int j = 0; j < 4; j++) o[j] *= f;
+    for (int j = 0; j < 4; j++) o[j] *= f.all;
 #pragma unroll
     for (int i = 0; i < kDeep; i++) {
       if (c0 + i * kAtOnce > r.last) continue;
-      const float g = mc[i] == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(mc[i] - m_new);
-      l += lc[i] * g;
+      const Exp2<MODE> e(mc[i] == kNegInf ? kNegInf : mc[i] - m_new);
+      const float g = e.all;
+      l += e.of_sum(lc[i]);
       o[0] += v[i].x * g;
       o[1] += v[i].y * g;
       o[2] += v[i].z * g;
@@ -761,9 +778,10 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(const PagedAttnAr
   l = o[0] = o[1] = o[2] = o[3] = 0.0f;
 #pragma unroll
   for (int c = 0; c < kAtOnce; c++) {
-    const float f = sh_m[c] == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(sh_m[c] - most);
+    const Exp2<MODE> e(sh_m[c] == kNegInf ? kNegInf : sh_m[c] - most);
+    const float f = e.all;
     const float4 v = sh_o[c][d];
-    l += f * sh_l[c];
+    l += e.of_sum(sh_l[c]);
     o[0] += f * v.x;
     o[1] += f * v.y;
     o[2] += f * v.z;
@@ -784,7 +802,7 @@ hipError_t launch_kernels(const PagedAttnArgs &a, int groups, hipStream_t s) {
                      parts, groups);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL((paged_merge_kernel<D, MODE & kSelected>), dim3(a.nq, a.c.sequences), dim3(kThreads), 0, s, a,
+  hipLaunchKernelGGL((paged_merge_kernel<D, MODE>), dim3(a.nq, a.c.sequences), dim3(kThreads), 0, s, a,
                      row_parts, parts, groups);
   return hipGetLastError();
 }
