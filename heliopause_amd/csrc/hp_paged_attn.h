@@ -109,12 +109,28 @@ __device__ __forceinline__ KeySpan span_of(const PagedAttnArgs &a, int row) {
 // Heads of a KV head's group in blocks of kHeads: rows of a sequence.
 __host__ __device__ __forceinline__ int blocks_of(int nq, int nkv) { return (nq / nkv + kHeads - 1) / kHeads; }
 
-// A part of a row: m and l of its heads, then the unnormalised sums.
+// A part of a row: m and l of its heads, then the unnormalised sums; with scales
+// what is left of m.
 template <int D>
-struct Part {
+struct PartSums {
   float m[kHeads], l[kHeads];
   float o[kHeads][D];
 };
+template <bool SCALED>
+struct PartLow {};
+template <>
+struct PartLow<true> {
+  float low[kHeads];
+};
+template <int D, int MODE>
+struct Part : PartSums<D>, PartLow<(MODE & kScaled) != 0> {};
+// How far a maximum is from 2^24, in steps of f32: below kFar where it is that
+// large (and finite), so that f32's steps are more than one and a scale's exponent
+// needs `low`; other maxima have 0 there.
+constexpr uint32_t kFar = 0x7f800000u - 0x4b800000u;
+__device__ __forceinline__ uint32_t distance_of(float m) {
+  return (__builtin_bit_cast(uint32_t, m) & 0x7fffffffu) - 0x4b800000u;
+}
 struct RowParts {
   int first, last;  // workgroups that hold the row's parts (the same: none)
 };
@@ -226,14 +242,15 @@ __device__ __forceinline__ void load_words(uint32_t (&d)[N], const uint8_t *p) {
 
 template <int D, int CT, int MODE, bool THIRD, bool STREAM>
 __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(const PagedAttnArgs a, RowParts *__restrict__ rows,
-                                                                 Part<D> *__restrict__ parts, int groups) {
+                                                                 Part<D, MODE> *__restrict__ parts, int groups) {
   using T = Tile<D, CT>;
   constexpr int kTiles = T::kTiles, kKeys = T::kKeys, kSub = 16 * kTiles, kStep = kSub * kWaves;
   constexpr int kE = T::kE, kFrags = D / 32, kRowBytes = D * kE, kT = D / 16;
   constexpr bool kList = (MODE & kSelected) != 0, kScales = (MODE & kScaled) != 0;
   __shared__ float4 sh_o[kWaves][kHeads][D / 4];
   __shared__ u32x4 sh_q[THIRD ? 2 : 1][kFrags][64];  // the query's operand fragments, the same for every wave
-  __shared__ float sh_m[kWaves][kHeads], sh_l[kWaves][kHeads];
+  __shared__ float sh_m[kWaves][kHeads], sh_l[kWaves][kHeads], sh_low[kScales ? kWaves : 1][kHeads];
+  __shared__ alignas(4) bool sh_far[kWaves];  // waves whose maxima have a second part
   __shared__ float sh_most[kWaves][16];  // largest elements of the query rows
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int q4 = lane >> 4, c16 = lane & 15;
@@ -317,6 +334,8 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(const PagedAttn
 #pragma unroll
     for (int t = 0; t < kT; t++) acc[t] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
     float m_run = kNegInf, l_part = 0.0f;
+    float m_low = 0.0f;  // (scales: the maximum is m_run + m_low)
+    bool far = false;    // (the same for the wave)
     bool has_key = false;  // the lane has seen a key that is not masked
 
     // this wave's tiles: key .. key + kSub - 1 at key = begin + kStep i + kSub wave
@@ -556,18 +575,26 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(const PagedAttn
       // a value scale s >= 2^e: the maximum is that of x + e, so that the weights
       // s 2^(x - m) of the stored values are within range whatever the blocks' scales
       // are.  2^(x - m) itself is at most 2^100, and below f32 only where the weight
-      // is less than 2^-26 of the largest, bias and all
+      // is less than 2^-26 of the largest, bias and all.  Where a step of x in f32 is
+      // more than one the maximum has a second part, what x + e was rounded by:
+      // without it equal scores under scales of 2^20 would weigh 2^30 (2^16 is past
+      // f16).  Scores that large take this way alone
+      auto exponent_of = [](float scale) -> float {
+        const int e = (int)(__builtin_bit_cast(uint32_t, scale) >> 23 & 255) - 127;
+        return e == 128 ? 0.0f : (float)max(e, -100);  // (an infinity or NaN)
+      };
+      auto most_of = [&](int h) -> float {
+        float v = x[4 * h];
+#pragma unroll
+        for (int j = 1; j < 4; j++) v = fmaxf(v, x[4 * h + j]);
+        return v;
+      };
       float most = kNegInf;
       if (kScales) {
 #pragma unroll
         for (int h = 0; h < kTiles; h++) {
-          const int exponent = (int)(__builtin_bit_cast(uint32_t, value_scale[h]) >> 23 & 255) - 127;
-          const float e = exponent == 128 ? 0.0f : (float)max(exponent, -100);  // (an infinity or NaN)
-          float of_tile = x[4 * h];
-#pragma unroll
-          for (int j = 1; j < 4; j++) of_tile = fmaxf(of_tile, x[4 * h + j]);
-          most = fmaxf(most, of_tile + e);
-          if (page[h] < 0) value_scale[h] = 0.0f;  // (whatever is there)
+          most = fmaxf(most, most_of(h) + exponent_of(value_scale[h]));
+          if (page[h] < 0) value_scale[h] = 0.0f;  // (whatever is there; its keys' scores are -inf)
         }
       } else {
         most = x[0];
@@ -575,9 +602,26 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(const PagedAttn
         for (int j = 1; j < kKeys; j++) most = fmaxf(most, x[j]);
       }
       most = column_max(most);
-      if (__any(most > m_run)) {
+      if (__any(most > m_run) || (kScales && far)) {
         const float m_new = fmaxf(m_run, most);
-        const Exp2<MODE> alpha(m_new == kNegInf ? 0.0f : m_run - m_new);
+        float drop = m_new == kNegInf ? 0.0f : m_run - m_new;
+        if (kScales) {
+          const bool were = far;
+          far = __any(distance_of(m_new) < kFar);
+          if (__builtin_expect(far || were, false)) {
+            float low = m_run == m_new ? m_low : kNegInf;
+#pragma unroll
+            for (int h = 0; h < kTiles; h++) {
+              const float v = most_of(h), e = exponent_of(value_scale[h]);
+              if (v + e == m_new) low = fmaxf(low, (v - (v + e)) + e);
+            }
+            low = column_max(low);
+            low = distance_of(m_new) < kFar ? low : 0.0f;
+            drop += m_low - low;
+            m_low = low;
+          }
+        }
+        const Exp2<MODE> alpha(drop);
         m_run = m_new;
         l_part = alpha.of_sum(l_part);
 #pragma unroll
@@ -588,6 +632,12 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(const PagedAttn
       // past f16
       float m_use = m_run == kNegInf ? 0.0f : m_run - kBias;
       m_use = m_run - m_use > 15.0f ? m_run : m_use;
+      if (kScales && __builtin_expect(far, false)) {
+        m_use = m_run == kNegInf ? 0.0f : m_run;
+#pragma unroll
+        for (int j = 0; j < kKeys; j++) x[j] = (x[j] - m_use) - (m_low - kBias);
+        m_use = 0.0f;
+      }
       uint32_t pf[kKeys / 2];
       const bool rest = c16 >= kHeads;
       uint32_t pb[kKeys];
@@ -654,6 +704,8 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(const PagedAttn
       if (q4 == 0) {
         sh_m[wave][c16] = m_run;
         sh_l[wave][c16] = l_run;
+        if (kScales) sh_low[kScales ? wave : 0][c16] = m_low;
+        if (kScales && c16 == 0) sh_far[wave] = far;
       }
 #pragma unroll
       for (int r = 0; r < 4; r++)
@@ -664,7 +716,9 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(const PagedAttn
     }
     __syncthreads();
     const bool whole = i0 == 0 && n == steps;
-    Part<D> *part = parts + 2 * ((int64_t)me * blocks + block) + (i0 == 0 ? 1 : 0);
+    static_assert(sizeof(sh_far) == sizeof(uint32_t), "one load");
+    const bool any_far = kScales && __builtin_amdgcn_readfirstlane((int)*reinterpret_cast<const uint32_t *>(sh_far)) != 0;
+    Part<D, MODE> *part = parts + 2 * ((int64_t)me * blocks + block) + (i0 == 0 ? 1 : 0);
     if (i0 == 0 && tid == 0) {
       rows[((int64_t)line * units + unit) * blocks + block] = RowParts{(int)me, (int)share_of(total, row_start + steps - 1, shares)};
     }
@@ -673,11 +727,19 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(const PagedAttn
       float m = kNegInf;
 #pragma unroll
       for (int w = 0; w < kWaves; w++) m = fmaxf(m, sh_m[w][h]);
+      float low = 0.0f;
+      if (__builtin_expect(any_far, false)) {
+        low = kNegInf;
+#pragma unroll
+        for (int w = 0; w < kWaves; w++) low = sh_m[w][h] == m ? fmaxf(low, sh_low[kScales ? w : 0][h]) : low;
+      }
       float l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int w = 0; w < kWaves; w++) {
         const float mw = sh_m[w][h];
-        const Exp2<MODE> e(mw == kNegInf ? kNegInf : mw - m);
+        float below = mw == kNegInf ? kNegInf : mw - m;
+        if (__builtin_expect(any_far, false)) below += sh_low[kScales ? w : 0][h] - low;
+        const Exp2<MODE> e(below);
         const float f = e.all;
         const float4 v = sh_o[w][h][d];
         l += e.of_sum(sh_l[w][h]);
@@ -697,6 +759,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(const PagedAttn
         if (d == 0) {
           part->m[h] = m;
           part->l[h] = l;
+          if constexpr (kScales) part->low[h] = low;
         }
       }
     }
@@ -709,9 +772,11 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(const PagedAttn
 // l_c with f = 2^(m_c - m); D / 4 threads a part, several parts at once.
 template <int D, int MODE>
 __global__ __launch_bounds__(kThreads) void paged_merge_kernel(const PagedAttnArgs a, const RowParts *__restrict__ rows,
-                                                               const Part<D> *__restrict__ parts, int groups) {
+                                                               const Part<D, MODE> *__restrict__ parts, int groups) {
   constexpr int kPer = D / 4, kAtOnce = kThreads / kPer;
+  constexpr bool kScales = (MODE & kScaled) != 0;
   __shared__ float sh_m[kAtOnce], sh_l[kAtOnce];
+  __shared__ alignas(4) bool sh_far[kWaves];
   __shared__ float4 sh_o[kAtOnce][kPer];
   const int group = a.nq / a.c.nkv, blocks = blocks_of(a.nq, a.c.nkv);
   const int head = blockIdx.x, seq = blockIdx.y;
@@ -730,6 +795,10 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(const PagedAttnAr
   }
   if (r.first >= r.last) return;  // written by the workgroup that had it whole
   float m = kNegInf, l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  auto part_of = [&](int c) -> const Part<D, MODE> & {
+    return parts[2 * ((int64_t)c * blocks + in_group / kHeads) + (c == r.first ? 1 : 0)];
+  };
+  uint32_t distance = ~0u;  // (the least of the parts')
   constexpr int kDeep = 8;  // parts that a thread has on their way
   for (int c0 = r.first + sub; c0 <= r.last; c0 += kAtOnce * kDeep) {
     float mc[kDeep], lc[kDeep];
@@ -737,7 +806,7 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(const PagedAttnAr
 #pragma unroll
     for (int i = 0; i < kDeep; i++) {
       const int c = min(c0 + i * kAtOnce, r.last);
-      const Part<D> &p = parts[2 * ((int64_t)c * blocks + in_group / kHeads) + (c == r.first ? 1 : 0)];
+      const Part<D, MODE> &p = part_of(c);
       mc[i] = p.m[h];
       lc[i] = p.l[h];
       v[i] = *reinterpret_cast<const float4 *>(&p.o[h][4 * d]);
@@ -747,6 +816,10 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(const PagedAttnAr
     for (int i = 0; i < kDeep; i++) {
       if (c0 + i * kAtOnce > r.last) mc[i] = kNegInf;
       m_new = fmaxf(m_new, mc[i]);
+    }
+    if (kScales) {
+#pragma unroll
+      for (int i = 0; i < kDeep; i++) distance = min(distance, distance_of(mc[i]));
     }
     const Exp2<MODE> f(m == kNegInf ? kNegInf : m - m_new);
     l = f.of_sum(l);
@@ -769,6 +842,7 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(const PagedAttnAr
     sh_m[sub] = m;
     sh_l[sub] = l;
   }
+  if (kScales) sh_far[tid >> 6] = __any(distance < kFar);
   sh_o[sub][d] = make_float4(o[0], o[1], o[2], o[3]);
   __syncthreads();
   if (sub != 0) return;
@@ -787,6 +861,31 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(const PagedAttnAr
     o[2] += f * v.z;
     o[3] += f * v.w;
   }
+  if constexpr (kScales) {
+    if (__builtin_expect(*reinterpret_cast<const uint32_t *>(sh_far) != 0, false)) {
+      // anew, with what is left of the maxima, one part after another
+      float low = 0.0f;
+      most = kNegInf;
+      l = o[0] = o[1] = o[2] = o[3] = 0.0f;
+#pragma unroll 1
+      for (int c = r.first; c <= r.last; c++) {
+        const Part<D, MODE> &p = part_of(c);
+        const float pm = p.m[h], pl = p.low[h];
+        const bool above = pm > most || (pm == most && pl > low);
+        const float to = above ? pm : most, to_low = above ? pl : low;
+        const Exp2<MODE> f(most == kNegInf ? kNegInf : (most - to) + (low - to_low));
+        const Exp2<MODE> g(pm == kNegInf ? kNegInf : (pm - to) + (pl - to_low));
+        const float4 v = *reinterpret_cast<const float4 *>(&p.o[h][4 * d]);
+        l = f.of_sum(l) + g.of_sum(p.l[h]);
+        o[0] = f.all * o[0] + g.all * v.x;
+        o[1] = f.all * o[1] + g.all * v.y;
+        o[2] = f.all * o[2] + g.all * v.z;
+        o[3] = f.all * o[3] + g.all * v.w;
+        most = to;
+        low = to_low;
+      }
+    }
+  }
   const float inv = row_scale(most, l, elem_bytes(a.c.type) == 1 ? a.c.value_scale : 1.0f);
 #pragma unroll
   for (int j = 0; j < 4; j++) o[j] *= inv;
@@ -795,7 +894,7 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(const PagedAttnAr
 
 template <int D, int CT, int MODE, bool THIRD, bool STREAM>
 hipError_t launch_kernels(const PagedAttnArgs &a, int groups, hipStream_t s) {
-  Part<D> *parts = reinterpret_cast<Part<D> *>(a.partials);
+  Part<D, MODE> *parts = reinterpret_cast<Part<D, MODE> *>(a.partials);
   const int blocks = blocks_of(a.nq, a.c.nkv), grid = (groups + kXcds - 1) / kXcds * kXcds * blocks;
   RowParts *row_parts = reinterpret_cast<RowParts *>(parts + 2 * (int64_t)groups * blocks);
   hipLaunchKernelGGL((paged_attn_kernel<D, CT, MODE, THIRD, STREAM>), dim3(grid), dim3(kThreads), 0, s, a, row_parts,

@@ -16,7 +16,9 @@ hipError_t launch_type(const PagedAttnArgs &a, int groups, hipStream_t s) {
                                  : launch<D, kElemBf16, kWhole, false>(a, groups, s);
 }
 
-size_t part_bytes(int head_dim) { return (size_t)kHeads * (head_dim + 2) * sizeof(float); }
+size_t part_bytes(int head_dim, bool scaled) { return (size_t)kHeads * (head_dim + 2 + scaled) * sizeof(float); }
+static_assert(sizeof(Part<64, kWhole>) == kHeads * 66 * sizeof(float) && sizeof(Part<64, kScaled>) == kHeads * 67 * sizeof(float),
+              "as the scratch has them");
 
 }  // namespace
 
@@ -38,7 +40,7 @@ int paged_attn_groups(const PagedAttnArgs &a, int num_cus) {
 
 size_t paged_attn_scratch_bytes(const PagedAttnArgs &a, int groups) {
   const size_t blocks = blocks_of(a.nq, a.c.nkv);
-  return blocks * (2 * (size_t)groups * part_bytes(a.c.head_dim) +
+  return blocks * (2 * (size_t)groups * part_bytes(a.c.head_dim, a.key_scales != nullptr) +
                    (size_t)a.c.sequences * a.c.nkv * sizeof(RowParts));
 }
 

@@ -137,3 +137,12 @@ def equal_scores(type, e, sign, D, n):
 def test_equal_scores_whatever_the_value_scales(hip, type, e, sign, D, n):
     """The sum of the weights has its share of every key, those of blocks whose scale is 2^200 below another's too."""
     equal_scores(type, e, sign, D, n)
+
+
+@pytest.mark.parametrize("type", ["i8", "e4m3"])
+@pytest.mark.parametrize("e", [24, 25, 26, 27, 28, 29, 30, 31, 33, 60])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("D,n", [(64, 100), (128, 5000), (256, 700)])
+def test_value_scales_under_large_scores(hip, type, e, sign, D, n):
+    """Scores whose steps in f32 are 2 to 2^37, so that a scale's exponent is less than a step of them."""
+    equal_scores(type, e, sign, D, n)
