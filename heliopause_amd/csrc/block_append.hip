@@ -4,11 +4,9 @@
 // magnitude among the call's rows in it
 //   i8:   s' = A (1 / 127)      e4m3: s' = the least power of two with A <= 448 s'
 // held within 2^-100 .. 2^100, and x is stored as round(x / s').  A block that
-// was begun before the call keeps its scale s while A <= M s (M = 127 (1 + 2^-22),
-// since the product with 1 / 127 may be 2^-23 below the quotient, which an element
-// as large as the one that set the scale has to pass; or 448); otherwise the scale
-// grows to s' (i8: at least 1.25 s, so that growing again and again adds less than
-// 5 half steps in all) and what it holds becomes
+// was begun before the call keeps its scale s while A <= M s (M = 127 or 448);
+// otherwise the scale grows to s' (i8: at least 1.25 s, so that growing again
+// and again adds less than 5 half steps in all) and what it holds becomes
 // round(stored * s / s').  e4m3's powers of two move its values without another
 // rounding, but for those that become subnormal.  An infinity or NaN among the
 // rows makes the block's scale NaN until the block is begun anew: 8 bits have no
@@ -342,7 +340,7 @@ __global__ __launch_bounds__(NT) void block_append_kernel(const PagedAppendArgs 
   }
   if (page < 0) return;  // rows of an absent page are dropped
 
-  constexpr float kM = CT == kElemI8 ? 0x1.fc0008p6f : 448.0f;  // 127 (1 + 2^-22)
+  constexpr float kM = stored_most<CT>();
   const bool grows = old_block && most > old * kM;
   float scale = old;
   if (!old_block || grows) scale = fresh_scale<CT>(most);

@@ -745,10 +745,9 @@ typedef struct hp_hip_cache_blocks {
  * largest magnitude among the call's rows of a block and KV head (keys and values
  * each for themselves): a block that begins with this call has the scale A * (1 / 127)
  * (i8) or the least power of two with A <= 448 scale (e4m3).  One begun before
- * keeps its scale as long as A is within it (127 scale (1 + 2^-22), so that an
- * element as large as the one that set it always is, or 448 scale); otherwise the
- * scale becomes that of A, i8's at least 1.25 times what it was, and what the block
- * holds is rounded to the new one.  Scales stay within 2^-100 .. 2^100, what is past them saturates.
+ * keeps its scale as long as A is within it; otherwise the scale becomes that of
+ * A, i8's at least 1.25 times what it was, and what the block holds is rounded to
+ * the new one.  Scales stay within 2^-100 .. 2^100, what is past them saturates.
  * An infinity or NaN makes the block's scale NaN until the block begins anew.
  * d_k_out and d_v_out have the rows before they are rounded to 8 bits.  The
  * angles' sines and cosines are f32's, of turns reduced in 64 bits. */

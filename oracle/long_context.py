@@ -65,7 +65,7 @@ def block_scale(kind, most):
 
 def grown_scale(kind, old, most):
     """The scale of a block that was begun with the scale `old`."""
-    if not most > old * (127.0 * (1 + 2.0 ** -22) if kind == "i8" else 448.0):
+    if not most > old * MOST[kind]:
         return old
     return min(max(block_scale(kind, most), 1.25 * old if kind == "i8" else 0.0), 2.0 ** 100)
 
