@@ -562,7 +562,7 @@ hipError_t launch_page_plan(const PagePlanArgs &a, void *scratch, hipStream_t s)
   if (a.sequences < 1 || a.width < 1 || a.page_count < 1 || (!scratch && page_plan_launches(a) > 1) || (!a.fresh && a.rows > a.sequences))
     return hipErrorInvalidValue;
   // one launch where one workgroup has a few turns of work (a token each of 201
-  // sequences, 2700 entries to look through: 6.3 us a call, in several launches 18.6;
+  // sequences, 2700 entries to look through: 6.4 us a call, in several launches 18.6;
   // as one of several tokens 8.9)
   if (page_plan_launches(a) == 1) {
     if (a.fresh)

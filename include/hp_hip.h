@@ -745,9 +745,10 @@ typedef struct hp_hip_cache_blocks {
  * largest magnitude among the call's rows of a block and KV head (keys and values
  * each for themselves): a block that begins with this call has the scale A * (1 / 127)
  * (i8) or the least power of two with A <= 448 scale (e4m3).  One begun before
- * keeps its scale as long as A is within it; otherwise the scale becomes that of
- * A, i8's at least 1.25 times what it was, and what the block holds is rounded to
- * the new one.  Scales stay within 2^-100 .. 2^100, what is past them saturates.
+ * keeps its scale as long as A <= 127 scale or 448 scale, by f32's product (an i8
+ * element as large as the one that set the scale may be past that by its last bit);
+ * otherwise the scale becomes that of A, i8's at least 1.25 times what it was, and
+ * what the block holds is rounded to the new one.  Scales stay within 2^-100 .. 2^100, what is past them saturates.
  * An infinity or NaN makes the block's scale NaN until the block begins anew.
  * d_k_out and d_v_out have the rows before they are rounded to 8 bits.  The
  * angles' sines and cosines are f32's, of turns reduced in 64 bits. */
@@ -757,7 +758,8 @@ int32_t hp_hip_block_append_device(const hp_hip_paged_cache_t *cache, const hp_h
 /* Forms d_key_bounds anew for every block that holds one of the new tokens, over
  * all its keys before the sequence's end: the tokens of a hp_hip_paged_append_device
  * or hp_hip_block_append_device call, with its d_offsets and token_count, once it
- * has been queued.  Bounds are rounded outward; a NaN among a block's keys counts
+ * has been queued.  A key's element here is f32's product of what is stored and
+ * the scale; bounds are rounded outward from it.  A NaN among a block's keys counts
  * as the smallest and the largest finite number. */
 int32_t hp_hip_block_bounds_device(const hp_hip_paged_cache_t *cache, const hp_hip_cache_blocks_t *blocks,
                                    const int32_t *d_offsets, size_t token_count, void *stream);
@@ -770,7 +772,7 @@ int32_t hp_hip_block_bounds_device(const hp_hip_paged_cache_t *cache, const hp_h
  * taken.  The first_blocks first and last_blocks last blocks are always taken,
  * and count.  Blocks on absent pages are not.  An infinite query element counts
  * as the largest finite number, a NaN as 0.  Two launches, over scratch of the
- * stream's. */
+ * stream's: 8 bytes for each sequence, KV head and block of a table. */
 typedef struct hp_hip_block_select {
   const void *d_q;      /* [sequence_count][head_count][head_dim] of q_type */
   size_t q_stride;      /* from sequence to sequence */
